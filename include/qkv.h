@@ -900,6 +900,88 @@ int qkv_prefill_block_scores(const int8_t* q8, int64_t batch, int64_t q_heads, i
 int qkv_prefill_block_topk(const float* bmax, int64_t rows, int64_t n, int64_t ld, int64_t k,
                            int32_t* out, void* stream);
 
+/* ======================================================================
+ * Paged K/V cache: pages of `page` tokens (a power of two in [16, 4096])
+ * that requests of different lengths take from one pool.  No reference
+ * counterpart: the reference keeps HF's dense cache, every sequence of a
+ * batch at one length (EV:7079-7111), and prefills with dense attention.
+ * ====================================================================== */
+
+/* A step's pages, slots and positions, decided on the GPU from the request
+ * lengths.  State: table int32 [requests, width] (row stride table_ld; page
+ * of a request's token t at [t / page], -1 where it holds none), lens int32
+ * [requests], and the pages no request holds, free int32 [pages] as a stack
+ * with count int32 [1] entries, top last.  The step adds new_lens[b] tokens
+ * (int32, negative read as 0) to request b:
+ *   need_b = ceil((lens_b + new_b) / page) - ceil(lens_b / page),
+ *   its k-th new page is free[count - 1 - sum_{a<b} need_a - k],
+ * and lens, table and count are updated.  A request is not served (its state
+ * stays, kv_lens 0, its rows without slots) where its tokens would not fit
+ * its table row, the stack ends before its pages, or its rows end past
+ * `rows`; failed int32 [1] receives how many with new tokens were not.
+ * Rows: request b has rows cu_rows[b] .. cu_rows[b+1]-1 (int32 [requests+1]);
+ * new_b of them where padded is 0, else `padded` each (rows = requests *
+ * padded), its tokens last.  kv_lens int32 [requests]: tokens after the
+ * step.  slots int64 [rows] = page id * page + t % page and positions int32
+ * [rows] = t of each row's token, -1 for rows without one.
+ * At most 4096 requests, 2^20 pages and 2^20 rows. */
+int qkv_paged_plan(const int32_t* new_lens, int32_t* table, int64_t table_ld, int32_t* lens, int32_t* free,
+                   int32_t* count, int64_t requests, int64_t width, int64_t pages, int64_t page, int64_t rows,
+                   int64_t padded, int32_t* cu_rows, int32_t* kv_lens, int64_t* slots, int32_t* positions,
+                   int32_t* failed, void* stream);
+
+/* Cuts every request to its first keep[b] tokens (int32; 0 ends it, lens_b
+ * and more leave it) and gives the pages behind them back, the first
+ * request's first page on top: a release of what the last step took leaves
+ * the stack as it was.  The same state as qkv_paged_plan; pages must belong
+ * to one request each. */
+int qkv_paged_release(const int32_t* keep, int32_t* table, int64_t table_ld, int32_t* lens, int32_t* free,
+                      int32_t* count, int64_t requests, int64_t width, int64_t pages, int64_t page, void* stream);
+
+/* Writes the K and V rows of a step into their pages.  key / value 16-bit
+ * [rows, kv_heads, head_dim] with strides {row, head}, channels contiguous;
+ * k_pages / v_pages [pages, kv_heads, page, head_dim] with strides {page,
+ * head, token}, rows 16-byte aligned; slots int64 [rows] as qkv_paged_plan
+ * writes them (outside [0, pages * page): the row is skipped; each slot at
+ * most once).  head_dim a multiple of 8. */
+int qkv_paged_append(const void* key, const int64_t* key_strides, const void* value, const int64_t* value_strides,
+                     void* k_pages, const int64_t* k_strides, void* v_pages, const int64_t* v_strides, int64_t pages,
+                     int64_t page, int64_t kv_heads, int64_t head_dim, const int64_t* slots, int64_t rows,
+                     void* stream);
+
+/* Bytes of workspace for qkv_paged_attention; 0 where no request can be long
+ * enough for its keys to be split, -1 for sizes it does not take. */
+int64_t qkv_paged_attention_workspace_bytes(int64_t rows, int64_t max_rows, int64_t requests, int64_t width,
+                                            int64_t page, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
+
+/* Attention of a step's rows over the cache: single tokens, drafted tokens,
+ * chunks of prompts and whole prompts, mixed as they come.  query / out
+ * [rows, q_heads, head_dim] with strides {row, head}; pages as in
+ * qkv_paged_append; table, cu_rows and kv_lens as in qkv_paged_plan.  Row i
+ * of request b is the token at p = kv_lens[b] - (cu_rows[b+1] - cu_rows[b])
+ * + i and sees the keys j with first_keys[row] <= j < max(p + 1,
+ * prefix_lens[b]), j < kv_lens[b]; a row with p < 0 or without a key gets
+ * zeros.  first_keys int32 [rows] (NULL: 0; a document's first token, or p +
+ * 1 - window) and prefix_lens int32 [requests] (NULL: 0; keys every row of
+ * the request sees).  Score: scaling * q.k, then softcap * tanh(score /
+ * softcap) where softcap > 0, then - slopes[head] * |p - j| (slopes f32
+ * [q_heads], NULL: 0).  Softmax in fp32; its weights are rounded to the
+ * dtype for the product with V.  Rows of out outside all requests are left
+ * as they were.  Keys whose table entry is not in [0, pages) are not seen;
+ * what pages hold behind kv_lens, and infinities and NaN at keys a row does
+ * not see, do not reach it.  max_rows: a hint, the largest number of rows a
+ * request has (up to 16 * kv_heads / q_heads the call takes fewer launches);
+ * the result does not depend on it.  head_dim 64 or 128, at most 128 query
+ * heads per KV head, scaling > 0.  workspace: 16-byte aligned, contents
+ * irrelevant; calls sharing one must not overlap in time. */
+int qkv_paged_attention(const void* query, const int64_t* q_strides, const void* k_pages, const int64_t* k_strides,
+                        const void* v_pages, const int64_t* v_strides, int64_t pages, int64_t page,
+                        const int32_t* table, int64_t table_ld, int64_t width, int64_t requests,
+                        const int32_t* cu_rows, const int32_t* kv_lens, int64_t rows, int64_t max_rows,
+                        int64_t q_heads, int64_t kv_heads, int64_t head_dim, float scaling, float softcap,
+                        const float* slopes, const int32_t* prefix_lens, const int32_t* first_keys, void* workspace,
+                        int64_t workspace_bytes, void* out, const int64_t* out_strides, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -140,6 +140,15 @@ _PROTOTYPES = {
     "qkv_reuse_select_bits_blocks": (_i32, [_vp, _vp, _P(_i64), _i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp,
                                             _i64, _i64, _i64, _f64, _i32, _f32, _i64, _vp, _i64, _vp, _vp, _vp,
                                             _i64, _vp, _i64, _vp]),
+    "qkv_paged_plan": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp,
+                              _vp, _vp]),
+    "qkv_paged_release": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
+    "qkv_paged_append": (_i32, [_vp, _P(_i64), _vp, _P(_i64), _vp, _P(_i64), _vp, _P(_i64), _i64, _i64, _i64, _i64,
+                                _vp, _i64, _vp]),
+    "qkv_paged_attention_workspace_bytes": (_i64, [_i64] * 8),
+    "qkv_paged_attention": (_i32, [_vp, _P(_i64), _vp, _P(_i64), _vp, _P(_i64), _i64, _i64, _vp, _i64, _i64, _i64,
+                                   _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _f32, _vp, _vp, _vp, _vp, _i64,
+                                   _vp, _P(_i64), _i32, _vp]),
 }
 
 _LIB = None

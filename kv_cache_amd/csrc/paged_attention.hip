@@ -1,0 +1,889 @@
+// Attention of the rows of a step over a paged K/V cache: single tokens, drafted tokens, chunks of prompts and whole
+// prompts, of requests of different lengths in one call.
+//
+// Row i of request b (rows cu[b] .. cu[b+1]-1) is the token at p = kv_len_b - rows_b + i.  It sees the keys j with
+// first_i <= j < max(p + 1, prefix_b), j < kv_len_b (none if p < 0), and
+//   s_j = cap * tanh(scaling * q.k_j / cap) - slope_h * |p - j|   (cap 0: scaling * q.k_j),
+//   out = sum_j exp(s_j) v_j / sum_j exp(s_j), zero where it sees none.
+//
+// Work.  The G query heads of a KV head share its K and V, so a tile holds the G heads of several tokens; a tile's
+// keys are split over several workgroups where there are few tiles.  How far is decided on the GPU from the lengths
+// (locate, below): no length is needed on the host.  Two kernels: `rows` for tiles of 128 (token, head) rows, whose
+// 4 waves hold 32 rows each and share tiles of 64 keys in LDS, bound by the matrix cores; `token` for requests of at
+// most 16 (token, head) rows, whose 4 waves walk different keys of the same rows, bound by memory.
+//
+// Both take the scores transposed, S^T = K Q^T, so that a lane holds scores of one row: the softmax is in-lane but
+// for one lane swap, and P^T leaves the score accumulators in the layout that the matrix instruction of O^T = V^T P^T
+// wants (the order of the keys within a step is free; V^T is read in the same order, by transposing LDS reads).
+#include "attend.h"
+
+namespace qkv {
+namespace {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kTile = 64;      // keys per step of the rows kernel; splits are multiples of it
+constexpr int kRowsM = 128;    // rows of a tile of the rows kernel
+constexpr int kTokenM = 16;    // rows of a tile of the token kernel
+// fp16 weights are scaled by 2^6: they stay below 2^14 (lazy rescaling lets them reach 2^8) and normal down to 2^-20
+// of the row's largest, so that the small weights of long rows keep their bits.
+template <bool F16>
+constexpr float kShift = F16 ? 6.0f : 0.0f;
+
+struct PagedArgs {
+  const uint16_t *q, *k, *v;
+  uint16_t* out;
+  int64_t q_row, q_head, k_page, k_head, k_tok, v_page, v_head, v_tok, o_row, o_head;
+  const int32_t *table, *cu, *kv_lens, *prefix, *first;
+  const float* slopes;
+  int64_t table_ld;
+  int width, pages, shift, requests, rows, kv_heads, group;
+  float scale_log2, tanh_scale, cap_log2;   // scaling * log2(e); 2 * scaling / cap * log2(e); cap * log2(e)
+  float *ws_acc, *ws_ml;
+};
+
+// What one class of requests is worked by: tiles of `tokens` tokens, for requests of more than `above` and at most
+// `most` rows, split along the keys into chunks of at least `min_keys` for about `target` workgroups.
+struct PagedClass {
+  int tokens, above, most, min_keys, target;
+  int max_parts;   // parts the workspace holds
+};
+
+// A workgroup's work.
+struct Where {
+  int b, tile, head, split, n_split, part, row0, n_rows, kv, chunk;
+};
+
+__device__ __forceinline__ int rows_of(const PagedArgs& a, int b, int& row0) {
+  row0 = min(max(a.cu[b], 0), a.rows);
+  return min(max(a.cu[b + 1], row0), a.rows) - row0;
+}
+
+// Which (request, tile, KV head, chunk of keys) workgroup `item` of a class has; false if there are fewer.  Every
+// workgroup derives it from the lengths: with the total work W = sum_b tiles_b * keys_b * heads, chunks have
+// C = max(min_keys, W / target) keys rounded up to kTile, request b is split into S_b = ceil(keys_b / C), and an
+// exclusive prefix sum of tiles_b * heads * S_b over the requests gives its first item.  PER_TILE: items are the
+// (tile, head) of requests with S_b > 1 only, for the kernel that joins the parts.
+// The head runs fastest (consecutive workgroups go to different XCDs, so that with 8 KV heads an XCD's L2 serves one
+// head), then the tile from the last one on (under a causal mask the longest).
+// Cost: about 1 us, once per workgroup, against a launch of its own for a plan.
+template <bool PER_TILE>
+__device__ __forceinline__ bool locate(const PagedArgs& a, const PagedClass& c, int item, Where& w) {
+  __shared__ unsigned long long s_tot[4];
+  __shared__ int s_part[8];
+  __shared__ int s_hit[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  auto load = [&](int b, int& nt, int& keys) {
+    nt = keys = 0;
+    if (b >= a.requests) return;
+    int row0;
+    const int n = rows_of(a, b, row0);
+    if (n <= c.above || n > c.most) return;
+    nt = (n + c.tokens - 1) / c.tokens;
+    keys = static_cast<int>(min(static_cast<int64_t>(max(a.kv_lens[b], 0)), static_cast<int64_t>(a.width) << a.shift));
+  };
+  int nt, keys;
+  unsigned long long tot = 0;
+  load(tid, nt, keys);
+  tot = static_cast<unsigned long long>(nt) * keys;
+  for (int b0 = 256; b0 < a.requests; b0 += 256) {
+    int nt2, keys2;
+    load(b0 + tid, nt2, keys2);
+    tot += static_cast<unsigned long long>(nt2) * keys2;
+  }
+  for (int m = 32; m >= 1; m >>= 1) tot += __shfl_xor(tot, m);
+  if (lane == 0) s_tot[wave] = tot;
+  if (tid == 0) s_hit[0] = -1;
+  __syncthreads();
+  tot = (s_tot[0] + s_tot[1] + s_tot[2] + s_tot[3]) * a.kv_heads;
+  const unsigned long long per = (tot + c.target - 1) / c.target;
+  const int chunk = static_cast<int>((max(per, static_cast<unsigned long long>(c.min_keys)) + kTile - 1) / kTile * kTile);
+  int carry = 0, part_carry = 0;
+  for (int b0 = 0; b0 < a.requests; b0 += 256) {
+    if (b0) load(b0 + tid, nt, keys);
+    const int ns = max(1, (keys + chunk - 1) / chunk);
+    const int parts = ns > 1 ? nt * a.kv_heads * ns : 0;
+    const int items = PER_TILE ? (ns > 1 ? nt * a.kv_heads : 0) : nt * a.kv_heads * ns;
+    const int up = wave_incl_scan(items), up_part = wave_incl_scan(parts);
+    if (lane == 63) {
+      s_part[2 * wave] = up;
+      s_part[2 * wave + 1] = up_part;
+    }
+    __syncthreads();
+    int before = carry, before_part = part_carry;
+    for (int i = 0; i < 4; ++i) {
+      if (i < wave) {
+        before += s_part[2 * i];
+        before_part += s_part[2 * i + 1];
+      }
+      carry += s_part[2 * i];
+      part_carry += s_part[2 * i + 1];
+    }
+    const int begin = before + up - items;
+    if (item >= begin && item < begin + items) {   // one thread at most
+      s_hit[0] = b0 + tid;
+      s_hit[1] = item - begin;
+      s_hit[2] = before_part + up_part - parts;
+      s_hit[3] = keys;
+    }
+    __syncthreads();
+    if (s_hit[0] >= 0 || item < carry) break;   // the same for every thread
+  }
+  const int b = __builtin_amdgcn_readfirstlane(s_hit[0]);
+  if (b < 0) return false;
+  w.b = b;
+  w.kv = __builtin_amdgcn_readfirstlane(s_hit[3]);
+  w.chunk = chunk;
+  w.n_split = max(1, (w.kv + chunk - 1) / chunk);
+  w.n_rows = rows_of(a, b, w.row0);
+  const int n_tiles = (w.n_rows + c.tokens - 1) / c.tokens;
+  const int at = __builtin_amdgcn_readfirstlane(s_hit[1]);
+  const int rest = at / a.kv_heads;
+  w.head = at - rest * a.kv_heads;
+  w.split = rest / n_tiles;
+  w.tile = n_tiles - 1 - (rest - w.split * n_tiles);
+  w.part = __builtin_amdgcn_readfirstlane(s_hit[2]) + (w.head * n_tiles + w.tile) * w.n_split;
+  // always so where cu_rows ascends; otherwise nothing is written out of bounds
+  if (w.n_split > 1 && (w.part < 0 || w.part > c.max_parts - w.n_split)) return false;
+  if (!PER_TILE) w.part += w.split;
+  return true;
+}
+
+// What a lane needs of its row: the keys [lo, hi) it sees, its position, its score bias.
+struct Row {
+  int64_t q_at, o_at;   // its offsets in q and out
+  int lo, hi, pos;
+  float slope;          // log2(e) * slope
+  bool on;
+};
+
+// Row `i` of the tile, G heads a token.  A row the tile does not have sees everything, so that it asks for no mask.
+template <bool FORM>
+__device__ __forceinline__ Row row_of(const PagedArgs& a, const PagedClass& c, const Where& w, int i) {
+  const int t = i / a.group, g = i - t * a.group;
+  const int token = w.tile * c.tokens + t;
+  Row r;
+  r.on = t < c.tokens && token < w.n_rows;
+  const int64_t row = w.row0 + (r.on ? token : 0);
+  const int head = w.head * a.group + (r.on ? g : 0);
+  r.q_at = row * a.q_row + head * a.q_head;
+  r.o_at = row * a.o_row + head * a.o_head;
+  const int kv = a.kv_lens[w.b];
+  r.pos = kv - w.n_rows + token;
+  r.lo = 0;
+  r.hi = 0x7FFFFFFF;
+  r.slope = 0.0f;
+  if (r.on) {
+    r.hi = 0;
+    if (r.pos >= 0) r.hi = min(w.kv, max(r.pos + 1, a.prefix ? a.prefix[w.b] : 0));
+    if (a.first) r.lo = max(0, a.first[row]);
+    if (FORM && a.slopes) r.slope = kLog2e * a.slopes[head];
+  }
+  return r;
+}
+
+// tanh(x) from t = exp2(2 x log2(e)): 1 - 2 / (t + 1), whose error of about 2^-23 is relative to 1, so that small x
+// take the odd polynomial (next term x^11 / 113: below 2^-27 of x at 0.25).
+__device__ __forceinline__ float tanh_of(float x, float x2log2e) {
+  const float t = __builtin_amdgcn_exp2f(x2log2e);
+  const float far = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(t + 1.0f), 1.0f);
+  const float y = x * x;
+  float p = __builtin_fmaf(y, 62.0f / 2835.0f, -17.0f / 315.0f);
+  p = __builtin_fmaf(y, p, 2.0f / 15.0f);
+  p = __builtin_fmaf(y, p, -1.0f / 3.0f);
+  const float near = __builtin_fmaf(x * y, p, x);
+  return fabsf(x) < 0.25f ? near : far;
+}
+
+// The score of a product q.k in log2 units, with cap and bias.
+__device__ __forceinline__ float form_score(const PagedArgs& a, const Row& r, float qk, int key) {
+  float s = qk * a.scale_log2;
+  if (a.cap_log2 != 0.0f) {
+    const float x2 = qk * a.tanh_scale;
+    s = a.cap_log2 * tanh_of(x2 * (0.5f / kLog2e), x2);
+  }
+  return __builtin_fmaf(-r.slope, fabsf(static_cast<float>(r.pos - key)), s);
+}
+
+// The id of the page with key `key`, or -1 where the request has none there (wave-uniform).
+__device__ __forceinline__ int page_id(const PagedArgs& a, const Where& w, int key) {
+  if (key >= w.kv) return -1;
+  const int id = a.table[w.b * a.table_ld + (key >> a.shift)];
+  return static_cast<unsigned>(id) < static_cast<unsigned>(a.pages) ? id : -1;
+}
+
+template <bool F16>
+__device__ __forceinline__ bool not_finite(uint32_t half) {
+  constexpr uint32_t e = F16 ? 0x7C00u : 0x7F80u;
+  return (half & e) == e;
+}
+
+// Takes the infinities and NaN out of eight 16-bit values; true if there were any.
+template <bool F16>
+__device__ __forceinline__ bool clean(u32x4_t& x) {
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool lo = not_finite<F16>(x[i]), hi = not_finite<F16>(x[i] >> 16);
+    x[i] &= (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
+    any |= lo | hi;
+  }
+  return any;
+}
+
+// 16-byte unit `u` of row `r` of a [rows][D] tile in LDS lies at unit u ^ swizzle(r) of its row: the 16-byte reads of
+// 8 rows at one unit, and the transposing reads of 8 rows, then fall on different banks.
+template <int D>
+__device__ __forceinline__ int swizzle(int r) {
+  return D == 128 ? (r & 7) << 1 : ((r >> 1) & 3) << 1;
+}
+
+typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
+
+// Four rows r0 .. r0+3 (by the address) of one column each: transposing read of 8 bytes a lane.
+__device__ __forceinline__ u32x2_t read_tr(const uint16_t* p) {
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)p));
+}
+
+template <bool F16>
+__device__ __forceinline__ f32x16_t mfma_32x32x16(u32x4_t a, u32x4_t b, f32x16_t c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
+                                                  0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                   0, 0, 0);
+}
+
+__device__ __forceinline__ int wave_max_i(int v) {
+  for (int m = 32; m >= 1; m >>= 1) v = max(v, shfl_xor_i(v, m));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// ---------------------------------------------------------------------------
+// Tiles of 128 rows.  Wave w holds rows 32w .. 32w+31 as columns of S^T and O^T; a lane holds one row's scores of 16
+// of the 32 keys of a score tile (its other half-wave the others), and one row's outputs.  K and V of 64 keys lie in
+// LDS, double-buffered: the loads of the next tile are issued before this one is computed and stored behind it, one
+// barrier a tile.
+// ---------------------------------------------------------------------------
+template <int D, bool F16, bool FORM>
+__global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs a, PagedClass c) {
+  constexpr int KS = D / 16;               // steps of 16 channels of Q.K
+  constexpr int DB = D / 32;               // blocks of 32 channels of P.V
+  constexpr int UR = D / 8;                // 16-byte units of a row
+  constexpr int NU = kTile * UR / 256;     // units a thread stages of K, and of V
+  __shared__ __attribute__((aligned(16))) uint16_t kbuf[2][kTile * D], vbuf[2][kTile * D];
+  __shared__ int s_odd[2], s_range[4][4];
+  Where w;
+  if (!locate<false>(a, c, blockIdx.x, w)) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = lane >> 5, l32 = lane & 31;
+  const float ninf = -__builtin_huge_valf();
+  const Row r = row_of<FORM>(a, c, w, 32 * wave + l32);
+
+  // keys that all rows see, and that any row sees: of the wave, then of the workgroup
+  const int all_lo = wave_max_i(r.lo), all_hi = -wave_max_i(-r.hi);
+  const int any_lo = -wave_max_i(r.on ? -r.lo : -0x7FFFFFFF), any_hi = wave_max_i(r.on ? r.hi : 0);
+  if (lane == 0) {
+    s_range[wave][0] = all_lo;
+    s_range[wave][1] = all_hi;
+    s_range[wave][2] = any_lo;
+    s_range[wave][3] = any_hi;
+  }
+  if (tid < 2) s_odd[tid] = -1;
+  __syncthreads();
+  int wg_all_lo = 0, wg_all_hi = 0x7FFFFFFF, wg_lo = 0x7FFFFFFF, wg_hi = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    wg_all_lo = max(wg_all_lo, s_range[i][0]);
+    wg_all_hi = min(wg_all_hi, s_range[i][1]);
+    wg_lo = min(wg_lo, s_range[i][2]);
+    wg_hi = max(wg_hi, s_range[i][3]);
+  }
+  wg_all_lo = __builtin_amdgcn_readfirstlane(wg_all_lo);
+  wg_all_hi = __builtin_amdgcn_readfirstlane(wg_all_hi);
+  const int begin = __builtin_amdgcn_readfirstlane(max(w.split * w.chunk, wg_lo / kTile * kTile));
+  const int end = __builtin_amdgcn_readfirstlane(static_cast<int>(min(static_cast<int64_t>(w.split + 1) * w.chunk, static_cast<int64_t>(wg_hi))));
+
+  u32x4_t qf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const uint4 x = load16u(a.q + r.q_at + 16 * s + 8 * half);
+    qf[s] = r.on ? u32x4_t{x.x, x.y, x.z, x.w} : u32x4_t{0u, 0u, 0u, 0u};
+  }
+
+  f32x16_t o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+  float m = ninf, l = 0.0f;
+
+  const int u_row = tid / UR, u_col = tid % UR;
+  const uint16_t* kh = a.k + w.head * a.k_head + 8 * u_col;
+  const uint16_t* vh = a.v + w.head * a.v_head + 8 * u_col;
+  u32x4_t kreg[NU], vreg[NU];
+  int ids[4];
+  auto load = [&](int t0) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) ids[g] = page_id(a, w, t0 + 16 * g);
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      // the 16-key group of this wave's rows
+      const int row = u_row + u * (256 / UR);
+      const int g = NU == 4 ? u : 2 * u + (wave >> 1);
+      const int id = max(g == 0 ? ids[0] : g == 1 ? ids[1] : g == 2 ? ids[2] : ids[3], 0);
+      const int at = (t0 + row) & ((1 << a.shift) - 1);
+      kreg[u] = *reinterpret_cast<const u32x4_t*>(kh + id * a.k_page + at * a.k_tok);
+      vreg[u] = *reinterpret_cast<const u32x4_t*>(vh + id * a.v_page + at * a.v_tok);
+    }
+  };
+  // Stores the loaded tile.  Where some row does not see all of it, what no row may read (a page's rest) becomes
+  // zero, and so do infinities and NaN of V, which a zero weight would not hide: add_odd adds those to the rows
+  // that do see them.
+  auto store = [&](int t0, int buf) {
+    const bool masked = t0 < wg_all_lo || t0 + kTile > wg_all_hi || (ids[0] | ids[1] | ids[2] | ids[3]) < 0;
+    if (masked) {
+      bool odd = false;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        const int row = u_row + u * (256 / UR);
+        const int g = NU == 4 ? u : 2 * u + (wave >> 1);
+        const int id = g == 0 ? ids[0] : g == 1 ? ids[1] : g == 2 ? ids[2] : ids[3];
+        if (id < 0 || t0 + row >= w.kv) vreg[u] = u32x4_t{0u, 0u, 0u, 0u};
+        else odd |= clean<F16>(vreg[u]);
+      }
+      if (odd) s_odd[buf] = t0;
+    }
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int row = u_row + u * (256 / UR);
+      const int at = row * D + 8 * (u_col ^ swizzle<D>(row));
+      *reinterpret_cast<u32x4_t*>(&kbuf[buf][at]) = kreg[u];
+      *reinterpret_cast<u32x4_t*>(&vbuf[buf][at]) = vreg[u];
+    }
+  };
+  auto add_odd = [&](int t0) {
+    for (int j = 0; j < kTile; ++j) {
+      const int key = t0 + j, id = page_id(a, w, key);
+      if (id < 0) continue;
+      const uint16_t* vr = a.v + id * a.v_page + w.head * a.v_head + (key & ((1 << a.shift) - 1)) * a.v_tok + 4 * half;
+      if (!(r.on && key >= r.lo && key < r.hi)) continue;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint16_t x = vr[32 * d + 8 * (i >> 2) + (i & 3)];
+          if (not_finite<F16>(x)) o[d][i] += half_to_f32<F16>(x);
+        }
+    }
+  };
+
+  const int k_at = l32 * D, k_sw = swizzle<D>(l32);
+  const int v_row = 4 * half + ((lane & 15) >> 2), v_unit = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), v_el = 4 * (lane & 1);
+  auto compute = [&](int t0, int buf, bool hole0, bool hole1, bool hole2, bool hole3) {
+    if (t0 >= any_hi || t0 + kTile <= any_lo) return;   // no row of the wave sees any of it
+    f32x16_t s[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(&kbuf[buf][kb * 32 * D + k_at + 8 * ((2 * ks + half) ^ k_sw)]);
+        s[kb] = mfma_32x32x16<F16>(kf, qf[ks], s[kb]);
+      }
+    }
+    const int key0 = t0 + 4 * half;   // element i of tile kb: key0 + 32 kb + 8 (i / 4) + i % 4
+    if constexpr (FORM) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kb][i] = form_score(a, r, s[kb][i], key0 + 32 * kb + 8 * (i >> 2) + (i & 3));
+    }
+    if (t0 < all_lo || t0 + kTile > all_hi || hole0 || hole1 || hole2 || hole3) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = key0 + 32 * kb + 8 * (i >> 2) + (i & 3);
+          const bool hole = kb == 0 ? (i < 8 ? hole0 : hole1) : (i < 8 ? hole2 : hole3);
+          if (hole || key < r.lo || key >= r.hi) s[kb][i] = ninf;
+        }
+    }
+    float cm = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) cm = fmaxf(cm, s[kb][i]);
+    cm = max_x32(cm);
+    const float sl = FORM ? 1.0f : a.scale_log2;
+    cm = cm * sl - kShift<F16>;
+    const float mn = fmaxf(m, cm);
+    if (__ballot(mn > m + kLazyLog2)) {   // wave-uniform
+      const float al = mn == ninf ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      l *= al;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] *= al;
+      m = mn;
+    }
+    const float ms = m == ninf ? 0.0f : m;
+    float sum0 = 0.0f, sum1 = 0.0f;
+    u32x4_t p[4];   // B operands of P.V: 16 keys each
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][4 * q + i], sl, -ms));
+        sum0 += e[0] + e[1];
+        sum1 += e[2] + e[3];
+        const u32x2_t x = pack4_half<F16>(e);
+        p[2 * kb + (q >> 1)][2 * (q & 1)] = x[0];
+        p[2 * kb + (q >> 1)][2 * (q & 1) + 1] = x[1];
+      }
+    l += sum0 + sum1;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const int r0 = 16 * ks + v_row, r1 = r0 + 8;
+        const u32x2_t x = read_tr(&vbuf[buf][r0 * D + 8 * ((4 * d + v_unit) ^ swizzle<D>(r0)) + v_el]);
+        const u32x2_t y = read_tr(&vbuf[buf][r1 * D + 8 * ((4 * d + v_unit) ^ swizzle<D>(r1)) + v_el]);
+        o[d] = mfma_32x32x16<F16>(u32x4_t{x[0], x[1], y[0], y[1]}, p[ks], o[d]);
+      }
+    if (s_odd[buf] == t0) add_odd(t0);
+  };
+
+  if (begin < end) {
+    load(begin);
+    store(begin, 0);
+    bool h0 = ids[0] < 0, h1 = ids[1] < 0, h2 = ids[2] < 0, h3 = ids[3] < 0;
+    __syncthreads();
+    int buf = 0;
+    for (int t0 = begin; t0 < end; t0 += kTile, buf ^= 1) {
+      const bool more = t0 + kTile < end;
+      if (more) load(t0 + kTile);
+      compute(t0, buf, h0, h1, h2, h3);
+      if (more) {
+        store(t0 + kTile, buf ^ 1);
+        h0 = ids[0] < 0, h1 = ids[1] < 0, h2 = ids[2] < 0, h3 = ids[3] < 0;
+      }
+      __syncthreads();
+    }
+  }
+
+  l = sum_x32(l);
+  if (w.n_split == 1) {
+    if (!r.on) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* out = a.out + r.o_at + 4 * half;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float x[4] = {o[d][4 * q] * inv, o[d][4 * q + 1] * inv, o[d][4 * q + 2] * inv, o[d][4 * q + 3] * inv};
+        *reinterpret_cast<u32x2_t*>(out + 32 * d + 8 * q) = pack4_half<F16>(x);
+      }
+    return;
+  }
+  const int64_t at = static_cast<int64_t>(w.part) * kRowsM + 32 * wave + l32;
+  if (half == 0) {
+    a.ws_ml[2 * at] = m;
+    a.ws_ml[2 * at + 1] = l;
+  }
+  if (l == 0.0f) return;   // the joining kernel leaves it out
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<float4*>(a.ws_acc + at * D + 4 * half + 32 * d + 8 * q) =
+          make_float4(o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]);
+}
+
+// ---------------------------------------------------------------------------
+// Tiles of at most 16 rows: the columns of 16-wide score tiles.  Wave w takes steps w, w + 4, ... of 32 keys of the
+// workgroup's chunk; K goes from memory to the matrix instruction's registers, V through the wave's own part of LDS
+// (stored as it lies, read transposed), no barrier until the waves are joined at the end.
+// ---------------------------------------------------------------------------
+template <int D, bool F16, bool FORM>
+__global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedArgs a, PagedClass c) {
+  constexpr int STEP = 32;
+  constexpr int KS = D / 32;               // steps of 32 channels of Q.K
+  constexpr int DB = D / 16;               // blocks of 16 channels of P.V
+  constexpr int UR = D / 8;                // 16-byte units of a row
+  constexpr int NV = STEP * UR / 64;       // units of V a lane stages
+  constexpr int PASS = 64 / UR;            // rows of V a load covers
+  __shared__ union {
+    uint16_t v[4][STEP * D];
+    float acc[4][kTokenM][D];
+  } lds;
+  __shared__ float s_m[4][kTokenM], s_l[4][kTokenM];
+  Where w;
+  if (!locate<false>(a, c, blockIdx.x, w)) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g4 = lane >> 4, c16 = lane & 15;
+  const float ninf = -__builtin_huge_valf();
+  const Row r = row_of<FORM>(a, c, w, c16);
+  const int all_lo = wave_max_i(r.lo), all_hi = -wave_max_i(-r.hi);
+  const int any_lo = -wave_max_i(r.on ? -r.lo : -0x7FFFFFFF), any_hi = wave_max_i(r.on ? r.hi : 0);
+  const int begin = max(w.split * w.chunk, any_lo / kTile * kTile);
+  const int end = static_cast<int>(min(static_cast<int64_t>(w.split + 1) * w.chunk, static_cast<int64_t>(any_hi)));
+
+  u32x4_t qf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const uint4 x = load16u(a.q + r.q_at + 32 * s + 8 * g4);
+    qf[s] = r.on ? u32x4_t{x.x, x.y, x.z, x.w} : u32x4_t{0u, 0u, 0u, 0u};
+  }
+  f32x4_t o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) o[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = ninf, l = 0.0f;
+  uint16_t* vt = lds.v[wave];
+  const uint16_t* kh = a.k + w.head * a.k_head + 8 * g4;
+  const uint16_t* vh = a.v + w.head * a.v_head + 8 * (lane % UR);
+  const int vr = lane / UR, mask = (1 << a.shift) - 1;
+
+  struct Step {
+    u32x4_t k[2][KS], v[NV];
+    int id[2];
+  };
+  auto load = [&](int t0, Step& x) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      x.id[t] = page_id(a, w, t0 + 16 * t);
+      const uint16_t* p = kh + max(x.id[t], 0) * a.k_page + ((t0 + 16 * t + c16) & mask) * a.k_tok;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) x.k[t][s] = ld_nt4(p + 32 * s);
+    }
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int row = u * PASS + vr;
+      x.v[u] = ld_nt4(vh + max(x.id[u * PASS / 16], 0) * a.v_page + ((t0 + row) & mask) * a.v_tok);
+    }
+  };
+  auto compute = [&](int t0, Step& x) {
+    const bool masked = t0 < all_lo || t0 + STEP > all_hi || (x.id[0] | x.id[1]) < 0;
+    bool odd = false;
+    if (masked) {   // as in paged_rows_kernel
+#pragma unroll
+      for (int u = 0; u < NV; ++u) {
+        if (x.id[u * PASS / 16] < 0 || t0 + u * PASS + vr >= w.kv) x.v[u] = u32x4_t{0u, 0u, 0u, 0u};
+        else odd |= clean<F16>(x.v[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int row = u * PASS + vr;
+      *reinterpret_cast<u32x4_t*>(&vt[row * D + 8 * ((lane % UR) ^ swizzle<D>(row))]) = x.v[u];
+    }
+    float s[2][4];
+    float cm = ninf;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) acc = mfma_16x16x32<F16>(x.k[t][ks], qf[ks], acc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = t0 + 16 * t + 4 * g4 + i;
+        float y = FORM ? form_score(a, r, acc[i], key) : acc[i] * a.scale_log2;
+        if (masked && (x.id[t] < 0 || key < r.lo || key >= r.hi)) y = ninf;
+        s[t][i] = y;
+        cm = fmaxf(cm, y);
+      }
+    }
+    cm = max_x32(max_x16(cm)) - kShift<F16>;
+    const float mn = fmaxf(m, cm);
+    if (__ballot(mn > m + kLazyLog2)) {   // wave-uniform
+      const float al = mn == ninf ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      l *= al;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[d][i] *= al;
+      m = mn;
+    }
+    const float ms = m == ninf ? 0.0f : m;
+    u32x4_t p;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(s[t][i] - ms);
+      l += (e[0] + e[1]) + (e[2] + e[3]);
+      const u32x2_t y = pack4_half<F16>(e);
+      p[2 * t] = y[0];
+      p[2 * t + 1] = y[1];
+    }
+    // element j of a lane's step: key 16 (j / 4) + 4 g4 + j % 4, of P and of V alike
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const int r0 = 4 * g4 + (c16 >> 2), r1 = r0 + 16, unit = 2 * d + ((lane & 3) >> 1), el = 4 * (lane & 1);
+      const u32x2_t y = read_tr(&vt[r0 * D + 8 * (unit ^ swizzle<D>(r0)) + el]);
+      const u32x2_t z = read_tr(&vt[r1 * D + 8 * (unit ^ swizzle<D>(r1)) + el]);
+      o[d] = mfma_16x16x32<F16>(u32x4_t{y[0], y[1], z[0], z[1]}, p, o[d]);
+    }
+    if (__ballot(odd)) {
+      for (int j = 0; j < STEP; ++j) {
+        const int key = t0 + j, id = page_id(a, w, key);
+        if (id < 0 || !(r.on && key >= r.lo && key < r.hi)) continue;
+        const uint16_t* p0 = a.v + id * a.v_page + w.head * a.v_head + (key & mask) * a.v_tok + 4 * g4;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (not_finite<F16>(p0[16 * d + i])) o[d][i] += half_to_f32<F16>(p0[16 * d + i]);
+      }
+    }
+  };
+
+  Step x[2];
+  int t0 = begin + STEP * wave;
+  if (t0 < end) load(t0, x[0]);
+  while (t0 < end) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (t0 < end) {
+        if (t0 + 4 * STEP < end) load(t0 + 4 * STEP, x[u ^ 1]);
+        compute(t0, x[u]);
+        t0 += 4 * STEP;
+      }
+    }
+  }
+
+  // the four waves' parts, joined
+  l = sum_x32(sum_x16(l));
+  __syncthreads();   // lds.v is done with
+  if (lane < kTokenM) {
+    s_m[wave][lane] = m;
+    s_l[wave][lane] = l;
+  }
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+    *reinterpret_cast<f32x4_t*>(&lds.acc[wave][c16][16 * d + 4 * g4]) = o[d];
+  __syncthreads();
+  constexpr int E = D / 16;   // values a thread joins
+  const int row = tid >> 4, d0 = (tid & 15) * E;
+  float mj = s_m[0][row];
+#pragma unroll
+  for (int i = 1; i < 4; ++i) mj = fmaxf(mj, s_m[i][row]);
+  float lj = 0.0f, y[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) y[e] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (s_l[i][row] == 0.0f) continue;
+    const float f = __builtin_amdgcn_exp2f(s_m[i][row] - mj);
+    lj = __builtin_fmaf(s_l[i][row], f, lj);
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = __builtin_fmaf(lds.acc[i][row][d0 + e], f, y[e]);
+  }
+  if (w.n_split == 1) {
+    const Row ro = row_of<false>(a, c, w, row);
+    if (!ro.on) return;
+    const float inv = lj == 0.0f ? 0.0f : 1.0f / lj;
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      const float z[4] = {y[e] * inv, y[e + 1] * inv, y[e + 2] * inv, y[e + 3] * inv};
+      *reinterpret_cast<u32x2_t*>(a.out + ro.o_at + d0 + e) = pack4_half<F16>(z);
+    }
+    return;
+  }
+  const int64_t at = static_cast<int64_t>(w.part) * kTokenM + row;
+  if ((tid & 15) == 0) {
+    a.ws_ml[2 * at] = mj;
+    a.ws_ml[2 * at + 1] = lj;
+  }
+#pragma unroll
+  for (int e = 0; e < E; e += 4)
+    *reinterpret_cast<float4*>(a.ws_acc + at * D + d0 + e) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+}
+
+// Joins the parts of the tiles whose keys were split: 16 rows a workgroup (blockIdx.y: which 16 of the tile), the
+// parts in the order of their keys, so that the result does not depend on which was done first.
+template <int D, bool F16, int M>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, PagedClass c) {
+  Where w;
+  if (!locate<true>(a, c, blockIdx.x, w)) return;
+  constexpr int E = D / 16;
+  const int row = blockIdx.y * 16 + (threadIdx.x >> 4), d0 = (threadIdx.x & 15) * E;
+  const Row r = row_of<false>(a, c, w, row);
+  if (!r.on) return;
+  const int64_t at = static_cast<int64_t>(w.part) * M + row;   // of split 0 (w.split is 0 here)
+  const float ninf = -__builtin_huge_valf();
+  float m = ninf, l = 0.0f, y[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) y[e] = 0.0f;
+  for (int s = 0; s < w.n_split; ++s) {
+    const int64_t p = at + static_cast<int64_t>(s) * M;
+    const float ls = a.ws_ml[2 * p + 1];
+    if (ls == 0.0f) continue;
+    const float ms = a.ws_ml[2 * p];
+    const float mn = fmaxf(m, ms);
+    const float fo = m == ninf ? 0.0f : __builtin_amdgcn_exp2f(m - mn), fn = __builtin_amdgcn_exp2f(ms - mn);
+    l = __builtin_fmaf(ls, fn, l * fo);
+    m = mn;
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(a.ws_acc + p * D + d0 + e);
+      y[e] = __builtin_fmaf(x.x, fn, y[e] * fo);
+      y[e + 1] = __builtin_fmaf(x.y, fn, y[e + 1] * fo);
+      y[e + 2] = __builtin_fmaf(x.z, fn, y[e + 2] * fo);
+      y[e + 3] = __builtin_fmaf(x.w, fn, y[e + 3] * fo);
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int e = 0; e < E; e += 4) {
+    const float z[4] = {y[e] * inv, y[e + 1] * inv, y[e + 2] * inv, y[e + 3] * inv};
+    *reinterpret_cast<u32x2_t*>(a.out + r.o_at + d0 + e) = pack4_half<F16>(z);
+  }
+}
+
+// The launches of a call, from what the host knows: rows, requests, and the tokens a table row covers.
+struct Shape {
+  PagedClass cls;
+  bool used;
+  int64_t items, parts, tiles;   // workgroups; parts in the workspace; split tiles
+};
+
+Shape shape_of(bool token, int64_t rows, int64_t max_rows, int64_t requests, int64_t max_keys, int64_t kv_heads,
+               int64_t group) {
+  const int64_t m = token ? kTokenM : kRowsM;
+  const int64_t token_rows = kTokenM / group;   // 0: every request takes the rows kernel
+  Shape s{};
+  s.cls.tokens = static_cast<int>(m / group);
+  s.cls.above = token ? 0 : static_cast<int>(token_rows);
+  // without a rows kernel the token kernel takes every request, a longer one in several tiles
+  s.cls.most = token && max_rows > token_rows ? static_cast<int>(token_rows) : 0x7FFFFFFF;
+  s.cls.min_keys = 256;
+  s.cls.target = token ? 1024 : 512;
+  s.used = rows > 0 && (token ? token_rows > 0 : max_rows > token_rows);
+  if (!s.used) return s;
+  const int64_t some = std::min(requests, rows);
+  const int64_t tiles = (s.cls.most == token_rows ? some : (rows + some * (s.cls.tokens - 1)) / s.cls.tokens) * kv_heads;
+  s.items = tiles;
+  if (max_keys > s.cls.min_keys) {
+    // sum over the requests of tiles * ceil(keys / C) <= W / C + tiles, W / C <= target; where a request is split its
+    // ceil(keys / C) is at most 2 keys / C
+    s.items = std::min(tiles + s.cls.target, tiles * cdiv(max_keys, s.cls.min_keys));
+    s.parts = std::min<int64_t>(2 * s.cls.target, s.items);
+    s.tiles = std::min<int64_t>(s.cls.target, tiles);
+  }
+  s.cls.max_parts = static_cast<int>(s.parts);
+  return s;
+}
+
+int64_t part_floats(int64_t m, int64_t head_dim) { return m * (head_dim + 2); }
+
+bool good_sizes(int64_t rows, int64_t requests, int64_t width, int64_t page, int64_t q_heads, int64_t kv_heads,
+                int64_t head_dim) {
+  return rows >= 0 && rows <= (1 << 30) && requests >= 1 && requests <= (1 << 20) && width >= 1 && page >= 16 &&
+         page <= 4096 && !(page & (page - 1)) && width <= ((1ll << 31) - page) / page && kv_heads >= 1 &&
+         q_heads >= kv_heads && q_heads % kv_heads == 0 && q_heads <= 65536 && q_heads / kv_heads <= kRowsM &&
+         (head_dim == 64 || head_dim == 128);
+}
+
+template <int D, bool F16, bool FORM>
+int launch(PagedArgs a, const Shape& rows, const Shape& token, hipStream_t st) {
+  if (rows.used)
+    paged_rows_kernel<D, F16, FORM><<<static_cast<unsigned>(rows.items), 256, 0, st>>>(a, rows.cls);
+  if (token.used) {
+    PagedArgs t = a;
+    t.ws_acc += rows.parts * kRowsM * D;
+    t.ws_ml += rows.parts * kRowsM * 2;
+    paged_token_kernel<D, F16, FORM><<<static_cast<unsigned>(token.items), 256, 0, st>>>(t, token.cls);
+    if (token.parts)
+      paged_join_kernel<D, F16, kTokenM><<<static_cast<unsigned>(token.tiles), 256, 0, st>>>(t, token.cls);
+  }
+  if (rows.used && rows.parts)
+    paged_join_kernel<D, F16, kRowsM><<<dim3(static_cast<unsigned>(rows.tiles), kRowsM / 16), 256, 0, st>>>(a, rows.cls);
+  return check_launch("qkv_paged_attention");
+}
+
+}  // namespace
+}  // namespace qkv
+
+using namespace qkv;
+
+QKV_EXPORT int64_t qkv_paged_attention_workspace_bytes(int64_t rows, int64_t max_rows, int64_t requests, int64_t width,
+                                                       int64_t page, int64_t q_heads, int64_t kv_heads,
+                                                       int64_t head_dim) {
+  if (!good_sizes(rows, requests, width, page, q_heads, kv_heads, head_dim)) return -1;
+  int64_t floats = 0;
+  for (const bool token : {false, true}) {
+    const Shape s = shape_of(token, rows, max_rows, requests, width * page, kv_heads, q_heads / kv_heads);
+    floats += s.parts * part_floats(token ? kTokenM : kRowsM, head_dim);
+  }
+  return 4 * floats;
+}
+
+QKV_EXPORT int qkv_paged_attention(const void* query, const int64_t* q_strides, const void* k_pages,
+                                   const int64_t* k_strides, const void* v_pages, const int64_t* v_strides,
+                                   int64_t pages, int64_t page, const int32_t* table, int64_t table_ld, int64_t width,
+                                   int64_t requests, const int32_t* cu_rows, const int32_t* kv_lens, int64_t rows,
+                                   int64_t max_rows, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                   float scaling, float softcap, const float* slopes, const int32_t* prefix_lens,
+                                   const int32_t* first_keys, void* workspace, int64_t workspace_bytes, void* out,
+                                   const int64_t* out_strides, int dtype, void* stream) {
+  const char* what = "qkv_paged_attention";
+  if (!q_strides || !k_pages || !k_strides || !v_pages || !v_strides || !table || !cu_rows || !kv_lens || !out_strides ||
+      (rows > 0 && (!query || !out)))
+    return fail(QKV_ERR_INVALID, "%s: null pointer", what);
+  bool f16;
+  if (const int rc = half_dtype(dtype, what, &f16)) return rc;
+  if (!good_sizes(rows, requests, width, page, q_heads, kv_heads, head_dim) || table_ld < width || pages < 1 ||
+      pages > (1ll << 30) || max_rows < 0)
+    return fail(QKV_ERR_UNSUPPORTED, "%s: unsupported sizes (head_dim 64 or 128, page a power of two in [16, 4096], "
+                "q_heads a multiple of kv_heads and at most %d times as many)", what, kRowsM);
+  if (!(scaling > 0.0f) || !(scaling < __builtin_huge_valf()) || !(softcap >= 0.0f) || !(softcap < __builtin_huge_valf()))
+    return fail(QKV_ERR_INVALID, "%s: scaling must be positive and softcap 0 or positive", what);
+  if (!aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(out, 16) || out_strides[0] % 8 || out_strides[1] % 8)
+    return fail(QKV_ERR_INVALID, "%s: pages and output must be 16-byte aligned", what);
+  for (int i = 0; i < 3; ++i)
+    if (k_strides[i] % 8 || v_strides[i] % 8)
+      return fail(QKV_ERR_INVALID, "%s: pages and output must be 16-byte aligned", what);
+  const int64_t group = q_heads / kv_heads;
+  const Shape sr = shape_of(false, rows, max_rows, requests, width * page, kv_heads, group);
+  const Shape sk = shape_of(true, rows, max_rows, requests, width * page, kv_heads, group);
+  if (sr.items > (1ll << 30) || sk.items > (1ll << 30)) return fail(QKV_ERR_UNSUPPORTED, "%s: too many rows", what);
+  const int64_t need = qkv_paged_attention_workspace_bytes(rows, max_rows, requests, width, page, q_heads, kv_heads, head_dim);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(QKV_ERR_INVALID, "%s: workspace must be 16-byte aligned and hold %lld bytes", what,
+                static_cast<long long>(need));
+  if (rows == 0) return QKV_OK;
+  PagedArgs a{};
+  a.q = static_cast<const uint16_t*>(query);
+  a.k = static_cast<const uint16_t*>(k_pages);
+  a.v = static_cast<const uint16_t*>(v_pages);
+  a.out = static_cast<uint16_t*>(out);
+  a.q_row = q_strides[0], a.q_head = q_strides[1];
+  a.k_page = k_strides[0], a.k_head = k_strides[1], a.k_tok = k_strides[2];
+  a.v_page = v_strides[0], a.v_head = v_strides[1], a.v_tok = v_strides[2];
+  a.o_row = out_strides[0], a.o_head = out_strides[1];
+  a.table = table, a.cu = cu_rows, a.kv_lens = kv_lens, a.prefix = prefix_lens, a.first = first_keys;
+  a.slopes = slopes;
+  a.table_ld = table_ld;
+  a.width = static_cast<int>(width), a.pages = static_cast<int>(pages);
+  a.shift = __builtin_ctz(static_cast<unsigned>(page));
+  a.requests = static_cast<int>(requests), a.rows = static_cast<int>(rows);
+  a.kv_heads = static_cast<int>(kv_heads), a.group = static_cast<int>(group);
+  a.scale_log2 = scaling * kLog2e;
+  a.tanh_scale = softcap > 0.0f ? 2.0f * kLog2e * scaling / softcap : 0.0f;
+  a.cap_log2 = softcap * kLog2e;
+  a.ws_acc = static_cast<float*>(workspace);
+  a.ws_ml = a.ws_acc + head_dim * (sr.parts * kRowsM + sk.parts * kTokenM);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool form = softcap > 0.0f || slopes;
+  return with_half(f16, [&](auto h) {
+    constexpr bool F = decltype(h)::value;
+    if (head_dim == 128) return form ? launch<128, F, true>(a, sr, sk, st) : launch<128, F, false>(a, sr, sk, st);
+    return form ? launch<64, F, true>(a, sr, sk, st) : launch<64, F, false>(a, sr, sk, st);
+  });
+}

@@ -1,0 +1,265 @@
+"""A paged K/V cache for requests of different lengths: its page table, its
+writes and the attention over it (MI355X).
+
+K and V lie in pages of ``page`` tokens that requests take from one pool:
+``k_pages`` / ``v_pages`` [pages, Hkv, page, D] (bf16 or fp16), and
+``table`` int32 [requests, width] holds the page of each request's token t at
+t // page.  A serving step does, once,
+
+1. ``plan_step``  -- pages for the step's new tokens from the stack of free
+                    ones, and each row's slot and position, decided on the
+                    GPU from the request lengths (``PageTable.step``);
+
+then for each layer
+
+2. ``append``     -- the rows' K and V into their slots;
+3. ``attention``  -- the rows over the cache: single tokens, drafted tokens,
+                    chunks of prompts, whole prompts, mixed as they come;
+                    scores may be capped by a tanh and biased by distance,
+                    the mask may have a two-sided prefix and documents;
+
+and ``release_pages`` gives back the pages of requests that ended or of
+tokens that were rejected.  No length is needed on the host, so a step can be
+captured into a graph and replayed while the requests grow.
+
+No reference counterpart: the reference keeps HF's dense cache, every
+sequence of a batch at one length, and prefills with dense attention
+(evaluate_qwen3_top2_head_limit3_ppl.py:7079-7111).  Everything runs on the
+GPU on the current stream and raises RuntimeError on bad input.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+
+
+def _require(cond: bool, msg: str) -> None:
+    if not cond:
+        raise RuntimeError(msg)
+
+
+class StepPlan(NamedTuple):
+    """What ``plan_step`` decides of a step: request b's rows are
+    ``cu_rows[b] .. cu_rows[b + 1] - 1`` and it holds ``kv_lens[b]`` tokens
+    after the step (0 if it was not served); ``slots`` and ``positions`` of
+    every row (-1 where it has no token); ``failed`` [1] counts the requests
+    whose new tokens found no room."""
+
+    cu_rows: torch.Tensor     # int32 [requests + 1]
+    kv_lens: torch.Tensor     # int32 [requests]
+    slots: torch.Tensor       # int64 [rows]
+    positions: torch.Tensor   # int32 [rows]
+    failed: torch.Tensor      # int32 [1]
+
+    @classmethod
+    def empty(cls, requests: int, rows: int, device) -> "StepPlan":
+        """Buffers for a step of ``rows`` rows (allocated as one)."""
+        words = torch.empty(2 * rows + rows + 2 * requests + 2, dtype=torch.int32, device=device)
+        slots, positions, cu, kv, failed = words.split([2 * rows, rows, requests + 1, requests, 1])
+        return cls(cu, kv, slots.view(torch.int64), positions, failed)
+
+
+def _i32(name: str, t: torch.Tensor, n: int, device) -> None:
+    if t.dtype != torch.int32 or t.device != device or t.dim() != 1 or t.size(0) != n or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous int32 [{n}] on {device}")
+
+
+def _check_table(table: torch.Tensor) -> None:
+    if not table.is_cuda or table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1:
+        raise RuntimeError("table must be CUDA int32 [requests, width] with contiguous rows")
+
+
+def plan_step(new_lens: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, free: torch.Tensor,
+              count: torch.Tensor, page: int, rows: int, *, padded: int = 0, out: StepPlan | None = None) -> StepPlan:
+    """Adds ``new_lens[b]`` tokens to every request: takes their pages from
+    the stack ``free`` int32 [pages] (``count`` int32 [1] entries, top last)
+    into ``table`` int32 [requests, width], raises ``lens`` int32 [requests],
+    and gives every one of the step's ``rows`` rows its slot and position.
+
+    Rows are packed, ``new_lens[b]`` for each request, or, with ``padded`` =
+    n, n for each with its tokens last (a left-padded batch; ``rows`` is then
+    requests * n).  Rows behind the last request's have no token.  A request
+    whose tokens do not fit its table row, the pool or ``rows`` is left as it
+    is, with kv_lens 0, and counted in ``failed``.  At most 4096 requests,
+    2^20 pages, 2^20 rows; ``page`` a power of two in [16, 4096]."""
+    lib = _lib.load()
+    _check_table(table)
+    n, dev = table.size(0), table.device
+    _i32("new_lens", new_lens, n, dev)
+    _i32("lens", lens, n, dev)
+    _i32("free", free, free.numel(), dev)
+    _i32("count", count, 1, dev)
+    if out is None:
+        out = StepPlan.empty(n, rows, dev)
+    else:
+        _i32("out.cu_rows", out.cu_rows, n + 1, dev)
+        _i32("out.kv_lens", out.kv_lens, n, dev)
+        _i32("out.positions", out.positions, rows, dev)
+        _i32("out.failed", out.failed, 1, dev)
+        _check_slots(out.slots, rows, dev)
+    with _lib.on_device(dev):
+        _lib.check(lib.qkv_paged_plan(new_lens.data_ptr(), table.data_ptr(), table.stride(0), lens.data_ptr(),
+                                      free.data_ptr(), count.data_ptr(), n, table.size(1), free.size(0), page, rows,
+                                      padded, out.cu_rows.data_ptr(), out.kv_lens.data_ptr(), out.slots.data_ptr(),
+                                      out.positions.data_ptr(), out.failed.data_ptr(), _lib.stream_of(table)))
+    return out
+
+
+def release_pages(keep: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, free: torch.Tensor,
+                  count: torch.Tensor, page: int) -> None:
+    """Cuts every request to its first ``keep[b]`` tokens (0 ends it, its
+    length or more leaves it) and gives the pages behind them back to
+    ``free``; the last step's tokens released leave the stack as it was."""
+    lib = _lib.load()
+    _check_table(table)
+    n, dev = table.size(0), table.device
+    _i32("keep", keep, n, dev)
+    _i32("lens", lens, n, dev)
+    _i32("free", free, free.numel(), dev)
+    _i32("count", count, 1, dev)
+    with _lib.on_device(dev):
+        _lib.check(lib.qkv_paged_release(keep.data_ptr(), table.data_ptr(), table.stride(0), lens.data_ptr(),
+                                         free.data_ptr(), count.data_ptr(), n, table.size(1), free.size(0), page,
+                                         _lib.stream_of(table)))
+
+
+class PageTable:
+    """The page table of ``requests`` requests of at most ``capacity`` tokens
+    over a pool of ``pages`` pages, one for all layers: ``table``, ``lens``,
+    ``free`` and ``count`` as ``plan_step`` takes them, all on the GPU."""
+
+    def __init__(self, requests: int, capacity: int, pages: int, page: int, device):
+        _require(requests >= 1 and capacity >= 1 and pages >= 1, "requests, capacity and pages must be positive")
+        _require(16 <= page <= 4096 and page & (page - 1) == 0, "page must be a power of two in [16, 4096]")
+        self.page, self.pages, self.capacity = int(page), int(pages), int(capacity)
+        dev = torch.device(device)
+        self.table = torch.full((requests, -(-capacity // page)), -1, dtype=torch.int32, device=dev)
+        self.lens = torch.zeros(requests, dtype=torch.int32, device=dev)
+        self.free = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=dev)   # page 0 on top
+        self.count = torch.full((1,), pages, dtype=torch.int32, device=dev)
+
+    def step(self, new_lens: torch.Tensor, rows: int, *, padded: int = 0, out: StepPlan | None = None) -> StepPlan:
+        """``plan_step`` on this table."""
+        return plan_step(new_lens, self.table, self.lens, self.free, self.count, self.page, rows, padded=padded,
+                         out=out)
+
+    def release(self, keep: torch.Tensor) -> None:
+        """``release_pages`` on this table."""
+        release_pages(keep, self.table, self.lens, self.free, self.count, self.page)
+
+
+def _check_slots(slots: torch.Tensor, rows: int, device) -> None:
+    if (slots.dtype != torch.int64 or slots.device != device or slots.dim() != 1 or slots.size(0) != rows
+            or not slots.is_contiguous()):
+        raise RuntimeError(f"slots must be contiguous int64 [{rows}] on {device}")
+
+
+def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor) -> int:
+    """Checks a layer's pages; returns their dtype code."""
+    code = _lib.half_code("k_pages", k_pages)
+    if (not k_pages.is_cuda or k_pages.dim() != 4 or k_pages.shape != v_pages.shape or v_pages.dtype != k_pages.dtype
+            or v_pages.device != k_pages.device or k_pages.stride(3) != 1 or v_pages.stride(3) != 1):
+        raise RuntimeError("k_pages and v_pages must be CUDA [pages, kv_heads, page, dim] of one shape, dtype and "
+                           "device with contiguous channels")
+    return code
+
+
+def append(key: torch.Tensor, value: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+           slots: torch.Tensor) -> None:
+    """Writes the rows' K and V, [rows, Hkv, D] at any strides with contiguous
+    channels, to their ``slots`` (int64 [rows], as ``plan_step`` gives them;
+    a row with -1 is skipped, no slot may come twice)."""
+    lib = _lib.load()
+    _check_pages(k_pages, v_pages)
+    pages, heads, page, dim = k_pages.shape
+    for name, t in (("key", key), ("value", value)):
+        if (t.dim() != 3 or t.size(1) != heads or t.size(2) != dim or t.dtype != k_pages.dtype
+                or t.device != k_pages.device or t.stride(2) != 1):
+            raise RuntimeError(f"{name} must be {k_pages.dtype} [rows, {heads}, {dim}] on {k_pages.device} with "
+                               "contiguous channels")
+    rows = key.size(0)
+    _require(value.size(0) == rows, "key and value must have as many rows")
+    _check_slots(slots, rows, key.device)
+    with _lib.on_device(key.device):
+        _lib.check(lib.qkv_paged_append(key.data_ptr(), _lib.strides(*key.stride()[:2]), value.data_ptr(),
+                                        _lib.strides(*value.stride()[:2]), k_pages.data_ptr(),
+                                        _lib.strides(*k_pages.stride()[:3]), v_pages.data_ptr(),
+                                        _lib.strides(*v_pages.stride()[:3]), pages, page, heads, dim,
+                                        slots.data_ptr(), rows, _lib.stream_of(key)))
+
+
+def attention_workspace(rows: int, max_rows: int, requests: int, width: int, page: int, q_heads: int, kv_heads: int,
+                        head_dim: int, device) -> torch.Tensor:
+    """A workspace for ``attention`` calls of these sizes (contents
+    irrelevant).  Calls that share one must not overlap in time."""
+    need = _lib.load().qkv_paged_attention_workspace_bytes(rows, max_rows, requests, width, page, q_heads, kv_heads,
+                                                           head_dim)
+    _require(need >= 0, "attention_workspace: sizes that attention does not take")
+    return torch.empty(need // 4, dtype=torch.float32, device=device)
+
+
+def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+              cu_rows: torch.Tensor, kv_lens: torch.Tensor, scaling: float, *, max_rows: int | None = None,
+              softcap: float = 0.0, slopes: torch.Tensor | None = None, prefix_lens: torch.Tensor | None = None,
+              first_keys: torch.Tensor | None = None, out: torch.Tensor | None = None,
+              workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """query [rows, Hq, D] over the cached keys of the rows' requests, whose
+    own K and V were appended before.  Row i of request b is the token at
+    p = kv_lens[b] - (cu_rows[b + 1] - cu_rows[b]) + i and sees the keys j
+    with first_keys[row] <= j < max(p + 1, prefix_lens[b]) that the request
+    holds; a row that sees none gets zeros.
+
+    ``softcap`` > 0 caps scores to softcap * tanh(scaling * q.k / softcap);
+    ``slopes`` f32 [Hq] then takes slopes[h] * |p - j| off; ``prefix_lens``
+    int32 [requests] opens the first keys to every row; ``first_keys`` int32
+    [rows] hides the keys before a row's document (or window: p + 1 - w).
+    ``max_rows``, the most rows a request has where the caller knows it,
+    spares launches (1 in a decode step); the result does not depend on it.
+    ``workspace`` (``attention_workspace``) spares an allocation.  Returns
+    [rows, Hq, D] in the query's dtype; rows of ``out`` behind the last
+    request are left as they were."""
+    lib = _lib.load()
+    code = _check_pages(k_pages, v_pages)
+    _check_table(table)
+    pages, kv_heads, page, dim = k_pages.shape
+    dev = k_pages.device
+    if (query.dim() != 3 or query.size(2) != dim or query.dtype != k_pages.dtype or query.device != dev
+            or query.stride(2) != 1):
+        raise RuntimeError(f"query must be {k_pages.dtype} [rows, q_heads, {dim}] on {dev} with contiguous channels")
+    rows, q_heads = query.size(0), query.size(1)
+    n, width = table.shape
+    _require(table.device == dev, f"table must be on {dev}")
+    _i32("cu_rows", cu_rows, n + 1, dev)
+    _i32("kv_lens", kv_lens, n, dev)
+    if prefix_lens is not None:
+        _i32("prefix_lens", prefix_lens, n, dev)
+    if first_keys is not None:
+        _i32("first_keys", first_keys, rows, dev)
+    if slopes is not None:
+        _require(slopes.dtype == torch.float32 and slopes.device == dev and slopes.shape == (q_heads,)
+                 and slopes.is_contiguous(), f"slopes must be contiguous float32 [{q_heads}] on {dev}")
+    if out is None:
+        out = torch.empty((rows, q_heads, dim), dtype=query.dtype, device=dev)
+    else:
+        _require(out.shape == query.shape and out.dtype == query.dtype and out.device == dev and out.stride(2) == 1,
+                 "out must have the query's shape, dtype and device with contiguous channels")
+    most = rows if max_rows is None else max_rows
+    need = lib.qkv_paged_attention_workspace_bytes(rows, most, n, width, page, q_heads, kv_heads, dim)
+    if workspace is None:
+        if need > 0:
+            workspace = torch.empty(need // 4, dtype=torch.float32, device=dev)
+    else:
+        _require(workspace.device == dev and workspace.is_contiguous(), f"workspace must be contiguous on {dev}")
+    with _lib.on_device(dev):
+        _lib.check(lib.qkv_paged_attention(
+            query.data_ptr(), _lib.strides(*query.stride()[:2]), k_pages.data_ptr(),
+            _lib.strides(*k_pages.stride()[:3]), v_pages.data_ptr(), _lib.strides(*v_pages.stride()[:3]), pages, page,
+            table.data_ptr(), table.stride(0), width, n, cu_rows.data_ptr(), kv_lens.data_ptr(), rows, most, q_heads,
+            kv_heads, dim, scaling, softcap, _lib.ptr(slopes), _lib.ptr(prefix_lens), _lib.ptr(first_keys),
+            _lib.ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
+            out.data_ptr(), _lib.strides(*out.stride()[:2]), code, _lib.stream_of(query)))
+    return out

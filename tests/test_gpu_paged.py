@@ -1,0 +1,626 @@
+"""Paged K/V cache on the GPU against plain implementations in 64 bits: the
+page table's steps against a list-based allocator, the writes bit for bit,
+and the attention within a bound that counts its roundings (the weights' and
+the output's, half a step each; the scores' and sums' in 32 bits)."""
+
+import random
+
+import pytest
+import torch
+
+from kv_cache_amd import paged
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+# -- page table -------------------------------------------------------------------
+
+
+class Model:
+    """The page table of lists."""
+
+    def __init__(self, requests, capacity, pages, page):
+        self.page, self.width = page, -(-capacity // page)
+        self.held, self.lens = [[] for _ in range(requests)], [0] * requests
+        self.free = list(range(pages - 1, -1, -1))
+
+    def step(self, new, rows, padded=0):
+        count, asked, at, failed = len(self.free), 0, 0, 0
+        cu, kv, slots, positions, fresh = [0], [], [-1] * rows, [-1] * rows, []
+        for b, n in enumerate(new):
+            n = max(n, 0)
+            want = -(-(self.lens[b] + n) // self.page)
+            fits = want <= self.width and (not padded or n <= padded)
+            need = want - len(self.held[b]) if fits else 0
+            asked += need
+            at += padded or n
+            served = fits and (need == 0 or asked <= count) and at <= rows
+            got = [self.free[count - 1 - (asked - need) - k] for k in range(need)] if served else []
+            fresh.append((served, got))
+            failed += (not served) and n > 0
+            kv.append(self.lens[b] + n if served else 0)
+            cu.append(min(at, rows))
+        taken = sum(len(g) for _, g in fresh)
+        self.free = self.free[: count - taken]
+        for b, (served, got) in enumerate(fresh):
+            n = max(new[b], 0)
+            self.held[b] += got
+            if not served:
+                continue
+            for i in range(n):
+                row, p = cu[b + 1] - n + i, self.lens[b] + i
+                slots[row], positions[row] = self.held[b][p // self.page] * self.page + p % self.page, p
+            self.lens[b] += n
+        return cu, kv, slots, positions, failed
+
+    def release(self, keep):
+        back = []
+        for b, n in enumerate(keep):
+            n = min(max(n, 0), self.lens[b])
+            stay = -(-n // self.page)
+            back += self.held[b][stay:]
+            self.held[b], self.lens[b] = self.held[b][:stay], n
+        self.free += back[::-1]
+
+    def check(self, t):
+        assert t.lens.tolist() == self.lens
+        n = int(t.count)
+        assert t.free[:n].tolist() == self.free
+        for b, row in enumerate(t.table.tolist()):
+            assert row[: len(self.held[b])] == self.held[b] and set(row[len(self.held[b]):]) <= {-1}
+
+
+def _same_step(model, table, new, rows, padded=0, out=None):
+    want = model.step(new, rows, padded)
+    got = table.step(_i32(new), rows, padded=padded, out=out)
+    assert got.cu_rows.tolist() == want[0]
+    assert got.kv_lens.tolist() == want[1]
+    assert got.slots.tolist() == want[2]
+    assert got.positions.tolist() == want[3]
+    assert int(got.failed) == want[4]
+    model.check(table)
+    return got
+
+
+@pytest.mark.parametrize("requests,capacity,pages,page,most", [
+    (1, 16, 1, 16, 1), (1, 100, 7, 16, 40), (3, 257, 40, 16, 70), (64, 500, 300, 32, 9), (65, 130, 200, 64, 5),
+    (1024, 64, 1500, 16, 3), (1025, 64, 2100, 16, 4), (4096, 32, 5000, 16, 2), (7, 5000, 90, 128, 3000)])
+def test_steps_and_releases(requests, capacity, pages, page, most):
+    rng = random.Random(requests * 7 + page)
+    model, table = Model(requests, capacity, pages, page), paged.PageTable(requests, capacity, pages, page, DEV)
+    for i in range(8):
+        new = [rng.choice([0, 1, 1, rng.randint(0, most)]) for _ in range(requests)]
+        if i == 3:
+            new[rng.randrange(requests)] = -5
+        # room for all rows and some more; sometimes too few
+        rows = max(1, sum(max(n, 0) for n in new) + rng.choice([0, 3, -2]))
+        _same_step(model, table, new, rows)
+        keep = [rng.choice([n, n, max(0, n - 1), n // 2, 0, n + 9, -1]) for n in model.lens]
+        model.release(keep)
+        table.release(_i32(keep))
+        model.check(table)
+
+
+@pytest.mark.parametrize("rows", [1, 4095, 4096, 4097, 9001])
+def test_many_rows(rows):
+    # one launch writes the slots of up to 4096 rows, two those of more
+    model, table = Model(5, 20000, 800, 32), paged.PageTable(5, 20000, 800, 32, DEV)
+    _same_step(model, table, [17, 0, 1, 33, 64], 200)
+    _same_step(model, table, [rows // 3, 0, rows - rows // 3 - rows // 7, rows // 7, 0], rows)
+    _same_step(model, table, [1, 1, 0, 1, 1], 4)
+
+
+def test_padded_rows():
+    model, table = Model(4, 300, 40, 16), paged.PageTable(4, 300, 40, 16, DEV)
+    got = _same_step(model, table, [7, 20, 0, 20], 80, padded=20)
+    assert got.positions.view(4, 20)[0].tolist() == [-1] * 13 + list(range(7))
+    _same_step(model, table, [1, 1, 1, 1], 4, padded=1)
+    _same_step(model, table, [3, 21, 1, 0], 80, padded=20)   # more tokens than rows: not served
+
+
+def test_pool_and_table_run_out():
+    model, table = Model(4, 64, 6, 16), paged.PageTable(4, 64, 6, 16, DEV)
+    got = _same_step(model, table, [40, 40, 1, 1], 100)      # 3 + 3 pages; the other two find none
+    assert int(got.failed) == 2
+    got = _same_step(model, table, [8, 30, 0, 0], 100)       # inside the last page; past the table row
+    assert int(got.failed) == 1 and table.lens.tolist() == [48, 40, 0, 0]
+    model.release([0, 99, 0, 0])
+    table.release(_i32([0, 99, 0, 0]))
+    _same_step(model, table, [1, 0, 1, 1], 3)
+
+
+def test_release_undoes_a_step():
+    table = paged.PageTable(9, 400, 120, 16, DEV)
+    table.step(_i32([5, 16, 17, 100, 0, 1, 31, 32, 33]), 300)
+    before = [t.clone() for t in (table.table, table.lens, table.count, table.free)]
+    table.step(_i32([7] * 9), 63)
+    table.release(before[1])
+    for t, b in zip((table.table, table.lens, table.count, table.free), before):
+        assert torch.equal(t, b)
+
+
+# -- writes -----------------------------------------------------------------------
+
+
+def _pages(pages, heads, page, dim, dt, seed, token_major=False):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    shape = (pages, page, heads, dim) if token_major else (pages, heads, page, dim)
+    x = torch.randn(shape, generator=g, device=DEV).to(dt)
+    return x.transpose(1, 2) if token_major else x
+
+
+@pytest.mark.parametrize("rows,heads,dim,page,dt,layout", [
+    (1, 1, 64, 16, "bf16", "plain"), (37, 8, 128, 16, "fp16", "plain"), (300, 3, 64, 64, "bf16", "heads_first"),
+    (300, 2, 128, 32, "bf16", "token_major"), (65, 5, 40, 128, "fp16", "unaligned")])
+def test_append(rows, heads, dim, page, dt, layout):
+    rng = random.Random(rows)
+    pages = -(-rows // page) + 3
+    kp, vp = (_pages(pages, heads, page, dim, DT[dt], s, layout == "token_major") for s in (1, 2))
+    g = torch.Generator(device=DEV).manual_seed(3)
+    if layout == "heads_first":
+        k, v = (torch.randn((heads, rows, dim), generator=g, device=DEV).to(DT[dt]).transpose(0, 1) for _ in range(2))
+    elif layout == "unaligned":
+        k, v = (torch.randn((rows, heads, dim + 3), generator=g, device=DEV).to(DT[dt])[..., 1:1 + dim] for _ in range(2))
+    else:
+        k, v = (torch.randn((rows, heads, dim), generator=g, device=DEV).to(DT[dt]) for _ in range(2))
+    at = rng.sample(range(pages * page), rows)
+    at[0] = -1 if rows > 1 else at[0]
+    if rows > 2:
+        at[2] = pages * page + 5   # outside the cache: skipped
+    want_k, want_v = kp.clone(), vp.clone()
+    for r, s in enumerate(at):
+        if 0 <= s < pages * page:
+            want_k[s // page, :, s % page], want_v[s // page, :, s % page] = k[r], v[r]
+    paged.append(k, v, kp, vp, torch.tensor(at, device=DEV))
+    assert torch.equal(kp, want_k) and torch.equal(vp, want_v)
+
+
+# -- attention ----------------------------------------------------------------------
+
+
+def _case(kv, rows, hq, hkv, dim, page, dt, seed=0, spare=2, token_major=False):
+    """Pages in random order; NaN behind every request's last token and in the pages nobody holds."""
+    rng = random.Random(seed)
+    need = [-(-n // page) for n in kv]
+    pool = sum(need) + spare
+    order = list(range(pool))
+    rng.shuffle(order)
+    table, at = torch.full((len(kv), max(need + [1]) + 1), -1, dtype=torch.int32), 0
+    kp, vp = (_pages(pool, hkv, page, dim, DT[dt], seed * 10 + s, token_major) for s in (1, 2))
+    for b, n in enumerate(need):
+        ids = order[at: at + n]
+        at += n
+        table[b, :n] = torch.tensor(ids, dtype=torch.int32)
+        if kv[b] % page:
+            kp[ids[-1], :, kv[b] % page:] = float("nan")
+            vp[ids[-1], :, kv[b] % page:] = float("nan")
+    for p in order[at:]:
+        kp[p] = vp[p] = float("nan")
+    cu = [0]
+    for n in rows:
+        cu.append(cu[-1] + n)
+    g = torch.Generator(device=DEV).manual_seed(seed * 10 + 3)
+    q = torch.randn((cu[-1], hq, dim), generator=g, device=DEV).to(DT[dt])
+    return dict(query=q, k_pages=kp, v_pages=vp, table=table.to(DEV), cu_rows=_i32(cu), kv_lens=_i32(kv),
+                scaling=dim ** -0.5)
+
+
+def _reference(c, softcap=0.0, slopes=None, prefix_lens=None, first_keys=None):
+    """(out, bound) in 64 bits.  The bound of an element counts, for every key j with weight w_j:
+    the weight's rounding to the dtype (half a step h), the score's error e_j in 32 bits -- the
+    product (dim + 8 roundings of sum |q k|), tanh (2^-20 of the score) and bias (2^-22), doubled for
+    the sum of the weights -- the exponential and the sums (n + 64 roundings); then the output's own
+    rounding h.  fp16 weights below 2^-14 (scaled by 2^6) are off by 2^-25 at most: n 2^-31 of the largest."""
+    q, kp, vp = c["query"], c["k_pages"], c["v_pages"]
+    page, dim = kp.shape[2], kp.shape[3]
+    group = q.shape[1] // kp.shape[1]
+    cu, kv = c["cu_rows"].tolist(), c["kv_lens"].tolist()
+    out = torch.zeros(q.shape, dtype=torch.float64, device=DEV)
+    tol = torch.zeros_like(out)
+    h = torch.finfo(q.dtype).eps / 2
+    for b, n in enumerate(kv):
+        m = cu[b + 1] - cu[b]
+        if m == 0 or n == 0:
+            continue
+        ids = c["table"][b, : -(-n // page)].long()
+        ok = ((ids >= 0) & (ids < kp.shape[0])).repeat_interleave(page)[:n]
+        ids = ids.clamp(0, kp.shape[0] - 1)
+        p = torch.arange(n - m, n, device=DEV)[:, None]
+        j = torch.arange(n, device=DEV)
+        last = p + 1 if prefix_lens is None else (p + 1).clamp(min=int(prefix_lens[b]))
+        seen = (j < last) & (p >= 0) & ok
+        if first_keys is not None:
+            seen &= j >= first_keys[cu[b]: cu[b + 1]].long()[:, None]
+        for head in range(q.shape[1]):
+            k = kp[ids, head // group].reshape(-1, dim)[:n].double()
+            v = vp[ids, head // group].reshape(-1, dim)[:n].double()
+            v = torch.where(seen.any(0)[:, None], v, 0.0)
+            k = torch.where(seen.any(0)[:, None], k, 0.0)
+            x = q[cu[b]: cu[b + 1], head].double()
+            s = x @ k.t().contiguous() * c["scaling"]
+            e = (dim + 8) * 2.0 ** -24 * c["scaling"] * (x.abs() @ k.abs().t().contiguous())
+            if softcap:
+                s = softcap * torch.tanh(s / softcap)
+                e += 2.0 ** -20 * s.abs()
+            if slopes is not None:
+                bias = slopes[head].double() * (p - j).abs()
+                s = s - bias
+                e += 2.0 ** -22 * (bias + s.abs())
+            s = torch.where(seen, s, -torch.inf)
+            none = ~seen.any(1)
+            w = torch.softmax(torch.where(none[:, None], 0.0, s), -1)
+            w[none] = 0.0
+            w = torch.where(seen, w, 0.0)
+            # only rows that see a key take its value, infinities included
+            odd = ~torch.isfinite(v)
+            y = w @ torch.where(odd, 0.0, v)
+            for key, d in odd.nonzero().tolist():
+                y[seen[:, key], d] += v[key, d]
+            out[cu[b]: cu[b + 1], head] = y
+            av = torch.where(odd, 0.0, v.abs())
+            we = w * (2 * e + 2.0 ** -20 + (n + 64) * 2.0 ** -24)
+            t = h * (w @ av) + we @ av + we.sum(1, keepdim=True) * (w @ av) + h * y.abs()
+            if q.dtype == torch.float16:
+                t = t + n * 2.0 ** -31 * w.amax(1, keepdim=True) * av.amax(0) + 2.0 ** -25
+            tol[cu[b]: cu[b + 1], head] = 1.02 * t
+    return out, tol
+
+
+def _check(c, **form):
+    hints = {k: form.pop(k) for k in ("max_rows", "workspace", "out") if k in form}
+    want, tol = _reference(c, **form)
+    got = paged.attention(**c, **form, **hints)
+    _within(got, want, tol)
+    return got
+
+
+def _within(got, want, tol):
+    g = got.double()
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isnan(g), torch.isnan(want))
+    assert torch.equal(g[~fine & ~torch.isnan(want)], want[~fine & ~torch.isnan(want)])
+    off = ((g - want).abs() / tol.clamp(min=1e-30))[fine]
+    assert off.numel() == 0 or float(off.max()) <= 1.0, float(off.max())
+
+
+HEADS = [(2, 2, 64), (4, 2, 128), (6, 2, 64), (8, 2, 128), (16, 1, 128), (24, 1, 64), (34, 2, 128)]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("hq,hkv,dim", HEADS)
+def test_single_tokens(hq, hkv, dim, dt):
+    kv = [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 0, 200, 256, 257, 700]
+    _check(_case(kv, [1] * len(kv), hq, hkv, dim, 16, dt, seed=1), max_rows=1)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("hq,hkv,dim", HEADS)
+def test_chunks(hq, hkv, dim, dt):
+    kv, rows = [1, 5, 33, 64, 129, 300, 431, 0], [1, 5, 2, 64, 65, 9, 130, 0]
+    _check(_case(kv, rows, hq, hkv, dim, 32, dt, seed=2))
+
+
+@pytest.mark.parametrize("page", [16, 64, 256, 4096])
+@pytest.mark.parametrize("token_major", [False, True])
+def test_pages(page, token_major):
+    c = _case([1, 100, 515, 1025], [1, 40, 3, 1], 4, 2, 128, page, "bf16", seed=3, token_major=token_major)
+    _check(c)
+
+
+@pytest.mark.parametrize("hq,hkv,dim,dt", [(8, 2, 128, "bf16"), (3, 1, 64, "fp16"), (40, 2, 64, "bf16")])
+def test_split_keys(hq, hkv, dim, dt):
+    # few rows over long caches: several workgroups a tile, joined by a second launch
+    for kv, rows in (([5000], [1]), ([3001, 70, 2048], [2, 70, 1]), ([2500, 2600], [40, 3]), ([4097], [130])):
+        _check(_case(kv, rows, hq, hkv, dim, 16, dt, seed=4))
+
+
+def test_split_and_unsplit_requests_and_hint():
+    c = _case([6000, 3, 900, 40, 0, 257], [1, 1, 1, 1, 1, 1], 8, 2, 128, 64, "bf16", seed=5)
+    a = _check(c, max_rows=1)
+    b = _check(c)
+    assert torch.equal(a, b)   # the hint changes launches, not the work
+    c = _case([600, 300, 50], [9, 30, 5], 8, 2, 128, 64, "bf16", seed=6)
+    _check(c, max_rows=1)      # a wrong hint costs time only
+    _check(c, max_rows=4)
+
+
+def test_many_requests():
+    rng = random.Random(7)
+    kv = [rng.choice([0, 1, rng.randint(1, 90)]) for _ in range(700)]
+    kv[650] = 3000
+    rows = [min(n, rng.choice([0, 1, 1, 1, 20])) for n in kv]
+    _check(_case(kv, rows, 4, 2, 64, 16, "bf16", seed=7))
+
+
+FORMS = ["cap", "bias", "cap_bias", "prefix", "documents", "prefix_documents_bias", "window"]
+
+
+@pytest.mark.parametrize("dt,dim", [("bf16", 128), ("fp16", 64)])
+@pytest.mark.parametrize("form", FORMS)
+def test_forms(form, dt, dim):
+    kv, rows = [1, 77, 300, 513, 40], [1, 77, 140, 2, 1]
+    c = _case(kv, rows, 8, 2, dim, 16, dt, seed=8)
+    f = {}
+    if "cap" in form:
+        f["softcap"] = 5.0
+    if "bias" in form:
+        f["slopes"] = torch.tensor([2.0 ** -i for i in range(8)], device=DEV)
+    if "prefix" in form:
+        f["prefix_lens"] = _i32([3, 50, 299, 0, 1000])
+    at = torch.cat([torch.arange(n - m, n) for n, m in zip(kv, rows)])
+    if "documents" in form:
+        f["first_keys"] = (at // 37 * 37).int().to(DEV)
+    if form == "window":
+        f["first_keys"] = (at - 63).int().to(DEV)   # below zero for the first tokens
+    _check(c, **f)
+
+
+def test_large_cap_is_exact():
+    c = _case([300, 90], [20, 1], 4, 2, 128, 16, "bf16", seed=9)
+    _check(c, softcap=1.0e6)
+    _check(c, softcap=0.05)
+
+
+def test_large_scores():
+    c = _case([400, 333], [30, 1], 4, 2, 128, 16, "fp16", seed=10)
+    c["query"] = c["query"] * 30
+    _check(c)
+    _check(c, slopes=torch.tensor([0.0, 1.0, 100.0, 1e5], device=DEV))
+
+
+def test_rows_that_see_nothing():
+    kv, rows = [50, 200, 5], [50, 3, 1]
+    c = _case(kv, rows, 4, 2, 128, 16, "bf16", seed=11)
+    first = torch.zeros(54, dtype=torch.int32)
+    first[3:7], first[51], first[53] = 50, 10 ** 6, 5
+    got = _check(c, first_keys=first.to(DEV))
+    assert (got[3:7] == 0).all() and (got[51] == 0).all() and (got[53] == 0).all()
+    # every row of a request, and of a whole call
+    got = _check(c, first_keys=torch.full((54,), 10 ** 6, dtype=torch.int32, device=DEV))
+    assert (got == 0).all()
+
+
+def test_left_padding_and_requests_without_tokens():
+    # more rows than tokens: the first rows are padding and get zeros; a request not served has kv_lens 0
+    for rows in ([40, 40, 40], [3, 3, 3]):
+        c = _case([17, 40, 0] if rows[0] == 40 else [1, 300, 0], rows, 8, 2, 128, 16, "bf16", seed=12)
+        got = _check(c, prefix_lens=_i32([9, 9, 9]))
+        assert (got[2 * rows[0]:] == 0).all()
+
+
+def test_rows_behind_the_last_request_stay():
+    c = _case([30, 100], [30, 1], 8, 2, 128, 16, "bf16", seed=13)
+    n = c["query"].shape[0]
+    c["query"] = torch.cat([c["query"], torch.full((9, 8, 128), float("nan"), device=DEV, dtype=torch.bfloat16)])
+    out = torch.full_like(c["query"], 7.0)
+    want, tol = _reference({**c, "query": c["query"][:n]})
+    got = paged.attention(**c, out=out)
+    assert got is out and (out[n:] == 7.0).all()
+    _within(out[:n], want, tol)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows", [[60, 1], [2, 1], [200, 1]])
+def test_infinities_and_nan_in_masked_places(rows, dt):
+    kv = [max(rows[0], 90) + 5, 400]
+    c = _case(kv, rows, 4, 2, 128, 16, dt, seed=14)
+    page, n = 16, kv[0]
+
+    def put(pages, b, t, d, x):
+        pages[int(c["table"][b, t // page]), :, t % page, d] = x
+
+    # V of the request's last tokens: rows before them do not see it, the last row does
+    put(c["v_pages"], 0, n - 1, 5, float("inf"))
+    put(c["v_pages"], 0, n - 1, 6, float("nan"))
+    put(c["v_pages"], 0, n - 2, 7, float("-inf"))
+    got = _check(c)
+    assert torch.isinf(got[rows[0] - 1, :, 5]).all() and torch.isfinite(got[: rows[0] - 2]).all()
+    # hidden by the documents' mask, K too
+    put(c["k_pages"], 1, 3, 0, float("nan"))
+    put(c["k_pages"], 1, 70, 1, float("inf"))
+    put(c["v_pages"], 1, 70, 0, float("nan"))
+    put(c["v_pages"], 1, 3, 0, float("-inf"))
+    first = torch.zeros(sum(rows), dtype=torch.int32)
+    first[-1] = 71
+    got = _check(c, first_keys=first.to(DEV))
+    assert torch.isfinite(got[-1]).all()
+
+
+def test_table_entries_outside_the_pool():
+    c = _case([200, 90, 40], [30, 1, 40], 8, 2, 128, 16, "bf16", seed=15)
+    c["table"][0, 3], c["table"][1, 0], c["table"][2, 2] = -1, 10 ** 9, c["k_pages"].shape[0]
+    _check(c)
+    # lengths past the table row are read as the row's end
+    c = _case([100], [1], 4, 2, 64, 16, "bf16", seed=16)
+    full = torch.full((1, 7), 0, dtype=torch.int32, device=DEV)
+    full[0] = c["table"][0, 0]
+    got = paged.attention(**{**c, "table": full, "kv_lens": _i32([10 ** 6])}, first_keys=_i32([0]))
+    assert torch.isfinite(got).all()
+
+
+def test_cu_rows_out_of_range():
+    # not ascending, negative, past the rows: in bounds, and the well-formed requests are right
+    c = _case([50, 60, 70], [10, 10, 10], 8, 2, 128, 16, "bf16", seed=17)
+    want, tol = _reference(c)
+    bad = {**c, "cu_rows": _i32([-5, 10, 20, 1000])}
+    got = paged.attention(**bad)
+    _within(got[10:20], want[10:20], tol[10:20])
+    paged.attention(**{**c, "cu_rows": _i32([30, 0, 30, 0])})
+    torch.cuda.synchronize()
+
+
+def test_strides():
+    c = _case([77, 300, 1], [40, 1, 1], 8, 2, 128, 16, "bf16", seed=18)
+    want, tol = _reference(c)
+    q = c["query"]
+    g = torch.empty((8, 42, 131), dtype=q.dtype, device=DEV)        # heads first, unaligned rows
+    odd = g[..., 1:129].transpose(0, 1)
+    odd.copy_(q)
+    wide = torch.zeros((42, 8, 256), dtype=q.dtype, device=DEV)
+    out = wide[..., 128:]
+    got = paged.attention(**{**c, "query": odd}, out=out)
+    assert got is out and (wide[..., :128] == 0).all()
+    _within(out, want, tol)
+    table = torch.full((3, 40), 5, dtype=torch.int32, device=DEV)
+    table[:, : c["table"].shape[1]] = c["table"]
+    _within(paged.attention(**{**c, "table": table[:, : c["table"].shape[1]]}), want, tol)
+
+
+def test_workspace():
+    c = _case([3000, 20], [1, 60], 8, 2, 128, 16, "bf16", seed=19)
+    ws = paged.attention_workspace(61, 61, 2, c["table"].shape[1], 16, 8, 2, 128, DEV)
+    a = paged.attention(**c, workspace=ws)
+    ws.fill_(float("nan"))
+    assert torch.equal(paged.attention(**c, workspace=ws), a)
+    assert torch.equal(paged.attention(**c), a)
+    with pytest.raises(RuntimeError, match="workspace"):
+        paged.attention(**c, workspace=ws[:100])
+
+
+def test_refusals():
+    c = _case([30], [2], 8, 2, 128, 16, "bf16", seed=20)
+    q = c["query"]
+    for change, msg in ((dict(query=q.half()), "query must be"), (dict(query=q[..., ::2]), "query must be"),
+                        (dict(query=q.cpu()), "query must be"), (dict(cu_rows=c["cu_rows"].long()), "cu_rows"),
+                        (dict(kv_lens=c["cu_rows"]), "kv_lens"), (dict(table=c["table"].long()), "table"),
+                        (dict(v_pages=c["v_pages"][:, :1]), "one shape"), (dict(scaling=0.0), "scaling"),
+                        (dict(query=q[:, :3]), "unsupported sizes")):
+        with pytest.raises(RuntimeError, match=msg):
+            paged.attention(**{**c, **change})
+    for extra, msg in ((dict(slopes=torch.zeros(7, device=DEV)), "slopes"), (dict(softcap=-1.0), "softcap"),
+                       (dict(prefix_lens=_i32([1, 2])), "prefix_lens"), (dict(first_keys=_i32([1])), "first_keys"),
+                       (dict(out=torch.empty_like(q).float()), "out must")):
+        with pytest.raises(RuntimeError, match=msg):
+            paged.attention(**c, **extra)
+    with pytest.raises(RuntimeError, match="slots"):
+        paged.append(q[:, :2], q[:, :2], c["k_pages"], c["v_pages"], _i32([1, 2]))
+    with pytest.raises(RuntimeError, match="as many rows"):
+        paged.append(q[:, :2], q[:1, :2], c["k_pages"], c["v_pages"], torch.tensor([1, 2], device=DEV))
+
+
+def test_no_rows():
+    c = _case([30], [0], 8, 2, 128, 16, "bf16", seed=21)
+    assert paged.attention(**c).shape == (0, 8, 128)
+    paged.append(c["query"][:, :2], c["query"][:, :2], c["k_pages"], c["v_pages"], torch.zeros(0, dtype=torch.int64, device=DEV))
+
+
+# -- a run of them together ------------------------------------------------------------
+
+
+def _dense(k, v, q, n, scaling):
+    """The last len(q) tokens' attention over the n tokens of one request, 64 bits; and the bound of _reference,
+    with 1.0 for its small terms."""
+    m, group = q.shape[0], q.shape[1] // k.shape[1]
+    k, v = (x[:n].double().repeat_interleave(group, 1) for x in (k, v))
+    s = torch.einsum("mhd,nhd->hmn", q.double(), k) * scaling
+    s = s.masked_fill(torch.arange(n, device=DEV) > torch.arange(n - m, n, device=DEV)[:, None], -torch.inf)
+    w = torch.softmax(s, -1)
+    return torch.einsum("hmn,nhd->mhd", w, v), torch.einsum("hmn,nhd->mhd", w, v.abs())
+
+
+def _serve(graph):
+    """Requests of different lengths through prompts, steps of single tokens, a draft that is taken back, one
+    request's end and another's start; captured (graph) or not."""
+    dt, hq, hkv, dim, page, cap = torch.bfloat16, 8, 2, 128, 16, 400
+    g = torch.Generator(device=DEV).manual_seed(22)
+    new = lambda h, n: torch.randn((n, h, dim), generator=g, device=DEV).to(dt)  # noqa: E731
+    table = paged.PageTable(3, cap, 60, page, DEV)
+    kp, vp = (torch.full((60, hkv, page, dim), float("nan"), device=DEV, dtype=dt) for _ in range(2))
+    ks, vs = ([torch.zeros((0, hkv, dim), device=DEV, dtype=dt) for _ in range(3)] for _ in range(2))
+    scaling = dim ** -0.5
+
+    def check(out, cu, q):
+        for b in range(3):
+            a, e = cu[b], cu[b + 1]
+            if a == e:
+                continue
+            want, av = _dense(ks[b], vs[b], q[a:e], ks[b].shape[0], scaling)
+            assert ((out[a:e].double() - want).abs() <= 2.0 ** -8 * 1.05 * (av + want.abs())).all(), b
+
+    def step(counts, rows):
+        n = sum(counts)
+        q, k, v = new(hq, rows), new(hkv, rows), new(hkv, rows)
+        plan = table.step(_i32(counts), rows)
+        paged.append(k, v, kp, vp, plan.slots)
+        out = paged.attention(q, kp, vp, table.table, plan.cu_rows, plan.kv_lens, scaling)
+        cu = plan.cu_rows.tolist()
+        assert int(plan.failed) == 0 and cu[-1] == n
+        for b in range(3):
+            ks[b], vs[b] = torch.cat([ks[b], k[cu[b]:cu[b + 1]]]), torch.cat([vs[b], v[cu[b]:cu[b + 1]]])
+        check(out, cu, q)
+
+    def back(keep):
+        table.release(_i32(keep))
+        for b, n in enumerate(keep):
+            ks[b], vs[b] = ks[b][:n], vs[b][:n]
+
+    step([100, 7, 33], 150)
+    step([1, 64, 1], 66)
+    step([5, 5, 5], 15)
+    back([103, 200, 35])
+    if not graph:
+        for _ in range(20):
+            step([1, 1, 1], 3)
+    else:
+        q, k, v, ones = new(hq, 3), new(hkv, 3), new(hkv, 3), _i32([1, 1, 1])
+        plan = paged.StepPlan.empty(3, 3, DEV)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            table.step(ones, 3, out=plan)
+            paged.append(k, v, kp, vp, plan.slots)
+            out = paged.attention(q, kp, vp, table.table, plan.cu_rows, plan.kv_lens, scaling, max_rows=1)
+        for _ in range(20):   # the lengths grow on the GPU, past page borders
+            q.copy_(new(hq, 3)), k.copy_(new(hkv, 3)), v.copy_(new(hkv, 3))
+            graph.replay()
+            for b in range(3):
+                ks[b], vs[b] = torch.cat([ks[b], k[b:b + 1]]), torch.cat([vs[b], v[b:b + 1]])
+            check(out, [0, 1, 2, 3], q)
+    back([0, 500, 500])
+    step([40, 1, 1], 42)
+    assert table.lens.tolist() == [x.shape[0] for x in ks]
+    held = sum(-(-x.shape[0] // page) for x in ks)
+    assert int(table.count) == 60 - held
+
+
+def test_serving_steps():
+    _serve(False)
+
+
+def test_serving_steps_captured():
+    _serve(True)
+
+
+def test_another_stream():
+    c = _case([2000, 90], [1, 30], 8, 2, 128, 16, "bf16", seed=23)
+    want = paged.attention(**c)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [paged.attention(**c) for _ in range(4)]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, want) for x in got)
+
+
+def test_offsets_past_32_bits():
+    # a pool of more than 2^31 elements: the pages of one request at its end
+    pages, hkv, page, dim = 70000, 2, 256, 64
+    kp = torch.empty((pages, hkv, page, dim), dtype=torch.bfloat16, device=DEV)
+    vp = torch.empty_like(kp)
+    assert kp.numel() > 2 ** 31
+    c = _case([700, 300], [40, 1], 4, hkv, dim, page, "bf16", seed=24)
+    ids = torch.tensor([pages - 1 - i for i in range(c["k_pages"].shape[0])], device=DEV)
+    kp[ids], vp[ids] = c["k_pages"], c["v_pages"]
+    moved = torch.where(c["table"] >= 0, pages - 1 - c["table"], -1).int()
+    assert torch.equal(paged.attention(**{**c, "k_pages": kp, "v_pages": vp, "table": moved}), paged.attention(**c))
+    slots = torch.tensor([pages * page - 1, 5], device=DEV)
+    rows = torch.randn((2, hkv, dim), device=DEV).to(torch.bfloat16)
+    paged.append(rows, rows, kp, vp, slots)
+    assert torch.equal(kp[-1, :, -1], rows[0]) and torch.equal(vp[0, :, 5], rows[1])
