@@ -31,6 +31,9 @@ constexpr int kTokenM = 16;    // rows of a tile of the token kernel
 template <bool F16>
 constexpr float kShift = F16 ? 6.0f : 0.0f;
 
+template <bool F16>
+constexpr uint32_t kOnes = F16 ? 0x3C003C00u : 0x3F803F80u;   // a pair of 1.0
+
 struct PagedArgs {
   const uint16_t *q, *k, *v;
   uint16_t* out;
@@ -246,6 +249,17 @@ __device__ __forceinline__ u32x2_t read_tr(const uint16_t* p) {
   return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)p));
 }
 
+// 16 bytes a lane from memory to LDS, at `to` (wave-uniform) + 16 bytes * lane, without registers.
+__device__ __forceinline__ void load_lds16(const char* from, uint16_t* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+// Every load of the workgroup into LDS has landed, and every wave is done with the tile before.
+__device__ __forceinline__ void loads_landed() {
+  __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+  __syncthreads();
+}
+
 template <bool F16>
 __device__ __forceinline__ f32x16_t mfma_32x32x16(u32x4_t a, u32x4_t b, f32x16_t c) {
   if constexpr (F16)
@@ -273,7 +287,8 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs a, PagedCl
   constexpr int DB = D / 32;               // blocks of 32 channels of P.V
   constexpr int UR = D / 8;                // 16-byte units of a row
   constexpr int NU = kTile * UR / 256;     // units a thread stages of K, and of V
-  __shared__ __attribute__((aligned(16))) uint16_t kbuf[2][kTile * D], vbuf[2][kTile * D];
+  // arrays of their own, so that the compiler sees that reads of one need not wait for the loads into another
+  __shared__ __attribute__((aligned(16))) uint16_t kbuf0[kTile * D], kbuf1[kTile * D], vbuf0[kTile * D], vbuf1[kTile * D];
   __shared__ int s_odd[2], s_range[4][4];
   Where w;
   if (!locate<false>(a, c, blockIdx.x, w)) return;
@@ -320,55 +335,54 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs a, PagedCl
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
   float m = ninf, l = 0.0f;
 
-  const int u_row = tid / UR, u_col = tid % UR;
-  const uint16_t* kh = a.k + w.head * a.k_head + 8 * u_col;
-  const uint16_t* vh = a.v + w.head * a.v_head + 8 * u_col;
-  u32x4_t kreg[NU], vreg[NU];
-  int ids[4];
-  auto load = [&](int t0) {
+  // A thread stages unit u_col of row u_row (+ 256 / UR per pass) of the tile: rows of one pass and wave lie in one
+  // 16-key group, so in one page, and their address is a wave-uniform base and a constant offset.  LDS holds unit
+  // tid of a pass at place tid, the swizzle is in which column is read.
+  const int u_row = tid / UR, u_col = (tid % UR) ^ swizzle<D>(tid / UR);
+  const uint32_t k_off = 2 * ((u_row & 15) * static_cast<uint32_t>(a.k_tok) + 8 * u_col);
+  const uint32_t v_off = 2 * ((u_row & 15) * static_cast<uint32_t>(a.v_tok) + 8 * u_col);
+  const char* kh = reinterpret_cast<const char*>(a.k + w.head * a.k_head);
+  const char* vh = reinterpret_cast<const char*>(a.v + w.head * a.v_head);
+  const int page_mask = (1 << a.shift) - 1;
+  auto group_of = [&](int u) { return NU == 4 ? u : 2 * u + (wave >> 1); };   // of pass u and this wave
+  const int64_t k_page = 2 * a.k_page, v_page = 2 * a.v_page;
+  const uint32_t k_tok = 2 * static_cast<uint32_t>(a.k_tok), v_tok = 2 * static_cast<uint32_t>(a.v_tok);
+  bool hole = false;   // the loaded tile has keys without a page
+  auto load = [&](int t0, uint16_t* kb, uint16_t* vb) {
+    int ids[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) ids[g] = page_id(a, w, t0 + 16 * g);
+    hole = (ids[0] | ids[1] | ids[2] | ids[3]) < 0;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-      // the 16-key group of this wave's rows
-      const int row = u_row + u * (256 / UR);
-      const int g = NU == 4 ? u : 2 * u + (wave >> 1);
-      const int id = max(g == 0 ? ids[0] : g == 1 ? ids[1] : g == 2 ? ids[2] : ids[3], 0);
-      const int at = (t0 + row) & ((1 << a.shift) - 1);
-      kreg[u] = *reinterpret_cast<const u32x4_t*>(kh + id * a.k_page + at * a.k_tok);
-      vreg[u] = *reinterpret_cast<const u32x4_t*>(vh + id * a.v_page + at * a.v_tok);
+      const int id = max(NU == 4 ? ids[u % 4] : wave >> 1 ? ids[(2 * u + 1) % 4] : ids[2 * u % 4], 0);
+      const uint32_t at = (t0 + 16 * group_of(u)) & page_mask;
+      load_lds16(kh + id * k_page + static_cast<uint64_t>(at) * k_tok + k_off, kb + 8 * (256 * u + 64 * wave));
+      load_lds16(vh + id * v_page + static_cast<uint64_t>(at) * v_tok + v_off, vb + 8 * (256 * u + 64 * wave));
     }
   };
-  // Stores the loaded tile.  Where some row does not see all of it, what no row may read (a page's rest) becomes
-  // zero, and so do infinities and NaN of V, which a zero weight would not hide: add_odd adds those to the rows
-  // that do see them.
-  auto store = [&](int t0, int buf) {
-    const bool masked = t0 < wg_all_lo || t0 + kTile > wg_all_hi || (ids[0] | ids[1] | ids[2] | ids[3]) < 0;
-    if (masked) {
-      bool odd = false;
-#pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        const int row = u_row + u * (256 / UR);
-        const int g = NU == 4 ? u : 2 * u + (wave >> 1);
-        const int id = g == 0 ? ids[0] : g == 1 ? ids[1] : g == 2 ? ids[2] : ids[3];
-        if (id < 0 || t0 + row >= w.kv) vreg[u] = u32x4_t{0u, 0u, 0u, 0u};
-        else odd |= clean<F16>(vreg[u]);
-      }
-      if (odd) s_odd[buf] = t0;
-    }
-#pragma unroll
+  // Where some row does not see all of a tile, what of V no row may read (a page's rest) becomes zero before it is
+  // used, and so do infinities and NaN, which a zero weight would not hide; add_odd adds those to the rows that do
+  // see them.
+  auto clean_tile = [&](int t0, uint16_t* vb, int buf) {
+    bool odd = false;
+#pragma unroll 1
     for (int u = 0; u < NU; ++u) {
-      const int row = u_row + u * (256 / UR);
-      const int at = row * D + 8 * (u_col ^ swizzle<D>(row));
-      *reinterpret_cast<u32x4_t*>(&kbuf[buf][at]) = kreg[u];
-      *reinterpret_cast<u32x4_t*>(&vbuf[buf][at]) = vreg[u];
+      u32x4_t x = *reinterpret_cast<u32x4_t*>(vb + 8 * (256 * u + tid));
+      const int key = t0 + u_row + u * (256 / UR);
+      if (page_id(a, w, t0 + 16 * group_of(u)) < 0 || key >= w.kv) x = u32x4_t{0u, 0u, 0u, 0u};
+      else odd |= clean<F16>(x);
+      *reinterpret_cast<u32x4_t*>(vb + 8 * (256 * u + tid)) = x;
     }
+    if (odd) s_odd[buf] = t0;
+    __syncthreads();
   };
   auto add_odd = [&](int t0) {
+#pragma unroll 1
     for (int j = 0; j < kTile; ++j) {
       const int key = t0 + j, id = page_id(a, w, key);
       if (id < 0) continue;
-      const uint16_t* vr = a.v + id * a.v_page + w.head * a.v_head + (key & ((1 << a.shift) - 1)) * a.v_tok + 4 * half;
+      const uint16_t* vr = a.v + id * a.v_page + w.head * a.v_head + (key & page_mask) * a.v_tok + 4 * half;
       if (!(r.on && key >= r.lo && key < r.hi)) continue;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
@@ -376,13 +390,14 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs a, PagedCl
         for (int i = 0; i < 16; ++i) {
           const uint16_t x = vr[32 * d + 8 * (i >> 2) + (i & 3)];
           if (not_finite<F16>(x)) o[d][i] += half_to_f32<F16>(x);
+          if ((i & 3) == 3) __builtin_amdgcn_sched_barrier(0);
         }
     }
   };
 
   const int k_at = l32 * D, k_sw = swizzle<D>(l32);
   const int v_row = 4 * half + ((lane & 15) >> 2), v_unit = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), v_el = 4 * (lane & 1);
-  auto compute = [&](int t0, int buf, bool hole0, bool hole1, bool hole2, bool hole3) {
+  auto compute = [&](int t0, bool masked, const uint16_t* kb_, const uint16_t* vb_, int buf) {
     if (t0 >= any_hi || t0 + kTile <= any_lo) return;   // no row of the wave sees any of it
     f32x16_t s[2];
 #pragma unroll
@@ -391,7 +406,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs a, PagedCl
       for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(&kbuf[buf][kb * 32 * D + k_at + 8 * ((2 * ks + half) ^ k_sw)]);
+        const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(kb_ + kb * 32 * D + k_at + 8 * ((2 * ks + half) ^ k_sw));
         s[kb] = mfma_32x32x16<F16>(kf, qf[ks], s[kb]);
       }
     }
@@ -402,14 +417,21 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs a, PagedCl
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[kb][i] = form_score(a, r, s[kb][i], key0 + 32 * kb + 8 * (i >> 2) + (i & 3));
     }
-    if (t0 < all_lo || t0 + kTile > all_hi || hole0 || hole1 || hole2 || hole3) {
+    if (masked) {
+      const int from = r.lo - key0;
+      const unsigned span = static_cast<unsigned>(max(r.hi - r.lo, 0));
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int key = key0 + 32 * kb + 8 * (i >> 2) + (i & 3);
-          const bool hole = kb == 0 ? (i < 8 ? hole0 : hole1) : (i < 8 ? hole2 : hole3);
-          if (hole || key < r.lo || key >= r.hi) s[kb][i] = ninf;
+          if (static_cast<unsigned>(32 * kb + 8 * (i >> 2) + (i & 3) - from) >= span) s[kb][i] = ninf;
+          if ((i & 3) == 3) __builtin_amdgcn_sched_barrier(0);   // few lane masks live at a time
+        }
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (page_id(a, w, t0 + 16 * g) < 0) {   // a page the request does not have
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s[g >> 1][8 * (g & 1) + i] = ninf;
         }
     }
     float cm = s[0][0];
@@ -440,9 +462,9 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs a, PagedCl
         float e[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][4 * q + i], sl, -ms));
-        sum0 += e[0] + e[1];
-        sum1 += e[2] + e[3];
         const u32x2_t x = pack4_half<F16>(e);
+        sum0 = dot2_half<F16>(x[0], kOnes<F16>, sum0);   // of the rounded weights, which V is weighted by
+        sum1 = dot2_half<F16>(x[1], kOnes<F16>, sum1);
         p[2 * kb + (q >> 1)][2 * (q & 1)] = x[0];
         p[2 * kb + (q >> 1)][2 * (q & 1) + 1] = x[1];
       }
@@ -452,28 +474,27 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs a, PagedCl
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
         const int r0 = 16 * ks + v_row, r1 = r0 + 8;
-        const u32x2_t x = read_tr(&vbuf[buf][r0 * D + 8 * ((4 * d + v_unit) ^ swizzle<D>(r0)) + v_el]);
-        const u32x2_t y = read_tr(&vbuf[buf][r1 * D + 8 * ((4 * d + v_unit) ^ swizzle<D>(r1)) + v_el]);
+        const u32x2_t x = read_tr(vb_ + r0 * D + 8 * ((4 * d + v_unit) ^ swizzle<D>(r0)) + v_el);
+        const u32x2_t y = read_tr(vb_ + r1 * D + 8 * ((4 * d + v_unit) ^ swizzle<D>(r1)) + v_el);
         o[d] = mfma_32x32x16<F16>(u32x4_t{x[0], x[1], y[0], y[1]}, p[ks], o[d]);
       }
-    if (s_odd[buf] == t0) add_odd(t0);
+    if (masked && s_odd[buf] == t0) add_odd(t0);
   };
 
+  // One barrier a tile: the next tile's loads are issued before this one is computed, and have landed behind it.
+  auto turn = [&](int t0, const uint16_t* kb_, uint16_t* vb_, int buf, uint16_t* kn, uint16_t* vn) {
+    const bool masked = t0 < wg_all_lo || t0 + kTile > wg_all_hi || hole;
+    if (t0 + kTile < end) load(t0 + kTile, kn, vn);
+    if (masked) clean_tile(t0, vb_, buf);
+    compute(t0, masked, kb_, vb_, buf);
+    loads_landed();
+  };
   if (begin < end) {
-    load(begin);
-    store(begin, 0);
-    bool h0 = ids[0] < 0, h1 = ids[1] < 0, h2 = ids[2] < 0, h3 = ids[3] < 0;
-    __syncthreads();
-    int buf = 0;
-    for (int t0 = begin; t0 < end; t0 += kTile, buf ^= 1) {
-      const bool more = t0 + kTile < end;
-      if (more) load(t0 + kTile);
-      compute(t0, buf, h0, h1, h2, h3);
-      if (more) {
-        store(t0 + kTile, buf ^ 1);
-        h0 = ids[0] < 0, h1 = ids[1] < 0, h2 = ids[2] < 0, h3 = ids[3] < 0;
-      }
-      __syncthreads();
+    load(begin, kbuf0, vbuf0);
+    loads_landed();
+    for (int t0 = begin; t0 < end; t0 += 2 * kTile) {
+      turn(t0, kbuf0, vbuf0, 0, kbuf1, vbuf1);
+      if (t0 + kTile < end) turn(t0 + kTile, kbuf1, vbuf1, 1, kbuf0, vbuf0);
     }
   }
 
@@ -849,6 +870,8 @@ QKV_EXPORT int qkv_paged_attention(const void* query, const int64_t* q_strides, 
   for (int i = 0; i < 3; ++i)
     if (k_strides[i] % 8 || v_strides[i] % 8)
       return fail(QKV_ERR_INVALID, "%s: pages and output must be 16-byte aligned", what);
+  if (k_strides[2] < 0 || k_strides[2] >= (1 << 26) || v_strides[2] < 0 || v_strides[2] >= (1 << 26))
+    return fail(QKV_ERR_UNSUPPORTED, "%s: token strides must be below 2^26", what);
   const int64_t group = q_heads / kv_heads;
   const Shape sr = shape_of(false, rows, max_rows, requests, width * page, kv_heads, group);
   const Shape sk = shape_of(true, rows, max_rows, requests, width * page, kv_heads, group);
