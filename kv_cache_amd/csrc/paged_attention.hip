@@ -49,7 +49,8 @@ struct PagedArgs {
 // What one class of requests is worked by: tiles of `tokens` tokens, for requests of more than `above` and at most
 // `most` rows, split along the keys into chunks of at least `min_keys` for about `target` workgroups.
 struct PagedClass {
-  int tokens, above, most, min_keys, target;
+  int tokens, above, most, min_keys;
+  float per_target;   // 1.0001 / target
   int max_parts;   // parts the workspace holds
 };
 
@@ -63,6 +64,53 @@ __device__ __forceinline__ int rows_of(const PagedArgs& a, int b, int& row0) {
   return min(max(a.cu[b + 1], row0), a.rows) - row0;
 }
 
+// Sum (wave total in lane 63) and maximum over the wave by DPP moves within rows of 16 lanes and across them: a
+// shuffle through LDS takes several times as long, and locate and the kernels' heads are chains of these.
+__device__ __forceinline__ int wave_scan(int v) {   // inclusive prefix sum
+  auto add = [&](auto ctrl, auto rows) {
+    v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+  };
+  using std::integral_constant;
+  add(integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});   // row_shr 1, 2, 4, 8
+  add(integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
+  add(integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
+  add(integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});   // row_bcast 15 and 31
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});
+  return v;
+}
+__device__ __forceinline__ float lane63(float v) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ __forceinline__ float wave_total(float v) {
+  auto add = [&](auto ctrl, auto rows) {
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, decltype(rows)::value,
+                                                    0xF, false));
+  };
+  using std::integral_constant;
+  add(integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});
+  add(integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
+  add(integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
+  add(integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});
+  return lane63(v);
+}
+__device__ __forceinline__ int wave_max_i(int x) {
+  auto fold = [&](auto ctrl, auto rows) {
+    x = max(x, static_cast<int>(dpp_mov<decltype(ctrl)::value, decltype(rows)::value>(static_cast<uint32_t>(x),
+                                                                                      static_cast<uint32_t>(x))));
+  };
+  using std::integral_constant;
+  fold(integral_constant<int, 0xB1>{}, integral_constant<int, 0xF>{});   // quad_perm, then row mirrors
+  fold(integral_constant<int, 0x4E>{}, integral_constant<int, 0xF>{});
+  fold(integral_constant<int, 0x141>{}, integral_constant<int, 0xF>{});
+  fold(integral_constant<int, 0x140>{}, integral_constant<int, 0xF>{});
+  fold(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});
+  fold(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
 // Which (request, tile, KV head, chunk of keys) workgroup `item` of a class has; false if there are fewer.  Every
 // workgroup derives it from the lengths: with the total work W = sum_b tiles_b * keys_b * heads, chunks have
 // C = max(min_keys, W / target) keys rounded up to kTile, request b is split into S_b = ceil(keys_b / C), and an
@@ -70,83 +118,110 @@ __device__ __forceinline__ int rows_of(const PagedArgs& a, int b, int& row0) {
 // (tile, head) of requests with S_b > 1 only, for the kernel that joins the parts.
 // The head runs fastest (consecutive workgroups go to different XCDs, so that with 8 KV heads an XCD's L2 serves one
 // head), then the tile from the last one on (under a causal mask the longest).
-// Cost: about 1 us, once per workgroup, against a launch of its own for a plan.
+// W is taken in fp32, every workgroup in the same order, and C a ten-thousandth larger, so that W / C stays below
+// target whatever was rounded.  Up to 64 requests every wave does it for itself.
 template <bool PER_TILE>
 __device__ __forceinline__ bool locate(const PagedArgs& a, const PagedClass& c, int item, Where& w) {
-  __shared__ unsigned long long s_tot[4];
-  __shared__ int s_part[8];
-  __shared__ int s_hit[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  auto load = [&](int b, int& nt, int& keys) {
-    nt = keys = 0;
-    if (b >= a.requests) return;
-    int row0;
-    const int n = rows_of(a, b, row0);
-    if (n <= c.above || n > c.most) return;
-    nt = (n + c.tokens - 1) / c.tokens;
-    keys = static_cast<int>(min(static_cast<int64_t>(max(a.kv_lens[b], 0)), static_cast<int64_t>(a.width) << a.shift));
+  struct Share {
+    int nt, keys, row0, n_rows;
   };
-  int nt, keys;
-  unsigned long long tot = 0;
-  load(tid, nt, keys);
-  tot = static_cast<unsigned long long>(nt) * keys;
-  for (int b0 = 256; b0 < a.requests; b0 += 256) {
-    int nt2, keys2;
-    load(b0 + tid, nt2, keys2);
-    tot += static_cast<unsigned long long>(nt2) * keys2;
-  }
-  for (int m = 32; m >= 1; m >>= 1) tot += __shfl_xor(tot, m);
-  if (lane == 0) s_tot[wave] = tot;
-  if (tid == 0) s_hit[0] = -1;
-  __syncthreads();
-  tot = (s_tot[0] + s_tot[1] + s_tot[2] + s_tot[3]) * a.kv_heads;
-  const unsigned long long per = (tot + c.target - 1) / c.target;
-  const int chunk = static_cast<int>((max(per, static_cast<unsigned long long>(c.min_keys)) + kTile - 1) / kTile * kTile);
-  int carry = 0, part_carry = 0;
-  for (int b0 = 0; b0 < a.requests; b0 += 256) {
-    if (b0) load(b0 + tid, nt, keys);
-    const int ns = max(1, (keys + chunk - 1) / chunk);
-    const int parts = ns > 1 ? nt * a.kv_heads * ns : 0;
-    const int items = PER_TILE ? (ns > 1 ? nt * a.kv_heads : 0) : nt * a.kv_heads * ns;
-    const int up = wave_incl_scan(items), up_part = wave_incl_scan(parts);
-    if (lane == 63) {
-      s_part[2 * wave] = up;
-      s_part[2 * wave + 1] = up_part;
-    }
-    __syncthreads();
-    int before = carry, before_part = part_carry;
-    for (int i = 0; i < 4; ++i) {
-      if (i < wave) {
-        before += s_part[2 * i];
-        before_part += s_part[2 * i + 1];
+  auto share_of = [&](int b) {
+    Share s{0, 0, 0, 0};
+    if (b < a.requests) {
+      s.n_rows = rows_of(a, b, s.row0);
+      if (s.n_rows > c.above && s.n_rows <= c.most) {
+        s.nt = (s.n_rows + c.tokens - 1) / c.tokens;
+        s.keys = static_cast<int>(min(static_cast<int64_t>(max(a.kv_lens[b], 0)), static_cast<int64_t>(a.width) << a.shift));
       }
-      carry += s_part[2 * i];
-      part_carry += s_part[2 * i + 1];
     }
-    const int begin = before + up - items;
-    if (item >= begin && item < begin + items) {   // one thread at most
-      s_hit[0] = b0 + tid;
-      s_hit[1] = item - begin;
-      s_hit[2] = before_part + up_part - parts;
-      s_hit[3] = keys;
+    return s;
+  };
+  auto chunk_of = [&](float total) {
+    const float per = total * static_cast<float>(a.kv_heads) * c.per_target;
+    const int least = max(c.min_keys, static_cast<int>(fminf(per, 1.0e9f)) + 1);
+    return __builtin_amdgcn_readfirstlane((least + kTile - 1) & -kTile);
+  };
+  auto splits_of = [&](const Share& s, int chunk) { return s.keys > chunk ? (s.keys + chunk - 1) / chunk : 1; };
+  int at, part, nt;
+  if (a.requests <= 64) {
+    const Share s = share_of(lane);
+    w.chunk = chunk_of(wave_total(static_cast<float>(s.nt) * static_cast<float>(s.keys)));
+    const int ns = splits_of(s, w.chunk), tiles = s.nt * a.kv_heads;
+    const int parts = ns > 1 ? tiles * ns : 0, items = PER_TILE ? (ns > 1 ? tiles : 0) : tiles * ns;
+    const int begin = wave_scan(items) - items, part_begin = wave_scan(parts) - parts;
+    const uint64_t hit = __ballot(item >= begin && item - begin < items);
+    if (!hit) return false;
+    w.b = __builtin_ctzll(hit);
+    at = item - __builtin_amdgcn_readlane(begin, w.b);
+    part = __builtin_amdgcn_readlane(part_begin, w.b);
+    nt = __builtin_amdgcn_readlane(s.nt, w.b);
+    w.kv = __builtin_amdgcn_readlane(s.keys, w.b);
+    w.n_split = __builtin_amdgcn_readlane(ns, w.b);
+    w.row0 = __builtin_amdgcn_readlane(s.row0, w.b);
+    w.n_rows = __builtin_amdgcn_readlane(s.n_rows, w.b);
+  } else {
+    __shared__ float s_tot[4];
+    __shared__ int s_part[8], s_hit[8];
+    float total = 0.0f;
+    for (int b0 = 0; b0 < a.requests; b0 += 256) {
+      const Share s = share_of(b0 + tid);
+      total += static_cast<float>(s.nt) * static_cast<float>(s.keys);
     }
+    total = wave_total(total);
+    if (lane == 0) s_tot[wave] = total;
+    if (tid == 0) s_hit[0] = -1;
     __syncthreads();
-    if (s_hit[0] >= 0 || item < carry) break;   // the same for every thread
+    w.chunk = chunk_of((s_tot[0] + s_tot[1]) + (s_tot[2] + s_tot[3]));
+    int carry = 0, part_carry = 0;
+    for (int b0 = 0; b0 < a.requests; b0 += 256) {
+      const Share s = share_of(b0 + tid);
+      const int ns = splits_of(s, w.chunk), tiles = s.nt * a.kv_heads;
+      const int parts = ns > 1 ? tiles * ns : 0, items = PER_TILE ? (ns > 1 ? tiles : 0) : tiles * ns;
+      const int up = wave_scan(items), up_part = wave_scan(parts);
+      if (lane == 63) {
+        s_part[2 * wave] = up;
+        s_part[2 * wave + 1] = up_part;
+      }
+      __syncthreads();
+      int begin = carry + up - items, part_begin = part_carry + up_part - parts;
+      for (int i = 0; i < 4; ++i) {
+        if (i < wave) {
+          begin += s_part[2 * i];
+          part_begin += s_part[2 * i + 1];
+        }
+        carry += s_part[2 * i];
+        part_carry += s_part[2 * i + 1];
+      }
+      if (item >= begin && item - begin < items) {   // one thread at most
+        s_hit[0] = b0 + tid;
+        s_hit[1] = item - begin;
+        s_hit[2] = part_begin;
+        s_hit[3] = s.nt;
+        s_hit[4] = s.keys;
+        s_hit[5] = ns;
+        s_hit[6] = s.row0;
+        s_hit[7] = s.n_rows;
+      }
+      __syncthreads();
+      if (s_hit[0] >= 0 || item < carry) break;   // the same for every thread
+    }
+    w.b = __builtin_amdgcn_readfirstlane(s_hit[0]);
+    if (w.b < 0) return false;
+    at = __builtin_amdgcn_readfirstlane(s_hit[1]);
+    part = __builtin_amdgcn_readfirstlane(s_hit[2]);
+    nt = __builtin_amdgcn_readfirstlane(s_hit[3]);
+    w.kv = __builtin_amdgcn_readfirstlane(s_hit[4]);
+    w.n_split = __builtin_amdgcn_readfirstlane(s_hit[5]);
+    w.row0 = __builtin_amdgcn_readfirstlane(s_hit[6]);
+    w.n_rows = __builtin_amdgcn_readfirstlane(s_hit[7]);
   }
-  const int b = __builtin_amdgcn_readfirstlane(s_hit[0]);
-  if (b < 0) return false;
-  w.b = b;
-  w.kv = __builtin_amdgcn_readfirstlane(s_hit[3]);
-  w.chunk = chunk;
-  w.n_split = max(1, (w.kv + chunk - 1) / chunk);
-  w.n_rows = rows_of(a, b, w.row0);
-  const int n_tiles = (w.n_rows + c.tokens - 1) / c.tokens;
-  const int at = __builtin_amdgcn_readfirstlane(s_hit[1]);
-  const int rest = at / a.kv_heads;
+  // divisions are done by the vector unit; what they give is the same in every lane
+  const int rest = __builtin_amdgcn_readfirstlane(at / a.kv_heads);
   w.head = at - rest * a.kv_heads;
-  w.split = rest / n_tiles;
-  w.tile = n_tiles - 1 - (rest - w.split * n_tiles);
-  w.part = __builtin_amdgcn_readfirstlane(s_hit[2]) + (w.head * n_tiles + w.tile) * w.n_split;
+  w.split = __builtin_amdgcn_readfirstlane(rest / nt);
+  w.tile = nt - 1 - (rest - w.split * nt);
+  w.part = part + (w.head * nt + w.tile) * w.n_split;
   // always so where cu_rows ascends; otherwise nothing is written out of bounds
   if (w.n_split > 1 && (w.part < 0 || w.part > c.max_parts - w.n_split)) return false;
   if (!PER_TILE) w.part += w.split;
@@ -212,7 +287,10 @@ __device__ __forceinline__ float form_score(const PagedArgs& a, const Row& r, fl
 // The id of the page with key `key`, or -1 where the request has none there (wave-uniform).
 __device__ __forceinline__ int page_id(const PagedArgs& a, const Where& w, int key) {
   if (key >= w.kv) return -1;
-  const int id = a.table[w.b * a.table_ld + (key >> a.shift)];
+  // through the constant address space: a scalar load, whatever the kernel stores meanwhile (a vector load would be
+  // waited for together with every load into LDS before it)
+  const auto* row = (const __attribute__((address_space(4))) int32_t*)(a.table + w.b * a.table_ld);
+  const int id = row[key >> a.shift];
   return static_cast<unsigned>(id) < static_cast<unsigned>(a.pages) ? id : -1;
 }
 
@@ -268,11 +346,6 @@ __device__ __forceinline__ f32x16_t mfma_32x32x16(u32x4_t a, u32x4_t b, f32x16_t
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
                                                    0, 0, 0);
-}
-
-__device__ __forceinline__ int wave_max_i(int v) {
-  for (int m = 32; m >= 1; m >>= 1) v = max(v, shfl_xor_i(v, m));
-  return __builtin_amdgcn_readfirstlane(v);
 }
 
 // ---------------------------------------------------------------------------
@@ -400,14 +473,19 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs a, PagedCl
   auto compute = [&](int t0, bool masked, const uint16_t* kb_, const uint16_t* vb_, int buf) {
     if (t0 >= any_hi || t0 + kTile <= any_lo) return;   // no row of the wave sees any of it
     f32x16_t s[2];
+    {
+      u32x4_t kf[2][KS];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
+        for (int ks = 0; ks < KS; ++ks)
+          kf[kb][ks] = *reinterpret_cast<const u32x4_t*>(kb_ + kb * 32 * D + k_at + 8 * ((2 * ks + half) ^ k_sw));
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(kb_ + kb * 32 * D + k_at + 8 * ((2 * ks + half) ^ k_sw));
-        s[kb] = mfma_32x32x16<F16>(kf, qf[ks], s[kb]);
+      for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s[kb] = mfma_32x32x16<F16>(kf[kb][ks], qf[ks], s[kb]);
       }
     }
     const int key0 = t0 + 4 * half;   // element i of tile kb: key0 + 32 kb + 8 (i / 4) + i % 4
@@ -726,45 +804,67 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedArgs a, PagedC
     *reinterpret_cast<float4*>(a.ws_acc + at * D + d0 + e) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
 }
 
-// Joins the parts of the tiles whose keys were split: 16 rows a workgroup (blockIdx.y: which 16 of the tile), the
-// parts in the order of their keys, so that the result does not depend on which was done first.
-template <int D, bool F16, int M>
+// Joins the parts of the tiles whose keys were split.  A workgroup takes R rows of a tile (blockIdx.y: which) and
+// walks their parts in P groups, part s in group s % P; the groups are joined in order, so that the result does not
+// depend on which workgroup was done first.  Tiles of the token kernel have few rows and up to a thousand parts (one
+// row a workgroup), those of the rows kernel many rows and few parts.
+template <int D, bool F16, int M, int R>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, PagedClass c) {
+  constexpr int L = D / 4;             // lanes of a row, 4 values each
+  constexpr int P = 256 / (R * L);
+  __shared__ float s_acc[P][R][D], s_m[P][R], s_l[P][R];
   Where w;
   if (!locate<true>(a, c, blockIdx.x, w)) return;
-  constexpr int E = D / 16;
-  const int row = blockIdx.y * 16 + (threadIdx.x >> 4), d0 = (threadIdx.x & 15) * E;
+  const int in_tile = threadIdx.x / L % R, group = threadIdx.x / (L * R), d0 = 4 * (threadIdx.x % L);
+  const int row = blockIdx.y * R + in_tile;
+  if (static_cast<int>(blockIdx.y) * R >= min(c.tokens, w.n_rows - w.tile * c.tokens) * a.group) return;   // none there
+  const float ninf = -__builtin_huge_valf();
+  float m = ninf, l = 0.0f;
+  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto add = [&](float mp, float lp, float4 x) {
+    if (lp == 0.0f) mp = ninf, x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // a part without keys holds no values
+    const float mn = fmaxf(m, mp), base = mn == ninf ? 0.0f : mn;
+    const float fo = __builtin_amdgcn_exp2f(m - base), fn = __builtin_amdgcn_exp2f(mp - base);
+    l = __builtin_fmaf(lp, fn, l * fo);
+    y.x = __builtin_fmaf(x.x, fn, y.x * fo);
+    y.y = __builtin_fmaf(x.y, fn, y.y * fo);
+    y.z = __builtin_fmaf(x.z, fn, y.z * fo);
+    y.w = __builtin_fmaf(x.w, fn, y.w * fo);
+    m = mn;
+  };
+  const int64_t at = static_cast<int64_t>(w.part) * M + row;   // of part 0
+  constexpr int U = 4;   // parts whose loads are issued together
+  for (int s0 = group; s0 < w.n_split; s0 += U * P) {
+    float mp[U], lp[U];
+    float4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t p = at + static_cast<int64_t>(min(s0 + u * P, w.n_split - 1)) * M;
+      mp[u] = a.ws_ml[2 * p];
+      lp[u] = a.ws_ml[2 * p + 1];
+      x[u] = *reinterpret_cast<const float4*>(a.ws_acc + p * D + d0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s0 + u * P < w.n_split) add(mp[u], lp[u], x[u]);
+  }
+  if constexpr (P > 1) {
+    *reinterpret_cast<float4*>(&s_acc[group][in_tile][d0]) = y;
+    if (d0 == 0) {
+      s_m[group][in_tile] = m;
+      s_l[group][in_tile] = l;
+    }
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int p = 1; p < P; ++p)
+      add(s_m[p][in_tile], s_l[p][in_tile], *reinterpret_cast<const float4*>(&s_acc[p][in_tile][d0]));
+  }
   const Row r = row_of<false>(a, c, w, row);
   if (!r.on) return;
-  const int64_t at = static_cast<int64_t>(w.part) * M + row;   // of split 0 (w.split is 0 here)
-  const float ninf = -__builtin_huge_valf();
-  float m = ninf, l = 0.0f, y[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) y[e] = 0.0f;
-  for (int s = 0; s < w.n_split; ++s) {
-    const int64_t p = at + static_cast<int64_t>(s) * M;
-    const float ls = a.ws_ml[2 * p + 1];
-    if (ls == 0.0f) continue;
-    const float ms = a.ws_ml[2 * p];
-    const float mn = fmaxf(m, ms);
-    const float fo = m == ninf ? 0.0f : __builtin_amdgcn_exp2f(m - mn), fn = __builtin_amdgcn_exp2f(ms - mn);
-    l = __builtin_fmaf(ls, fn, l * fo);
-    m = mn;
-#pragma unroll
-    for (int e = 0; e < E; e += 4) {
-      const float4 x = *reinterpret_cast<const float4*>(a.ws_acc + p * D + d0 + e);
-      y[e] = __builtin_fmaf(x.x, fn, y[e] * fo);
-      y[e + 1] = __builtin_fmaf(x.y, fn, y[e + 1] * fo);
-      y[e + 2] = __builtin_fmaf(x.z, fn, y[e + 2] * fo);
-      y[e + 3] = __builtin_fmaf(x.w, fn, y[e + 3] * fo);
-    }
-  }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int e = 0; e < E; e += 4) {
-    const float z[4] = {y[e] * inv, y[e + 1] * inv, y[e + 2] * inv, y[e + 3] * inv};
-    *reinterpret_cast<u32x2_t*>(a.out + r.o_at + d0 + e) = pack4_half<F16>(z);
-  }
+  const float z[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
+  *reinterpret_cast<u32x2_t*>(a.out + r.o_at + d0) = pack4_half<F16>(z);
 }
 
 // The launches of a call, from what the host knows: rows, requests, and the tokens a table row covers.
@@ -783,8 +883,9 @@ Shape shape_of(bool token, int64_t rows, int64_t max_rows, int64_t requests, int
   s.cls.above = token ? 0 : static_cast<int>(token_rows);
   // without a rows kernel the token kernel takes every request, a longer one in several tiles
   s.cls.most = token && max_rows > token_rows ? static_cast<int>(token_rows) : 0x7FFFFFFF;
-  s.cls.min_keys = 256;
-  s.cls.target = token ? 1024 : 512;
+  s.cls.min_keys = token ? 512 : 256;
+  const int64_t target = token ? 1024 : 512;
+  s.cls.per_target = 1.0001f / static_cast<float>(target);
   s.used = rows > 0 && (token ? token_rows > 0 : max_rows > token_rows);
   if (!s.used) return s;
   const int64_t some = std::min(requests, rows);
@@ -793,9 +894,9 @@ Shape shape_of(bool token, int64_t rows, int64_t max_rows, int64_t requests, int
   if (max_keys > s.cls.min_keys) {
     // sum over the requests of tiles * ceil(keys / C) <= W / C + tiles, W / C <= target; where a request is split its
     // ceil(keys / C) is at most 2 keys / C
-    s.items = std::min(tiles + s.cls.target, tiles * cdiv(max_keys, s.cls.min_keys));
-    s.parts = std::min<int64_t>(2 * s.cls.target, s.items);
-    s.tiles = std::min<int64_t>(s.cls.target, tiles);
+    s.items = std::min(tiles + target, tiles * cdiv(max_keys, s.cls.min_keys));
+    s.parts = std::min<int64_t>(2 * target, s.items);
+    s.tiles = std::min<int64_t>(target, tiles);
   }
   s.cls.max_parts = static_cast<int>(s.parts);
   return s;
@@ -821,10 +922,10 @@ int launch(PagedArgs a, const Shape& rows, const Shape& token, hipStream_t st) {
     t.ws_ml += rows.parts * kRowsM * 2;
     paged_token_kernel<D, F16, FORM><<<static_cast<unsigned>(token.items), 256, 0, st>>>(t, token.cls);
     if (token.parts)
-      paged_join_kernel<D, F16, kTokenM><<<static_cast<unsigned>(token.tiles), 256, 0, st>>>(t, token.cls);
+      paged_join_kernel<D, F16, kTokenM, 1><<<dim3(static_cast<unsigned>(token.tiles), kTokenM), 256, 0, st>>>(t, token.cls);
   }
   if (rows.used && rows.parts)
-    paged_join_kernel<D, F16, kRowsM><<<dim3(static_cast<unsigned>(rows.tiles), kRowsM / 16), 256, 0, st>>>(a, rows.cls);
+    paged_join_kernel<D, F16, kRowsM, 8><<<dim3(static_cast<unsigned>(rows.tiles), kRowsM / 8), 256, 0, st>>>(a, rows.cls);
   return check_launch("qkv_paged_attention");
 }
 

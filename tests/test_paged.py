@@ -74,7 +74,7 @@ def test_nothing_to_do():
 
 def test_workspace_bytes():
     f = lib.qkv_paged_attention_workspace_bytes
-    assert f(32, 1, 32, 16, 16, 32, 8, 128) == 0          # 256 keys a request at most: never split
+    assert f(32, 1, 32, 32, 16, 32, 8, 128) == 0          # 512 keys a request at most: never split
     assert f(4, 4, 2, 8, 16, 6, 4, 64) == -1
     assert f(4, 4, 2, 8, 16, 4, 4, 96) == -1
     small, large = f(1, 1, 1, 64, 16, 16, 8, 128), f(32, 1, 32, 2048, 16, 32, 8, 128)
