@@ -25,7 +25,9 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 64;      // keys per step of the rows kernel; splits are multiples of it
 constexpr int kRowsM = 128;    // rows of a tile of the rows kernel
-constexpr int kTokenM = 16;    // rows of a tile of the token kernel
+constexpr int kTokenM = 16;    // rows of a column set of the token kernel, which has one or two
+constexpr int kJoinRows = 8;   // rows of such a tile a workgroup joins
+constexpr int kStep = 32;      // keys a wave of the token kernel takes at a time
 // fp16 weights are scaled by 2^6: they stay below 2^14 (lazy rescaling lets them reach 2^8) and normal down to 2^-20
 // of the row's largest, so that the small weights of long rows keep their bits.
 template <bool F16>
@@ -43,7 +45,7 @@ struct PagedArgs {
   int64_t table_ld;
   int width, pages, shift, requests, rows, kv_heads, group;
   float scale_log2, tanh_scale, cap_log2;   // scaling * log2(e); 2 * scaling / cap * log2(e); cap * log2(e)
-  float *ws_acc, *ws_ml;
+  int wide;                                 // the cap is larger than kNearCap
 };
 
 // What one class of requests is worked by: tiles of `tokens` tokens, for requests of more than `above` and at most
@@ -51,7 +53,8 @@ struct PagedArgs {
 struct PagedClass {
   int tokens, above, most, min_keys;
   float per_target;   // 1.0001 / target
-  int max_parts;   // parts the workspace holds
+  int max_parts;       // parts the workspace holds
+  float *acc, *ml;     // them: weighted values, then (maximum, sum)
 };
 
 // A workgroup's work.
@@ -261,27 +264,41 @@ __device__ __forceinline__ Row row_of(const PagedArgs& a, const PagedClass& c, c
   return r;
 }
 
-// tanh(x) from t = exp2(2 x log2(e)): 1 - 2 / (t + 1), whose error of about 2^-23 is relative to 1, so that small x
-// take the odd polynomial (next term x^11 / 113: below 2^-27 of x at 0.25).
-__device__ __forceinline__ float tanh_of(float x, float x2log2e) {
-  const float t = __builtin_amdgcn_exp2f(x2log2e);
-  const float far = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(t + 1.0f), 1.0f);
-  const float y = x * x;
+// cap * tanh(x / cap) in log2 units, of a product q.k.  Near: 1 - 2 / (exp(2x) + 1), in error by 2^-22 of the cap or
+// so, which for caps up to kNearCap is below 2^-14.  For larger ones that error would show, and small x take the odd
+// polynomial (next term x^11 / 113: below 2^-27 of x at 0.25).
+constexpr float kNearCap = 256.0f;
+__device__ __forceinline__ float near_cap(const PagedArgs& a, float qk) {
+  const float t = __builtin_amdgcn_exp2f(qk * a.tanh_scale);
+  return __builtin_fmaf(-2.0f * a.cap_log2, __builtin_amdgcn_rcpf(t + 1.0f), a.cap_log2);
+}
+__device__ __forceinline__ float wide_cap(const PagedArgs& a, float qk) {
+  const float x = qk * a.tanh_scale * (0.5f / kLog2e), y = x * x;
   float p = __builtin_fmaf(y, 62.0f / 2835.0f, -17.0f / 315.0f);
   p = __builtin_fmaf(y, p, 2.0f / 15.0f);
   p = __builtin_fmaf(y, p, -1.0f / 3.0f);
-  const float near = __builtin_fmaf(x * y, p, x);
-  return fabsf(x) < 0.25f ? near : far;
+  return fabsf(x) < 0.25f ? a.cap_log2 * __builtin_fmaf(x * y, p, x) : near_cap(a, qk);
 }
 
-// The score of a product q.k in log2 units, with cap and bias.
-__device__ __forceinline__ float form_score(const PagedArgs& a, const Row& r, float qk, int key) {
-  float s = qk * a.scale_log2;
-  if (a.cap_log2 != 0.0f) {
-    const float x2 = qk * a.tanh_scale;
-    s = a.cap_log2 * tanh_of(x2 * (0.5f / kLog2e), x2);
+// Scores in log2 units of N products q.k, the i-th `off(i)` keys behind the first, which is `ahead` keys behind the
+// row's own; the branches are the same for every lane of the call.
+template <int N, typename V, typename F>
+__device__ __forceinline__ void form_scores(const PagedArgs& a, const Row& r, int first_key, V& s, F off) {
+  if (a.cap_log2 == 0.0f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] *= a.scale_log2;
+  } else if (!a.wide) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = near_cap(a, s[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = wide_cap(a, s[i]);
   }
-  return __builtin_fmaf(-r.slope, fabsf(static_cast<float>(r.pos - key)), s);
+  if (a.slopes) {
+    const float away = static_cast<float>(r.pos - first_key);
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = __builtin_fmaf(-r.slope, fabsf(away - static_cast<float>(off(i))), s[i]);
+  }
 }
 
 // The id of the page with key `key`, or -1 where the request has none there (wave-uniform).
@@ -333,6 +350,8 @@ __device__ __forceinline__ void load_lds16(const char* from, uint16_t* to) {
                                    (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 // Every load of the workgroup into LDS has landed, and every wave is done with the tile before.
+// Those of this wave have.
+__device__ __forceinline__ void wave_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void loads_landed() {
   __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
   __syncthreads();
@@ -355,16 +374,16 @@ __device__ __forceinline__ f32x16_t mfma_32x32x16(u32x4_t a, u32x4_t b, f32x16_t
 // barrier a tile.
 // ---------------------------------------------------------------------------
 template <int D, bool F16, bool FORM>
-__global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs a, PagedClass c) {
+__device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& c, int item, uint16_t* stage0,
+                                          uint16_t* stage1) {
   constexpr int KS = D / 16;               // steps of 16 channels of Q.K
   constexpr int DB = D / 32;               // blocks of 32 channels of P.V
   constexpr int UR = D / 8;                // 16-byte units of a row
   constexpr int NU = kTile * UR / 256;     // units a thread stages of K, and of V
-  // arrays of their own, so that the compiler sees that reads of one need not wait for the loads into another
-  __shared__ __attribute__((aligned(16))) uint16_t kbuf0[kTile * D], kbuf1[kTile * D], vbuf0[kTile * D], vbuf1[kTile * D];
+  uint16_t *kbuf0 = stage0, *vbuf0 = stage0 + kTile * D, *kbuf1 = stage1, *vbuf1 = stage1 + kTile * D;
   __shared__ int s_odd[2], s_range[4][4];
   Where w;
-  if (!locate<false>(a, c, blockIdx.x, w)) return;
+  if (!locate<false>(a, c, item, w)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, l32 = lane & 31;
   const float ninf = -__builtin_huge_valf();
@@ -492,8 +511,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs a, PagedCl
     if constexpr (FORM) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[kb][i] = form_score(a, r, s[kb][i], key0 + 32 * kb + 8 * (i >> 2) + (i & 3));
+        form_scores<16>(a, r, key0 + 32 * kb, s[kb], [](int i) { return 8 * (i >> 2) + (i & 3); });
     }
     if (masked) {
       const int from = r.lo - key0;
@@ -592,232 +610,316 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs a, PagedCl
   }
   const int64_t at = static_cast<int64_t>(w.part) * kRowsM + 32 * wave + l32;
   if (half == 0) {
-    a.ws_ml[2 * at] = m;
-    a.ws_ml[2 * at + 1] = l;
+    c.ml[2 * at] = m;
+    c.ml[2 * at + 1] = l;
   }
   if (l == 0.0f) return;   // the joining kernel leaves it out
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      *reinterpret_cast<float4*>(a.ws_acc + at * D + 4 * half + 32 * d + 8 * q) =
+      *reinterpret_cast<float4*>(c.acc + at * D + 4 * half + 32 * d + 8 * q) =
           make_float4(o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]);
 }
 
 // ---------------------------------------------------------------------------
-// Tiles of at most 16 rows: the columns of 16-wide score tiles.  Wave w takes steps w, w + 4, ... of 32 keys of the
-// workgroup's chunk; K goes from memory to the matrix instruction's registers, V through the wave's own part of LDS
-// (stored as it lies, read transposed), no barrier until the waves are joined at the end.
+// Tiles of at most 16 NQ rows: NQ sets of 16 columns of 16-wide score tiles.  Wave w takes steps w, w + 4, ... of 32
+// keys of the workgroup's chunk; K goes from memory to the matrix instruction's registers, V through the wave's own
+// part of LDS (as it lies, read transposed), no barrier until the waves are joined at the end.
 // ---------------------------------------------------------------------------
-template <int D, bool F16, bool FORM>
-__global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedArgs a, PagedClass c) {
-  constexpr int STEP = 32;
+template <int D, bool F16, bool FORM, int NQ>
+__device__ __forceinline__ void token_body(const PagedArgs& a, const PagedClass& c, int item, uint16_t* stage0,
+                                           uint16_t* stage1) {
   constexpr int KS = D / 32;               // steps of 32 channels of Q.K
   constexpr int DB = D / 16;               // blocks of 16 channels of P.V
   constexpr int UR = D / 8;                // 16-byte units of a row
-  constexpr int NV = STEP * UR / 64;       // units of V a lane stages
+  constexpr int NV = kStep * UR / 64;      // units of V a lane stages
   constexpr int PASS = 64 / UR;            // rows of V a load covers
-  __shared__ union {
-    uint16_t v[4][STEP * D];
-    float acc[4][kTokenM][D];
-  } lds;
   __shared__ float s_m[4][kTokenM], s_l[4][kTokenM];
   Where w;
-  if (!locate<false>(a, c, blockIdx.x, w)) return;
+  if (!locate<false>(a, c, item, w)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g4 = lane >> 4, c16 = lane & 15;
   const float ninf = -__builtin_huge_valf();
-  const Row r = row_of<FORM>(a, c, w, c16);
-  const int all_lo = wave_max_i(r.lo), all_hi = -wave_max_i(-r.hi);
-  const int any_lo = -wave_max_i(r.on ? -r.lo : -0x7FFFFFFF), any_hi = wave_max_i(r.on ? r.hi : 0);
+  Row r[NQ];
+  u32x4_t qf[NQ][KS];
+  int lo = 0, hi = 0x7FFFFFFF, first = 0x7FFFFFFF, last = 0;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    r[n] = row_of<FORM>(a, c, w, 16 * n + c16);
+    lo = max(lo, r[n].lo);
+    hi = min(hi, r[n].hi);
+    if (r[n].on) first = min(first, r[n].lo), last = max(last, r[n].hi);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const uint4 x = load16u(a.q + r[n].q_at + 32 * s + 8 * g4);
+      qf[n][s] = r[n].on ? u32x4_t{x.x, x.y, x.z, x.w} : u32x4_t{0u, 0u, 0u, 0u};
+    }
+  }
+  const int all_lo = wave_max_i(lo), all_hi = -wave_max_i(-hi), any_lo = -wave_max_i(-first), any_hi = wave_max_i(last);
   const int begin = max(w.split * w.chunk, any_lo / kTile * kTile);
   const int end = static_cast<int>(min(static_cast<int64_t>(w.split + 1) * w.chunk, static_cast<int64_t>(any_hi)));
 
-  u32x4_t qf[KS];
+  f32x4_t o[NQ][DB];
+  float m[NQ], l[NQ];
 #pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    const uint4 x = load16u(a.q + r.q_at + 32 * s + 8 * g4);
-    qf[s] = r.on ? u32x4_t{x.x, x.y, x.z, x.w} : u32x4_t{0u, 0u, 0u, 0u};
+  for (int n = 0; n < NQ; ++n) {
+    m[n] = ninf;
+    l[n] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[n][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  f32x4_t o[DB];
-#pragma unroll
-  for (int d = 0; d < DB; ++d) o[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = ninf, l = 0.0f;
-  uint16_t* vt = lds.v[wave];
-  const uint16_t* kh = a.k + w.head * a.k_head + 8 * g4;
-  const uint16_t* vh = a.v + w.head * a.v_head + 8 * (lane % UR);
-  const int vr = lane / UR, mask = (1 << a.shift) - 1;
-
+  const int page_mask = (1 << a.shift) - 1;
+  const int64_t k_page = 2 * a.k_page, v_page = 2 * a.v_page;
+  const uint32_t k_tok = 2 * static_cast<uint32_t>(a.k_tok), v_tok = 2 * static_cast<uint32_t>(a.v_tok);
+  const char* kh = reinterpret_cast<const char*>(a.k + w.head * a.k_head);
+  const char* vh = reinterpret_cast<const char*>(a.v + w.head * a.v_head);
+  const uint32_t k_off = c16 * k_tok + 16 * g4;
+  // row u * PASS + lane / UR of V; its swizzle goes by the row's low bits, so by the parity of u where PASS is 4
+  const uint32_t v_off0 = lane / UR * v_tok + 16 * ((lane % UR) ^ swizzle<D>(lane / UR));
+  const uint32_t v_off1 = lane / UR * v_tok + 16 * ((lane % UR) ^ swizzle<D>(PASS + lane / UR));
+  const auto* table_row = (const __attribute__((address_space(4))) int32_t*)(a.table + w.b * a.table_ld);
   struct Step {
-    u32x4_t k[2][KS], v[NV];
+    u32x4_t k[2][KS];
     int id[2];
   };
-  auto load = [&](int t0, Step& x) {
+  struct Entries {
+    int v[2];
+  };
+  auto entries_of = [&](int t0) __attribute__((always_inline)) {   // of the step's two 16-key groups
+    Entries e;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) e.v[t] = table_row[min(t0 + 16 * t, w.kv - 1) >> a.shift];
+    return e;
+  };
+  auto load = [&](int t0, const Entries& e, Step& x, uint16_t* vt) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      x.id[t] = page_id(a, w, t0 + 16 * t);
-      const uint16_t* p = kh + max(x.id[t], 0) * a.k_page + ((t0 + 16 * t + c16) & mask) * a.k_tok;
+      const int key = t0 + 16 * t;
+      x.id[t] = key < w.kv && static_cast<unsigned>(e.v[t]) < static_cast<unsigned>(a.pages) ? e.v[t] : -1;
+      const uint32_t at = key & page_mask;
+      const char* vp = vh + max(x.id[t], 0) * v_page + static_cast<uint64_t>(at) * v_tok;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) x.k[t][s] = ld_nt4(p + 32 * s);
-    }
+      for (int u = t * NV / 2; u < (t + 1) * NV / 2; ++u)
+        load_lds16(vp + u * PASS % 16 * v_tok + (u % 2 ? v_off1 : v_off0), vt + 8 * 64 * u);
+      const char* kp = kh + max(x.id[t], 0) * k_page + static_cast<uint64_t>(at) * k_tok;
 #pragma unroll
-    for (int u = 0; u < NV; ++u) {
-      const int row = u * PASS + vr;
-      x.v[u] = ld_nt4(vh + max(x.id[u * PASS / 16], 0) * a.v_page + ((t0 + row) & mask) * a.v_tok);
+      for (int s = 0; s < KS; ++s) x.k[t][s] = ld_nt4(reinterpret_cast<const uint16_t*>(kp + k_off + 64 * s));
     }
   };
-  auto compute = [&](int t0, Step& x) {
-    const bool masked = t0 < all_lo || t0 + STEP > all_hi || (x.id[0] | x.id[1]) < 0;
+  auto compute = [&](int t0, Step& x, uint16_t* vt) __attribute__((always_inline)) {
+    const bool masked = t0 < all_lo || t0 + kStep > all_hi || (x.id[0] | x.id[1]) < 0;
     bool odd = false;
-    if (masked) {   // as in paged_rows_kernel
+    if (masked) {   // as in rows_body; a wave's LDS operations keep their order
 #pragma unroll
       for (int u = 0; u < NV; ++u) {
-        if (x.id[u * PASS / 16] < 0 || t0 + u * PASS + vr >= w.kv) x.v[u] = u32x4_t{0u, 0u, 0u, 0u};
-        else odd |= clean<F16>(x.v[u]);
+        u32x4_t* p = reinterpret_cast<u32x4_t*>(vt + 8 * (64 * u + lane));
+        u32x4_t y = *p;
+        if (x.id[u * PASS / 16] < 0 || t0 + u * PASS + lane / UR >= w.kv) y = u32x4_t{0u, 0u, 0u, 0u};
+        else odd |= clean<F16>(y);
+        *p = y;
+      }
+    }
+    f32x4_t s[NQ][2];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) s[n][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) s[n][t] = mfma_16x16x32<F16>(x.k[t][ks], qf[n][ks], s[n][t]);
+    u32x4_t p[NQ];
+    float mn[NQ];
+    bool raise = false;
+    const float sl = FORM ? 1.0f : a.scale_log2;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      float cm = ninf;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int key0 = t0 + 16 * t + 4 * g4;
+        if constexpr (FORM) form_scores<4>(a, r[n], key0, s[n][t], [](int i) { return i; });
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (x.id[t] < 0 || key0 + i < r[n].lo || key0 + i >= r[n].hi) s[n][t][i] = ninf;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cm = fmaxf(cm, s[n][t][i]);
+      }
+      mn[n] = fmaxf(m[n], max_x32(max_x16(cm)) * sl - kShift<F16>);
+      raise |= mn[n] > m[n] + kLazyLog2;
+    }
+    if (__ballot(raise)) {   // wave-uniform
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        const float al = mn[n] == ninf ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn[n]);
+        l[n] *= al;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[n][d][i] *= al;
+        m[n] = mn[n];
       }
     }
 #pragma unroll
-    for (int u = 0; u < NV; ++u) {
-      const int row = u * PASS + vr;
-      *reinterpret_cast<u32x4_t*>(&vt[row * D + 8 * ((lane % UR) ^ swizzle<D>(row))]) = x.v[u];
-    }
-    float s[2][4];
-    float cm = ninf;
+    for (int n = 0; n < NQ; ++n) {
+      const float ms = m[n] == ninf ? 0.0f : m[n];
+      float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int t = 0; t < 2; ++t) {
+        float e[4];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) acc = mfma_16x16x32<F16>(x.k[t][ks], qf[ks], acc);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = t0 + 16 * t + 4 * g4 + i;
-        float y = FORM ? form_score(a, r, acc[i], key) : acc[i] * a.scale_log2;
-        if (masked && (x.id[t] < 0 || key < r.lo || key >= r.hi)) y = ninf;
-        s[t][i] = y;
-        cm = fmaxf(cm, y);
+        for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][t][i], sl, -ms));
+        const u32x2_t y = pack4_half<F16>(e);
+        sum0 = dot2_half<F16>(y[0], kOnes<F16>, sum0);
+        sum1 = dot2_half<F16>(y[1], kOnes<F16>, sum1);
+        p[n][2 * t] = y[0];
+        p[n][2 * t + 1] = y[1];
       }
-    }
-    cm = max_x32(max_x16(cm)) - kShift<F16>;
-    const float mn = fmaxf(m, cm);
-    if (__ballot(mn > m + kLazyLog2)) {   // wave-uniform
-      const float al = mn == ninf ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-      l *= al;
-#pragma unroll
-      for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[d][i] *= al;
-      m = mn;
-    }
-    const float ms = m == ninf ? 0.0f : m;
-    u32x4_t p;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      float e[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(s[t][i] - ms);
-      l += (e[0] + e[1]) + (e[2] + e[3]);
-      const u32x2_t y = pack4_half<F16>(e);
-      p[2 * t] = y[0];
-      p[2 * t + 1] = y[1];
+      l[n] += sum0 + sum1;
     }
     // element j of a lane's step: key 16 (j / 4) + 4 g4 + j % 4, of P and of V alike
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
       const int r0 = 4 * g4 + (c16 >> 2), r1 = r0 + 16, unit = 2 * d + ((lane & 3) >> 1), el = 4 * (lane & 1);
-      const u32x2_t y = read_tr(&vt[r0 * D + 8 * (unit ^ swizzle<D>(r0)) + el]);
-      const u32x2_t z = read_tr(&vt[r1 * D + 8 * (unit ^ swizzle<D>(r1)) + el]);
-      o[d] = mfma_16x16x32<F16>(u32x4_t{y[0], y[1], z[0], z[1]}, p, o[d]);
+      const u32x2_t y = read_tr(vt + r0 * D + 8 * (unit ^ swizzle<D>(r0)) + el);
+      const u32x2_t z = read_tr(vt + r1 * D + 8 * (unit ^ swizzle<D>(r1)) + el);
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) o[n][d] = mfma_16x16x32<F16>(u32x4_t{y[0], y[1], z[0], z[1]}, p[n], o[n][d]);
     }
-    if (__ballot(odd)) {
-      for (int j = 0; j < STEP; ++j) {
+    if (masked && __ballot(odd)) {
+#pragma unroll 1
+      for (int j = 0; j < kStep; ++j) {
         const int key = t0 + j, id = page_id(a, w, key);
-        if (id < 0 || !(r.on && key >= r.lo && key < r.hi)) continue;
-        const uint16_t* p0 = a.v + id * a.v_page + w.head * a.v_head + (key & mask) * a.v_tok + 4 * g4;
+        if (id < 0) continue;
+        const uint16_t* p0 = a.v + id * a.v_page + w.head * a.v_head + (key & page_mask) * a.v_tok + 4 * g4;
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int n = 0; n < NQ; ++n) {
+          if (!(r[n].on && key >= r[n].lo && key < r[n].hi)) continue;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (not_finite<F16>(p0[16 * d + i])) o[d][i] += half_to_f32<F16>(p0[16 * d + i]);
+          for (int d = 0; d < DB; ++d) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (not_finite<F16>(p0[16 * d + i])) o[n][d][i] += half_to_f32<F16>(p0[16 * d + i]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
       }
     }
   };
 
-  Step x[2];
-  int t0 = begin + STEP * wave;
-  if (t0 < end) load(t0, x[0]);
-  while (t0 < end) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (t0 < end) {
-        if (t0 + 4 * STEP < end) load(t0 + 4 * STEP, x[u ^ 1]);
-        compute(t0, x[u]);
-        t0 += 4 * STEP;
-      }
+  // A step's loads are issued when those of the step before have landed, and land while that one is computed.  (Issued
+  // before that wait, two steps deep, 32 requests of up to 32768 keys take the same 580 us: eight waves a CU with 16 KB
+  // each on its way are enough.)
+  Step x0, x1;
+  Entries e;
+  uint16_t *vt0 = stage0 + wave * kStep * D, *vt1 = stage1 + wave * kStep * D;
+  int t0 = begin + kStep * wave;
+  if (t0 < end) {
+    load(t0, entries_of(t0), x0, vt0);
+    e = entries_of(t0 + 4 * kStep);
+  }
+  auto turn = [&](Step& x, uint16_t* vt, Step& xn, uint16_t* vn) __attribute__((always_inline)) {
+    wave_landed();
+    if (t0 + 4 * kStep < end) {
+      load(t0 + 4 * kStep, e, xn, vn);
+      e = entries_of(t0 + 8 * kStep);
     }
+    compute(t0, x, vt);
+    t0 += 4 * kStep;
+  };
+  while (t0 < end) {
+    turn(x0, vt0, x1, vt1);
+    if (t0 >= end) break;
+    turn(x1, vt1, x0, vt0);
   }
 
   // the four waves' parts, joined
-  l = sum_x32(sum_x16(l));
-  __syncthreads();   // lds.v is done with
-  if (lane < kTokenM) {
-    s_m[wave][lane] = m;
-    s_l[wave][lane] = l;
-  }
+  float* acc = reinterpret_cast<float*>(stage0);   // [4][16][D]
+  constexpr int E = D / 16;                        // values a thread joins
+  const int jr = tid >> 4, d0 = (tid & 15) * E;
 #pragma unroll
-  for (int d = 0; d < DB; ++d)
-    *reinterpret_cast<f32x4_t*>(&lds.acc[wave][c16][16 * d + 4 * g4]) = o[d];
-  __syncthreads();
-  constexpr int E = D / 16;   // values a thread joins
-  const int row = tid >> 4, d0 = (tid & 15) * E;
-  float mj = s_m[0][row];
-#pragma unroll
-  for (int i = 1; i < 4; ++i) mj = fmaxf(mj, s_m[i][row]);
-  float lj = 0.0f, y[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) y[e] = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (s_l[i][row] == 0.0f) continue;
-    const float f = __builtin_amdgcn_exp2f(s_m[i][row] - mj);
-    lj = __builtin_fmaf(s_l[i][row], f, lj);
-#pragma unroll
-    for (int e = 0; e < E; ++e) y[e] = __builtin_fmaf(lds.acc[i][row][d0 + e], f, y[e]);
-  }
-  if (w.n_split == 1) {
-    const Row ro = row_of<false>(a, c, w, row);
-    if (!ro.on) return;
-    const float inv = lj == 0.0f ? 0.0f : 1.0f / lj;
-#pragma unroll
-    for (int e = 0; e < E; e += 4) {
-      const float z[4] = {y[e] * inv, y[e + 1] * inv, y[e + 2] * inv, y[e + 3] * inv};
-      *reinterpret_cast<u32x2_t*>(a.out + ro.o_at + d0 + e) = pack4_half<F16>(z);
+  for (int n = 0; n < NQ; ++n) {
+    const float ln = sum_x32(sum_x16(l[n]));
+    __syncthreads();   // stage0 is done with
+    if (lane < kTokenM) {
+      s_m[wave][lane] = m[n];
+      s_l[wave][lane] = ln;
     }
-    return;
-  }
-  const int64_t at = static_cast<int64_t>(w.part) * kTokenM + row;
-  if ((tid & 15) == 0) {
-    a.ws_ml[2 * at] = mj;
-    a.ws_ml[2 * at + 1] = lj;
-  }
 #pragma unroll
-  for (int e = 0; e < E; e += 4)
-    *reinterpret_cast<float4*>(a.ws_acc + at * D + d0 + e) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+    for (int d = 0; d < DB; ++d)
+      *reinterpret_cast<f32x4_t*>(acc + (wave * kTokenM + c16) * D + 16 * d + 4 * g4) = o[n][d];
+    __syncthreads();
+    float mj = s_m[0][jr];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) mj = fmaxf(mj, s_m[i][jr]);
+    float lj = 0.0f, y[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (s_l[i][jr] == 0.0f) continue;
+      const float f = __builtin_amdgcn_exp2f(s_m[i][jr] - mj);
+      lj = __builtin_fmaf(s_l[i][jr], f, lj);
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[e] = __builtin_fmaf(acc[(i * kTokenM + jr) * D + d0 + e], f, y[e]);
+    }
+    if (w.n_split == 1) {
+      const Row ro = row_of<false>(a, c, w, 16 * n + jr);
+      if (!ro.on) continue;
+      const float inv = lj == 0.0f ? 0.0f : 1.0f / lj;
+#pragma unroll
+      for (int e = 0; e < E; e += 4) {
+        const float z[4] = {y[e] * inv, y[e + 1] * inv, y[e + 2] * inv, y[e + 3] * inv};
+        *reinterpret_cast<u32x2_t*>(a.out + ro.o_at + d0 + e) = pack4_half<F16>(z);
+      }
+      continue;
+    }
+    const int64_t at = static_cast<int64_t>(w.part) * (NQ * kTokenM) + 16 * n + jr;
+    if ((tid & 15) == 0) {
+      c.ml[2 * at] = mj;
+      c.ml[2 * at + 1] = lj;
+    }
+#pragma unroll
+    for (int e = 0; e < E; e += 4)
+      *reinterpret_cast<float4*>(c.acc + at * D + d0 + e) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+  }
 }
 
-// Joins the parts of the tiles whose keys were split.  A workgroup takes R rows of a tile (blockIdx.y: which) and
+// Both kernels stage K and V in two halves of LDS, of which the compiler sees that reads of one need not wait for
+// the loads into the other.
+template <int D, bool F16, bool FORM, int NQ>
+__global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedArgs a, PagedClass c) {
+  __shared__ __attribute__((aligned(16))) uint16_t stage0[2 * kTile * D], stage1[2 * kTile * D];
+  token_body<D, F16, FORM, NQ>(a, c, blockIdx.x, stage0, stage1);
+}
+// Requests of both classes in one launch, the long ones first.
+template <int D, bool F16, bool FORM>
+__global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs a, PagedClass rows, PagedClass token, int n_rows) {
+  __shared__ __attribute__((aligned(16))) uint16_t stage0[2 * kTile * D], stage1[2 * kTile * D];
+  if (static_cast<int>(blockIdx.x) < n_rows) rows_body<D, F16, FORM>(a, rows, blockIdx.x, stage0, stage1);
+  else token_body<D, F16, FORM, 2>(a, token, blockIdx.x - n_rows, stage0, stage1);
+}
+
+// Joins the parts of the tiles whose keys were split.  A workgroup takes R rows of a tile and
 // walks their parts in P groups, part s in group s % P; the groups are joined in order, so that the result does not
 // depend on which workgroup was done first.  Tiles of the token kernel have few rows and up to a thousand parts (one
 // row a workgroup), those of the rows kernel many rows and few parts.
 template <int D, bool F16, int M, int R>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, PagedClass c) {
+__device__ __forceinline__ void join_body(const PagedArgs& a, const PagedClass& c, int item) {
   constexpr int L = D / 4;             // lanes of a row, 4 values each
   constexpr int P = 256 / (R * L);
   __shared__ float s_acc[P][R][D], s_m[P][R], s_l[P][R];
   Where w;
-  if (!locate<true>(a, c, blockIdx.x, w)) return;
+  if (!locate<true>(a, c, item / (M / R), w)) return;
+  const int rows_at = item % (M / R) * R;
   const int in_tile = threadIdx.x / L % R, group = threadIdx.x / (L * R), d0 = 4 * (threadIdx.x % L);
-  const int row = blockIdx.y * R + in_tile;
-  if (static_cast<int>(blockIdx.y) * R >= min(c.tokens, w.n_rows - w.tile * c.tokens) * a.group) return;   // none there
+  const int row = rows_at + in_tile;
+  if (rows_at >= min(c.tokens, w.n_rows - w.tile * c.tokens) * a.group) return;   // none there
   const float ninf = -__builtin_huge_valf();
   float m = ninf, l = 0.0f;
   float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -840,9 +942,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, PagedClass
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t p = at + static_cast<int64_t>(min(s0 + u * P, w.n_split - 1)) * M;
-      mp[u] = a.ws_ml[2 * p];
-      lp[u] = a.ws_ml[2 * p + 1];
-      x[u] = *reinterpret_cast<const float4*>(a.ws_acc + p * D + d0);
+      mp[u] = c.ml[2 * p];
+      lp[u] = c.ml[2 * p + 1];
+      x[u] = *reinterpret_cast<const float4*>(c.acc + p * D + d0);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -867,29 +969,31 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, PagedClass
   *reinterpret_cast<u32x2_t*>(a.out + r.o_at + d0) = pack4_half<F16>(z);
 }
 
+template <int D, bool F16, int NQ>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, PagedClass rows, PagedClass token, int n_rows) {
+  if (static_cast<int>(blockIdx.x) < n_rows) join_body<D, F16, kRowsM, kJoinRows>(a, rows, blockIdx.x);
+  else join_body<D, F16, NQ * kTokenM, 1>(a, token, blockIdx.x - n_rows);
+}
+
 // The launches of a call, from what the host knows: rows, requests, and the tokens a table row covers.
 struct Shape {
   PagedClass cls;
-  bool used;
   int64_t items, parts, tiles;   // workgroups; parts in the workspace; split tiles
 };
 
-Shape shape_of(bool token, int64_t rows, int64_t max_rows, int64_t requests, int64_t max_keys, int64_t kv_heads,
-               int64_t group) {
-  const int64_t m = token ? kTokenM : kRowsM;
-  const int64_t token_rows = kTokenM / group;   // 0: every request takes the rows kernel
+// Tiles of m rows for requests of more than `above` and at most `most` rows.
+Shape shape_of(bool token, int64_t m, int64_t above, int64_t most, int64_t rows, int64_t requests, int64_t max_keys,
+               int64_t kv_heads, int64_t group) {
   Shape s{};
   s.cls.tokens = static_cast<int>(m / group);
-  s.cls.above = token ? 0 : static_cast<int>(token_rows);
-  // without a rows kernel the token kernel takes every request, a longer one in several tiles
-  s.cls.most = token && max_rows > token_rows ? static_cast<int>(token_rows) : 0x7FFFFFFF;
+  s.cls.above = static_cast<int>(above);
+  s.cls.most = static_cast<int>(most);
   s.cls.min_keys = token ? 512 : 256;
   const int64_t target = token ? 1024 : 512;
   s.cls.per_target = 1.0001f / static_cast<float>(target);
-  s.used = rows > 0 && (token ? token_rows > 0 : max_rows > token_rows);
-  if (!s.used) return s;
+  if (rows == 0 || s.cls.tokens == 0) return s;
   const int64_t some = std::min(requests, rows);
-  const int64_t tiles = (s.cls.most == token_rows ? some : (rows + some * (s.cls.tokens - 1)) / s.cls.tokens) * kv_heads;
+  const int64_t tiles = (most <= s.cls.tokens ? some : (rows + some * (s.cls.tokens - 1)) / s.cls.tokens) * kv_heads;
   s.items = tiles;
   if (max_keys > s.cls.min_keys) {
     // sum over the requests of tiles * ceil(keys / C) <= W / C + tiles, W / C <= target; where a request is split its
@@ -900,6 +1004,26 @@ Shape shape_of(bool token, int64_t rows, int64_t max_rows, int64_t requests, int
   }
   s.cls.max_parts = static_cast<int>(s.parts);
   return s;
+}
+
+// One column set where every request's rows fit it, two where they fit those; otherwise the rows kernel, and two
+// column sets for the requests that fit them.
+struct Plan {
+  Shape rows, token;
+  int sets;
+};
+Plan plan_of(int64_t rows, int64_t max_rows, int64_t requests, int64_t max_keys, int64_t kv_heads, int64_t group) {
+  constexpr int64_t kAny = 0x7FFFFFFF;
+  Plan p{};
+  p.sets = max_rows * group <= kTokenM ? 1 : 2;
+  const int64_t m = p.sets * kTokenM;
+  if (max_rows * group <= m) {   // a longer request, if there is one after all, takes several tiles
+    p.token = shape_of(true, m, 0, kAny, rows, requests, max_keys, kv_heads, group);
+    return p;
+  }
+  p.token = shape_of(true, m, 0, m / group, rows, requests, max_keys, kv_heads, group);
+  p.rows = shape_of(false, kRowsM, m / group, kAny, rows, requests, max_keys, kv_heads, group);
+  return p;
 }
 
 int64_t part_floats(int64_t m, int64_t head_dim) { return m * (head_dim + 2); }
@@ -913,19 +1037,23 @@ bool good_sizes(int64_t rows, int64_t requests, int64_t width, int64_t page, int
 }
 
 template <int D, bool F16, bool FORM>
-int launch(PagedArgs a, const Shape& rows, const Shape& token, hipStream_t st) {
-  if (rows.used)
-    paged_rows_kernel<D, F16, FORM><<<static_cast<unsigned>(rows.items), 256, 0, st>>>(a, rows.cls);
-  if (token.used) {
-    PagedArgs t = a;
-    t.ws_acc += rows.parts * kRowsM * D;
-    t.ws_ml += rows.parts * kRowsM * 2;
-    paged_token_kernel<D, F16, FORM><<<static_cast<unsigned>(token.items), 256, 0, st>>>(t, token.cls);
-    if (token.parts)
-      paged_join_kernel<D, F16, kTokenM, 1><<<dim3(static_cast<unsigned>(token.tiles), kTokenM), 256, 0, st>>>(t, token.cls);
+int launch(const PagedArgs& a, const Plan& p, hipStream_t st) {
+  const auto n = [](int64_t x) { return static_cast<unsigned>(x); };
+  if (p.rows.items) {
+    paged_rows_kernel<D, F16, FORM><<<n(p.rows.items + p.token.items), 256, 0, st>>>(a, p.rows.cls, p.token.cls,
+                                                                                   static_cast<int>(p.rows.items));
+  } else if (p.sets == 1) {
+    paged_token_kernel<D, F16, FORM, 1><<<n(p.token.items), 256, 0, st>>>(a, p.token.cls);
+  } else {
+    paged_token_kernel<D, F16, FORM, 2><<<n(p.token.items), 256, 0, st>>>(a, p.token.cls);
   }
-  if (rows.used && rows.parts)
-    paged_join_kernel<D, F16, kRowsM, 8><<<dim3(static_cast<unsigned>(rows.tiles), kRowsM / 8), 256, 0, st>>>(a, rows.cls);
+  const int64_t joins = p.rows.tiles * (kRowsM / kJoinRows), all = joins + p.token.tiles * p.sets * kTokenM;
+  if (all) {
+    if (p.sets == 1)
+      paged_join_kernel<D, F16, 1><<<n(all), 256, 0, st>>>(a, p.rows.cls, p.token.cls, static_cast<int>(joins));
+    else
+      paged_join_kernel<D, F16, 2><<<n(all), 256, 0, st>>>(a, p.rows.cls, p.token.cls, static_cast<int>(joins));
+  }
   return check_launch("qkv_paged_attention");
 }
 
@@ -938,12 +1066,8 @@ QKV_EXPORT int64_t qkv_paged_attention_workspace_bytes(int64_t rows, int64_t max
                                                        int64_t page, int64_t q_heads, int64_t kv_heads,
                                                        int64_t head_dim) {
   if (!good_sizes(rows, requests, width, page, q_heads, kv_heads, head_dim)) return -1;
-  int64_t floats = 0;
-  for (const bool token : {false, true}) {
-    const Shape s = shape_of(token, rows, max_rows, requests, width * page, kv_heads, q_heads / kv_heads);
-    floats += s.parts * part_floats(token ? kTokenM : kRowsM, head_dim);
-  }
-  return 4 * floats;
+  const Plan p = plan_of(rows, max_rows, requests, width * page, kv_heads, q_heads / kv_heads);
+  return 4 * (p.rows.parts * part_floats(kRowsM, head_dim) + p.token.parts * part_floats(p.sets * kTokenM, head_dim));
 }
 
 QKV_EXPORT int qkv_paged_attention(const void* query, const int64_t* q_strides, const void* k_pages,
@@ -974,9 +1098,8 @@ QKV_EXPORT int qkv_paged_attention(const void* query, const int64_t* q_strides, 
   if (k_strides[2] < 0 || k_strides[2] >= (1 << 26) || v_strides[2] < 0 || v_strides[2] >= (1 << 26))
     return fail(QKV_ERR_UNSUPPORTED, "%s: token strides must be below 2^26", what);
   const int64_t group = q_heads / kv_heads;
-  const Shape sr = shape_of(false, rows, max_rows, requests, width * page, kv_heads, group);
-  const Shape sk = shape_of(true, rows, max_rows, requests, width * page, kv_heads, group);
-  if (sr.items > (1ll << 30) || sk.items > (1ll << 30)) return fail(QKV_ERR_UNSUPPORTED, "%s: too many rows", what);
+  Plan p = plan_of(rows, max_rows, requests, width * page, kv_heads, group);
+  if (p.rows.items + p.token.items > (1ll << 30)) return fail(QKV_ERR_UNSUPPORTED, "%s: too many rows", what);
   const int64_t need = qkv_paged_attention_workspace_bytes(rows, max_rows, requests, width, page, q_heads, kv_heads, head_dim);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(QKV_ERR_INVALID, "%s: workspace must be 16-byte aligned and hold %lld bytes", what,
@@ -1001,13 +1124,16 @@ QKV_EXPORT int qkv_paged_attention(const void* query, const int64_t* q_strides, 
   a.scale_log2 = scaling * kLog2e;
   a.tanh_scale = softcap > 0.0f ? 2.0f * kLog2e * scaling / softcap : 0.0f;
   a.cap_log2 = softcap * kLog2e;
-  a.ws_acc = static_cast<float*>(workspace);
-  a.ws_ml = a.ws_acc + head_dim * (sr.parts * kRowsM + sk.parts * kTokenM);
+  a.wide = softcap > kNearCap;
+  p.rows.cls.acc = static_cast<float*>(workspace);
+  p.token.cls.acc = p.rows.cls.acc + head_dim * p.rows.parts * kRowsM;
+  p.rows.cls.ml = p.token.cls.acc + head_dim * p.token.parts * p.sets * kTokenM;
+  p.token.cls.ml = p.rows.cls.ml + 2 * p.rows.parts * kRowsM;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool form = softcap > 0.0f || slopes;
   return with_half(f16, [&](auto h) {
     constexpr bool F = decltype(h)::value;
-    if (head_dim == 128) return form ? launch<128, F, true>(a, sr, sk, st) : launch<128, F, false>(a, sr, sk, st);
-    return form ? launch<64, F, true>(a, sr, sk, st) : launch<64, F, false>(a, sr, sk, st);
+    if (head_dim == 128) return form ? launch<128, F, true>(a, p, st) : launch<128, F, false>(a, p, st);
+    return form ? launch<64, F, true>(a, p, st) : launch<64, F, false>(a, p, st);
   });
 }
