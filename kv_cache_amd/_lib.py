@@ -143,12 +143,12 @@ _PROTOTYPES = {
     "qkv_paged_plan": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp,
                               _vp, _vp]),
     "qkv_paged_release": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
-    "qkv_paged_append": (_i32, [_vp, _P(_i64), _vp, _P(_i64), _vp, _P(_i64), _vp, _P(_i64), _i64, _i64, _i64, _i64,
-                                _vp, _i64, _vp]),
+    # strides by address: the callers lay all of a call's out in one array
+    "qkv_paged_append": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
     "qkv_paged_attention_workspace_bytes": (_i64, [_i64] * 8),
-    "qkv_paged_attention": (_i32, [_vp, _P(_i64), _vp, _P(_i64), _vp, _P(_i64), _i64, _i64, _vp, _i64, _i64, _i64,
-                                   _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _f32, _vp, _vp, _vp, _vp, _i64,
-                                   _vp, _P(_i64), _i32, _vp]),
+    "qkv_paged_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64,
+                                   _i64, _i64, _i64, _i64, _f32, _f32, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i32,
+                                   _vp]),
 }
 
 _LIB = None
@@ -185,7 +185,7 @@ def check(rc: int) -> None:
         raise RuntimeError(load().qkv_last_error().decode())
 
 
-_STRIDE_ARRAYS = [ctypes.c_int64 * n for n in range(8)]
+_STRIDE_ARRAYS = [ctypes.c_int64 * n for n in range(11)]
 
 
 def strides(*vals: int):

@@ -26,7 +26,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 64;      // keys per step of the rows kernel; splits are multiples of it
 constexpr int kRowsM = 128;    // rows of a tile of the rows kernel
 constexpr int kTokenM = 16;    // rows of a column set of the token kernel, which has one or two
-constexpr int kJoinRows = 8;   // rows of such a tile a workgroup joins
+constexpr int kRowsJoins = 4, kTokenJoins = 8;   // workgroups that join the parts of such a tile
 constexpr int kStep = 32;      // keys a wave of the token kernel takes at a time
 // fp16 weights are scaled by 2^6: they stay below 2^14 (lazy rescaling lets them reach 2^8) and normal down to 2^-20
 // of the row's largest, so that the small weights of long rows keep their bits.
@@ -905,74 +905,76 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs a, PagedCl
   else token_body<D, F16, FORM, 2>(a, token, blockIdx.x - n_rows, stage0, stage1);
 }
 
-// Joins the parts of the tiles whose keys were split.  A workgroup takes R rows of a tile and
-// walks their parts in P groups, part s in group s % P; the groups are joined in order, so that the result does not
-// depend on which workgroup was done first.  Tiles of the token kernel have few rows and up to a thousand parts (one
-// row a workgroup), those of the rows kernel many rows and few parts.
-template <int D, bool F16, int M, int R>
+// Joins the parts of the tiles whose keys were split.  G workgroups share a tile's rows, R at a time; each walks a
+// row's parts in P groups, part s in group s % P, which are joined in order, so that the result does not depend
+// on which workgroup was done first.  Tiles of the token kernel have few rows and up to a thousand parts (one row at a
+// time), those of the rows kernel many rows and few parts.
+template <int D, bool F16, int M, int R, int G>
 __device__ __forceinline__ void join_body(const PagedArgs& a, const PagedClass& c, int item) {
   constexpr int L = D / 4;             // lanes of a row, 4 values each
   constexpr int P = 256 / (R * L);
   __shared__ float s_acc[P][R][D], s_m[P][R], s_l[P][R];
   Where w;
-  if (!locate<true>(a, c, item / (M / R), w)) return;
-  const int rows_at = item % (M / R) * R;
+  if (!locate<true>(a, c, item / G, w)) return;
   const int in_tile = threadIdx.x / L % R, group = threadIdx.x / (L * R), d0 = 4 * (threadIdx.x % L);
-  const int row = rows_at + in_tile;
-  if (rows_at >= min(c.tokens, w.n_rows - w.tile * c.tokens) * a.group) return;   // none there
+  const int n_rows = min(c.tokens, w.n_rows - w.tile * c.tokens) * a.group;
   const float ninf = -__builtin_huge_valf();
-  float m = ninf, l = 0.0f;
-  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  auto add = [&](float mp, float lp, float4 x) {
-    if (lp == 0.0f) mp = ninf, x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // a part without keys holds no values
-    const float mn = fmaxf(m, mp), base = mn == ninf ? 0.0f : mn;
-    const float fo = __builtin_amdgcn_exp2f(m - base), fn = __builtin_amdgcn_exp2f(mp - base);
-    l = __builtin_fmaf(lp, fn, l * fo);
-    y.x = __builtin_fmaf(x.x, fn, y.x * fo);
-    y.y = __builtin_fmaf(x.y, fn, y.y * fo);
-    y.z = __builtin_fmaf(x.z, fn, y.z * fo);
-    y.w = __builtin_fmaf(x.w, fn, y.w * fo);
-    m = mn;
-  };
-  const int64_t at = static_cast<int64_t>(w.part) * M + row;   // of part 0
-  constexpr int U = 4;   // parts whose loads are issued together
-  for (int s0 = group; s0 < w.n_split; s0 += U * P) {
-    float mp[U], lp[U];
-    float4 x[U];
+  for (int rows_at = item % G * R; rows_at < n_rows; rows_at += G * R) {
+    const int row = rows_at + in_tile;
+    float m = ninf, l = 0.0f;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto add = [&](float mp, float lp, float4 x) {
+      if (lp == 0.0f) mp = ninf, x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // a part without keys holds no values
+      const float mn = fmaxf(m, mp), base = mn == ninf ? 0.0f : mn;
+      const float fo = __builtin_amdgcn_exp2f(m - base), fn = __builtin_amdgcn_exp2f(mp - base);
+      l = __builtin_fmaf(lp, fn, l * fo);
+      y.x = __builtin_fmaf(x.x, fn, y.x * fo);
+      y.y = __builtin_fmaf(x.y, fn, y.y * fo);
+      y.z = __builtin_fmaf(x.z, fn, y.z * fo);
+      y.w = __builtin_fmaf(x.w, fn, y.w * fo);
+      m = mn;
+    };
+    const int64_t at = static_cast<int64_t>(w.part) * M + row;   // of part 0
+    constexpr int U = 4;   // parts whose loads are issued together
+    for (int s0 = group; s0 < w.n_split; s0 += U * P) {
+      float mp[U], lp[U];
+      float4 x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t p = at + static_cast<int64_t>(min(s0 + u * P, w.n_split - 1)) * M;
-      mp[u] = c.ml[2 * p];
-      lp[u] = c.ml[2 * p + 1];
-      x[u] = *reinterpret_cast<const float4*>(c.acc + p * D + d0);
+      for (int u = 0; u < U; ++u) {
+        const int64_t p = at + static_cast<int64_t>(min(s0 + u * P, w.n_split - 1)) * M;
+        mp[u] = c.ml[2 * p];
+        lp[u] = c.ml[2 * p + 1];
+        x[u] = *reinterpret_cast<const float4*>(c.acc + p * D + d0);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (s0 + u * P < w.n_split) add(mp[u], lp[u], x[u]);
     }
+    if constexpr (P > 1) {
+      __syncthreads();   // the row before is done with
+      *reinterpret_cast<float4*>(&s_acc[group][in_tile][d0]) = y;
+      if (d0 == 0) {
+        s_m[group][in_tile] = m;
+        s_l[group][in_tile] = l;
+      }
+      __syncthreads();
+      if (group > 0) continue;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (s0 + u * P < w.n_split) add(mp[u], lp[u], x[u]);
-  }
-  if constexpr (P > 1) {
-    *reinterpret_cast<float4*>(&s_acc[group][in_tile][d0]) = y;
-    if (d0 == 0) {
-      s_m[group][in_tile] = m;
-      s_l[group][in_tile] = l;
+      for (int p = 1; p < P; ++p)
+        add(s_m[p][in_tile], s_l[p][in_tile], *reinterpret_cast<const float4*>(&s_acc[p][in_tile][d0]));
     }
-    __syncthreads();
-    if (group > 0) return;
-#pragma unroll
-    for (int p = 1; p < P; ++p)
-      add(s_m[p][in_tile], s_l[p][in_tile], *reinterpret_cast<const float4*>(&s_acc[p][in_tile][d0]));
+    const Row r = row_of<false>(a, c, w, row);
+    if (!r.on) continue;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float z[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
+    *reinterpret_cast<u32x2_t*>(a.out + r.o_at + d0) = pack4_half<F16>(z);
   }
-  const Row r = row_of<false>(a, c, w, row);
-  if (!r.on) return;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const float z[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
-  *reinterpret_cast<u32x2_t*>(a.out + r.o_at + d0) = pack4_half<F16>(z);
 }
 
 template <int D, bool F16, int NQ>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, PagedClass rows, PagedClass token, int n_rows) {
-  if (static_cast<int>(blockIdx.x) < n_rows) join_body<D, F16, kRowsM, kJoinRows>(a, rows, blockIdx.x);
-  else join_body<D, F16, NQ * kTokenM, 1>(a, token, blockIdx.x - n_rows);
+  if (static_cast<int>(blockIdx.x) < n_rows) join_body<D, F16, kRowsM, 8, kRowsJoins>(a, rows, blockIdx.x);
+  else join_body<D, F16, NQ * kTokenM, 1, kTokenJoins>(a, token, blockIdx.x - n_rows);
 }
 
 // The launches of a call, from what the host knows: rows, requests, and the tokens a table row covers.
@@ -1047,7 +1049,7 @@ int launch(const PagedArgs& a, const Plan& p, hipStream_t st) {
   } else {
     paged_token_kernel<D, F16, FORM, 2><<<n(p.token.items), 256, 0, st>>>(a, p.token.cls);
   }
-  const int64_t joins = p.rows.tiles * (kRowsM / kJoinRows), all = joins + p.token.tiles * p.sets * kTokenM;
+  const int64_t joins = p.rows.tiles * kRowsJoins, all = joins + p.token.tiles * kTokenJoins;
   if (all) {
     if (p.sets == 1)
       paged_join_kernel<D, F16, 1><<<n(all), 256, 0, st>>>(a, p.rows.cls, p.token.cls, static_cast<int>(joins));

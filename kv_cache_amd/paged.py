@@ -30,6 +30,7 @@ GPU on the current stream and raises RuntimeError on bad input.
 
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple
 
 import torch
@@ -59,12 +60,12 @@ class StepPlan(NamedTuple):
     def empty(cls, requests: int, rows: int, device) -> "StepPlan":
         """Buffers for a step of ``rows`` rows (allocated as one)."""
         words = torch.empty(2 * rows + rows + 2 * requests + 2, dtype=torch.int32, device=device)
-        slots, positions, cu, kv, failed = words.split([2 * rows, rows, requests + 1, requests, 1])
+        slots, positions, cu, kv, failed = words.split_with_sizes([2 * rows, rows, requests + 1, requests, 1])
         return cls(cu, kv, slots.view(torch.int64), positions, failed)
 
 
 def _i32(name: str, t: torch.Tensor, n: int, device) -> None:
-    if t.dtype != torch.int32 or t.device != device or t.dim() != 1 or t.size(0) != n or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous() or t.device != device:
         raise RuntimeError(f"{name} must be contiguous int32 [{n}] on {device}")
 
 
@@ -153,8 +154,7 @@ class PageTable:
 
 
 def _check_slots(slots: torch.Tensor, rows: int, device) -> None:
-    if (slots.dtype != torch.int64 or slots.device != device or slots.dim() != 1 or slots.size(0) != rows
-            or not slots.is_contiguous()):
+    if slots.dtype is not torch.int64 or slots.shape != (rows,) or not slots.is_contiguous() or slots.device != device:
         raise RuntimeError(f"slots must be contiguous int64 [{rows}] on {device}")
 
 
@@ -185,11 +185,11 @@ def append(key: torch.Tensor, value: torch.Tensor, k_pages: torch.Tensor, v_page
     _require(value.size(0) == rows, "key and value must have as many rows")
     _check_slots(slots, rows, key.device)
     with _lib.on_device(key.device):
-        _lib.check(lib.qkv_paged_append(key.data_ptr(), _lib.strides(*key.stride()[:2]), value.data_ptr(),
-                                        _lib.strides(*value.stride()[:2]), k_pages.data_ptr(),
-                                        _lib.strides(*k_pages.stride()[:3]), v_pages.data_ptr(),
-                                        _lib.strides(*v_pages.stride()[:3]), pages, page, heads, dim,
-                                        slots.data_ptr(), rows, _lib.stream_of(key)))
+        st = _lib.strides(*key.stride()[:2], *value.stride()[:2], *k_pages.stride()[:3], *v_pages.stride()[:3])
+        at = ctypes.addressof(st)
+        _lib.check(lib.qkv_paged_append(key.data_ptr(), at, value.data_ptr(), at + 16, k_pages.data_ptr(), at + 32,
+                                        v_pages.data_ptr(), at + 56, pages, page, heads, dim, slots.data_ptr(), rows,
+                                        _lib.stream_of(key)))
 
 
 def attention_workspace(rows: int, max_rows: int, requests: int, width: int, page: int, q_heads: int, kv_heads: int,
@@ -243,7 +243,7 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         _require(slopes.dtype == torch.float32 and slopes.device == dev and slopes.shape == (q_heads,)
                  and slopes.is_contiguous(), f"slopes must be contiguous float32 [{q_heads}] on {dev}")
     if out is None:
-        out = torch.empty((rows, q_heads, dim), dtype=query.dtype, device=dev)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
     else:
         _require(out.shape == query.shape and out.dtype == query.dtype and out.device == dev and out.stride(2) == 1,
                  "out must have the query's shape, dtype and device with contiguous channels")
@@ -255,11 +255,12 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     else:
         _require(workspace.device == dev and workspace.is_contiguous(), f"workspace must be contiguous on {dev}")
     with _lib.on_device(dev):
+        st = _lib.strides(*query.stride()[:2], *k_pages.stride()[:3], *v_pages.stride()[:3], *out.stride()[:2])
+        at = ctypes.addressof(st)
         _lib.check(lib.qkv_paged_attention(
-            query.data_ptr(), _lib.strides(*query.stride()[:2]), k_pages.data_ptr(),
-            _lib.strides(*k_pages.stride()[:3]), v_pages.data_ptr(), _lib.strides(*v_pages.stride()[:3]), pages, page,
+            query.data_ptr(), at, k_pages.data_ptr(), at + 16, v_pages.data_ptr(), at + 40, pages, page,
             table.data_ptr(), table.stride(0), width, n, cu_rows.data_ptr(), kv_lens.data_ptr(), rows, most, q_heads,
             kv_heads, dim, scaling, softcap, _lib.ptr(slopes), _lib.ptr(prefix_lens), _lib.ptr(first_keys),
             _lib.ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
-            out.data_ptr(), _lib.strides(*out.stride()[:2]), code, _lib.stream_of(query)))
+            out.data_ptr(), at + 64, code, _lib.stream_of(query)))
     return out
