@@ -26,6 +26,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 64;      // keys per step of the rows kernel; splits are multiples of it
 constexpr int kRowsM = 128;    // rows of a tile of the rows kernel
 constexpr int kTokenM = 16;    // rows of a column set of the token kernel, which has one or two
+constexpr int kRound = 512;    // workgroups that run at once: two a CU
 constexpr int kRowsJoins = 4, kTokenJoins = 8;   // workgroups that join the parts of such a tile
 constexpr int kStep = 32;      // keys a wave of the token kernel takes at a time
 // fp16 weights are scaled by 2^6: they stay below 2^14 (lazy rescaling lets them reach 2^8) and normal down to 2^-20
@@ -52,7 +53,8 @@ struct PagedArgs {
 // `most` rows, split along the keys into chunks of at least `min_keys` for about `target` workgroups.
 struct PagedClass {
   int tokens, above, most, min_keys;
-  float per_target;   // 1.0001 / target
+  float per_round;     // 1.0001 / kRound
+  int finer;
   int max_parts;       // parts the workspace holds
   float *acc, *ml;     // them: weighted values, then (maximum, sum)
 };
@@ -115,14 +117,15 @@ __device__ __forceinline__ int wave_max_i(int x) {
 }
 
 // Which (request, tile, KV head, chunk of keys) workgroup `item` of a class has; false if there are fewer.  Every
-// workgroup derives it from the lengths: with the total work W = sum_b tiles_b * keys_b * heads, chunks have
-// C = max(min_keys, W / target) keys rounded up to kTile, request b is split into S_b = ceil(keys_b / C), and an
+// workgroup derives it from the lengths: the total work W = sum_b tiles_b * keys_b * heads over the workgroups that run
+// at once gives the keys of a chunk, C (chunk_of); request b is split into S_b = ceil(keys_b / C), and an
 // exclusive prefix sum of tiles_b * heads * S_b over the requests gives its first item.  PER_TILE: items are the
 // (tile, head) of requests with S_b > 1 only, for the kernel that joins the parts.
 // The head runs fastest (consecutive workgroups go to different XCDs, so that with 8 KV heads an XCD's L2 serves one
 // head), then the tile from the last one on (under a causal mask the longest).
-// W is taken in fp32, every workgroup in the same order, and C a ten-thousandth larger, so that W / C stays below
-// target whatever was rounded.  Up to 64 requests every wave does it for itself.
+// W is taken in fp32, every workgroup in the same order, and C a ten-thousandth larger, so that W / C stays below its
+// bound whatever was rounded.  Up to 64 requests every wave does it for itself (four requests a lane, so that 256 do,
+// took 100 requests of up to 2000 keys from 114 to 120 us).
 template <bool PER_TILE>
 __device__ __forceinline__ bool locate(const PagedArgs& a, const PagedClass& c, int item, Where& w) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -140,9 +143,13 @@ __device__ __forceinline__ bool locate(const PagedArgs& a, const PagedClass& c, 
     }
     return s;
   };
+  // One round of equal chunks is best for one request (131011 keys: 94 us, 100 in two rounds).  With several, the last
+  // chunks differ and a round ends with few workgroups: two rounds are better, three where chunks stay above 2048 keys
+  // (32 requests of up to 32768: 625, 574, 554 us with one, two, three; 8 of up to 16384: three 88, two 85.5).
   auto chunk_of = [&](float total) {
-    const float per = total * static_cast<float>(a.kv_heads) * c.per_target;
-    const int least = max(c.min_keys, static_cast<int>(fminf(per, 1.0e9f)) + 1);
+    const float per = total * static_cast<float>(a.kv_heads) * c.per_round;
+    const float keys = c.finer ? fmaxf(per * (1.0f / 3.0f), fminf(per * 0.5f, 2048.0f)) : per;
+    const int least = max(c.min_keys, static_cast<int>(fminf(keys, 1.0e9f)) + 1);
     return __builtin_amdgcn_readfirstlane((least + kTile - 1) & -kTile);
   };
   auto splits_of = [&](const Share& s, int chunk) { return s.keys > chunk ? (s.keys + chunk - 1) / chunk : 1; };
@@ -990,14 +997,15 @@ Shape shape_of(bool token, int64_t m, int64_t above, int64_t most, int64_t rows,
   s.cls.tokens = static_cast<int>(m / group);
   s.cls.above = static_cast<int>(above);
   s.cls.most = static_cast<int>(most);
-  s.cls.min_keys = token ? 512 : 256;
-  const int64_t target = token ? 1024 : 512;
-  s.cls.per_target = 1.0001f / static_cast<float>(target);
+  s.cls.min_keys = 256;
+  const int64_t target = token && requests > 1 ? 3 * kRound : kRound;   // the most that chunk_of asks for
+  s.cls.per_round = 1.0001f / static_cast<float>(kRound);
+  s.cls.finer = token && requests > 1;
   if (rows == 0 || s.cls.tokens == 0) return s;
   const int64_t some = std::min(requests, rows);
   const int64_t tiles = (most <= s.cls.tokens ? some : (rows + some * (s.cls.tokens - 1)) / s.cls.tokens) * kv_heads;
   s.items = tiles;
-  if (max_keys > s.cls.min_keys) {
+  if (max_keys > (token ? 512 : 256)) {
     // sum over the requests of tiles * ceil(keys / C) <= W / C + tiles, W / C <= target; where a request is split its
     // ceil(keys / C) is at most 2 keys / C
     s.items = std::min(tiles + target, tiles * cdiv(max_keys, s.cls.min_keys));
