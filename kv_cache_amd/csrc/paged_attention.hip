@@ -45,7 +45,11 @@ struct PagedArgs {
   const float* slopes;
   int64_t table_ld;
   int width, pages, shift, requests, rows, kv_heads, group;
+  int per_group;            // 65536 / group + 1: i * per_group >> 16 is i / group for rows of a tile (i < 128)
   float scale_log2, tanh_scale, cap_log2;   // scaling * log2(e); 2 * scaling / cap * log2(e); cap * log2(e)
+  // Scores are kept as products q.k, or in log2 units where there is a cap: what takes them to log2 units, and a slope
+  // to theirs.
+  float unit_log2, slope_unit;
   int wide;                                 // the cap is larger than kNearCap
 };
 
@@ -143,20 +147,34 @@ __device__ __forceinline__ bool locate(const PagedArgs& a, const PagedClass& c, 
     }
     return s;
   };
-  // One round of equal chunks is best for one request (131011 keys: 94 us, 100 in two rounds).  With several, the last
-  // chunks differ and a round ends with few workgroups: two rounds are better, three where chunks stay above 2048 keys
-  // (32 requests of up to 32768: 625, 574, 554 us with one, two, three; 8 of up to 16384: three 88, two 85.5).
-  auto chunk_of = [&](float total) {
-    const float per = total * static_cast<float>(a.kv_heads) * c.per_round;
-    const float keys = c.finer ? fmaxf(per * (1.0f / 3.0f), fminf(per * 0.5f, 2048.0f)) : per;
+  auto round_up = [&](float keys) {
     const int least = max(c.min_keys, static_cast<int>(fminf(keys, 1.0e9f)) + 1);
     return __builtin_amdgcn_readfirstlane((least + kTile - 1) & -kTile);
   };
+  // `per` keys for each of the workgroups that run at once.  One round of them is best where it comes out even (one
+  // request of 131011 keys: 94 us, 100 in two rounds).  The last chunks of several requests differ, and a second round
+  // of a few workgroups costs as much as a full one: then two rounds, or three where chunks stay above 2048 keys (32
+  // requests of up to 32768: 625, 574, 554 us with one, two, three; 8 of up to 16384: three 88, two 85.5).
+  auto chunk_of = [&](float per) { return round_up(fmaxf(per * (1.0f / 3.0f), fminf(per * 0.5f, 2048.0f))); };
   auto splits_of = [&](const Share& s, int chunk) { return s.keys > chunk ? (s.keys + chunk - 1) / chunk : 1; };
   int at, part, nt;
   if (a.requests <= 64) {
     const Share s = share_of(lane);
-    w.chunk = chunk_of(wave_total(static_cast<float>(s.nt) * static_cast<float>(s.keys)));
+    const float per = wave_total(static_cast<float>(s.nt) * static_cast<float>(s.keys)) * a.kv_heads * c.per_round;
+    w.chunk = round_up(per);
+    if (c.finer) {
+      // the shortest chunks, up to a fifth longer, that make one round (4 requests of up to 30000 keys: 60 us, 66 in
+      // two; a third longer, as 32 of up to 32768 would need, 615 instead of 554)
+      const int tiles = s.nt * a.kv_heads;
+      int i = 0;
+      for (; i < 4; ++i) {
+        w.chunk = round_up(per * (1.0f + 0.0667f * i));
+        // without a division: one more or less is near enough to choose by
+        const int ns = static_cast<int>(static_cast<float>(s.keys - 1) * __builtin_amdgcn_rcpf(static_cast<float>(w.chunk))) + 1;
+        if (__builtin_amdgcn_readlane(wave_scan(tiles * ns), 63) <= kRound) break;
+      }
+      if (i == 4) w.chunk = chunk_of(per);
+    }
     const int ns = splits_of(s, w.chunk), tiles = s.nt * a.kv_heads;
     const int parts = ns > 1 ? tiles * ns : 0, items = PER_TILE ? (ns > 1 ? tiles : 0) : tiles * ns;
     const int begin = wave_scan(items) - items, part_begin = wave_scan(parts) - parts;
@@ -182,7 +200,8 @@ __device__ __forceinline__ bool locate(const PagedArgs& a, const PagedClass& c, 
     if (lane == 0) s_tot[wave] = total;
     if (tid == 0) s_hit[0] = -1;
     __syncthreads();
-    w.chunk = chunk_of((s_tot[0] + s_tot[1]) + (s_tot[2] + s_tot[3]));
+    const float per = ((s_tot[0] + s_tot[1]) + (s_tot[2] + s_tot[3])) * a.kv_heads * c.per_round;
+    w.chunk = c.finer ? chunk_of(per) : round_up(per);
     int carry = 0, part_carry = 0;
     for (int b0 = 0; b0 < a.requests; b0 += 256) {
       const Share s = share_of(b0 + tid);
@@ -242,14 +261,14 @@ __device__ __forceinline__ bool locate(const PagedArgs& a, const PagedClass& c, 
 struct Row {
   int64_t q_at, o_at;   // its offsets in q and out
   int lo, hi, pos;
-  float slope;          // log2(e) * slope
+  float slope;          // slope in the units that the scores are kept in
   bool on;
 };
 
 // Row `i` of the tile, G heads a token.  A row the tile does not have sees everything, so that it asks for no mask.
 template <bool FORM>
 __device__ __forceinline__ Row row_of(const PagedArgs& a, const PagedClass& c, const Where& w, int i) {
-  const int t = i / a.group, g = i - t * a.group;
+  const int t = i * a.per_group >> 16, g = i - t * a.group;
   const int token = w.tile * c.tokens + t;
   Row r;
   r.on = t < c.tokens && token < w.n_rows;
@@ -266,7 +285,7 @@ __device__ __forceinline__ Row row_of(const PagedArgs& a, const PagedClass& c, c
     r.hi = 0;
     if (r.pos >= 0) r.hi = min(w.kv, max(r.pos + 1, a.prefix ? a.prefix[w.b] : 0));
     if (a.first) r.lo = max(0, a.first[row]);
-    if (FORM && a.slopes) r.slope = kLog2e * a.slopes[head];
+    if (FORM && a.slopes) r.slope = a.slope_unit * a.slopes[head];
   }
   return r;
 }
@@ -287,13 +306,11 @@ __device__ __forceinline__ float wide_cap(const PagedArgs& a, float qk) {
   return fabsf(x) < 0.25f ? a.cap_log2 * __builtin_fmaf(x * y, p, x) : near_cap(a, qk);
 }
 
-// Scores in log2 units of N products q.k, the i-th `off(i)` keys behind the first, which is `ahead` keys behind the
-// row's own; the branches are the same for every lane of the call.
+// Scores of N products q.k, the i-th with key first_key + off(i); the branches are the same for every lane.
 template <int N, typename V, typename F>
 __device__ __forceinline__ void form_scores(const PagedArgs& a, const Row& r, int first_key, V& s, F off) {
   if (a.cap_log2 == 0.0f) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) s[i] *= a.scale_log2;
+    // as they are
   } else if (!a.wide) {
 #pragma unroll
     for (int i = 0; i < N; ++i) s[i] = near_cap(a, s[i]);
@@ -388,7 +405,7 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
   constexpr int UR = D / 8;                // 16-byte units of a row
   constexpr int NU = kTile * UR / 256;     // units a thread stages of K, and of V
   uint16_t *kbuf0 = stage0, *vbuf0 = stage0 + kTile * D, *kbuf1 = stage1, *vbuf1 = stage1 + kTile * D;
-  __shared__ int s_odd[2], s_range[4][4];
+  __shared__ int s_odd[2];
   Where w;
   if (!locate<false>(a, c, item, w)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -396,29 +413,23 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
   const float ninf = -__builtin_huge_valf();
   const Row r = row_of<FORM>(a, c, w, 32 * wave + l32);
 
-  // keys that all rows see, and that any row sees: of the wave, then of the workgroup
-  const int all_lo = wave_max_i(r.lo), all_hi = -wave_max_i(-r.hi);
-  const int any_lo = -wave_max_i(r.on ? -r.lo : -0x7FFFFFFF), any_hi = wave_max_i(r.on ? r.hi : 0);
-  if (lane == 0) {
-    s_range[wave][0] = all_lo;
-    s_range[wave][1] = all_hi;
-    s_range[wave][2] = any_lo;
-    s_range[wave][3] = any_hi;
+  // Keys that all rows see, and that any row sees, of the workgroup and of the wave (the wave's first key apart).  They
+  // follow from the first and the last token; only first_keys have to be read, two tokens a lane.
+  const int n_tok = min(c.tokens, w.n_rows - w.tile * c.tokens);
+  const int pos0 = a.kv_lens[w.b] - w.n_rows + w.tile * c.tokens, prefix = a.prefix ? a.prefix[w.b] : 0;
+  auto hi_of = [&](int token) { return pos0 + token < 0 ? 0 : min(w.kv, max(pos0 + token + 1, prefix)); };
+  int wg_all_lo = 0, wg_lo = 0;
+  if (a.first) {
+    const int64_t at = w.row0 + w.tile * c.tokens;
+    const int f0 = a.first[at + min(lane, n_tok - 1)], f1 = a.first[at + min(lane + 64, n_tok - 1)];
+    wg_all_lo = max(0, wave_max_i(max(f0, f1)));
+    wg_lo = max(0, -wave_max_i(max(-f0, -f1)));
   }
-  if (tid < 2) s_odd[tid] = -1;
-  __syncthreads();
-  int wg_all_lo = 0, wg_all_hi = 0x7FFFFFFF, wg_lo = 0x7FFFFFFF, wg_hi = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    wg_all_lo = max(wg_all_lo, s_range[i][0]);
-    wg_all_hi = min(wg_all_hi, s_range[i][1]);
-    wg_lo = min(wg_lo, s_range[i][2]);
-    wg_hi = max(wg_hi, s_range[i][3]);
-  }
-  wg_all_lo = __builtin_amdgcn_readfirstlane(wg_all_lo);
-  wg_all_hi = __builtin_amdgcn_readfirstlane(wg_all_hi);
-  const int begin = __builtin_amdgcn_readfirstlane(max(w.split * w.chunk, wg_lo / kTile * kTile));
-  const int end = __builtin_amdgcn_readfirstlane(static_cast<int>(min(static_cast<int64_t>(w.split + 1) * w.chunk, static_cast<int64_t>(wg_hi))));
+  const int wg_all_hi = hi_of(0), wg_hi = hi_of(n_tok - 1);
+  const int tok_a = 32 * wave * a.per_group >> 16, tok_b = (32 * wave + 31) * a.per_group >> 16;
+  const int any_hi = tok_a < n_tok ? hi_of(min(tok_b, n_tok - 1)) : 0;
+  const int begin = max(w.split * w.chunk, wg_lo / kTile * kTile);
+  const int end = static_cast<int>(min(static_cast<int64_t>(w.split + 1) * w.chunk, static_cast<int64_t>(wg_hi)));
 
   u32x4_t qf[KS];
 #pragma unroll
@@ -446,15 +457,27 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
   auto group_of = [&](int u) { return NU == 4 ? u : 2 * u + (wave >> 1); };   // of pass u and this wave
   const int64_t k_page = 2 * a.k_page, v_page = 2 * a.v_page;
   const uint32_t k_tok = 2 * static_cast<uint32_t>(a.k_tok), v_tok = 2 * static_cast<uint32_t>(a.v_tok);
-  bool hole = false;   // the loaded tile has keys without a page
-  auto load = [&](int t0, uint16_t* kb, uint16_t* vb) {
-    int ids[4];
+  const auto* table_row = (const __attribute__((address_space(4))) int32_t*)(a.table + w.b * a.table_ld);
+  // The pages of a tile's four 16-key groups, -1 where there is none: the table's entries are read all at once (past
+  // the request's end its last one), and before they are needed.
+  struct Pages {
+    int id[4];
+  };
+  auto pages_of = [&](int t0) __attribute__((always_inline)) {
+    Pages p;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) ids[g] = page_id(a, w, t0 + 16 * g);
-    hole = (ids[0] | ids[1] | ids[2] | ids[3]) < 0;
+    for (int g = 0; g < 4; ++g) p.id[g] = table_row[min(t0 + 16 * g, w.kv - 1) >> a.shift];
+    return p;
+  };
+  bool hole = false;   // the loaded tile has keys without a page
+  auto load = [&](int t0, Pages p, uint16_t* kb, uint16_t* vb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      if (static_cast<unsigned>(p.id[g]) >= static_cast<unsigned>(a.pages)) p.id[g] = -1;
+    hole = (p.id[0] | p.id[1] | p.id[2] | p.id[3]) < 0;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-      const int id = max(NU == 4 ? ids[u % 4] : wave >> 1 ? ids[(2 * u + 1) % 4] : ids[2 * u % 4], 0);
+      const int id = max(NU == 4 ? p.id[u % 4] : wave >> 1 ? p.id[(2 * u + 1) % 4] : p.id[2 * u % 4], 0);
       const uint32_t at = (t0 + 16 * group_of(u)) & page_mask;
       load_lds16(kh + id * k_page + static_cast<uint64_t>(at) * k_tok + k_off, kb + 8 * (256 * u + 64 * wave));
       load_lds16(vh + id * v_page + static_cast<uint64_t>(at) * v_tok + v_off, vb + 8 * (256 * u + 64 * wave));
@@ -463,15 +486,18 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
   // Where some row does not see all of a tile, what of V no row may read (a page's rest) becomes zero before it is
   // used, and so do infinities and NaN, which a zero weight would not hide; add_odd adds those to the rows that do
   // see them.
-  auto clean_tile = [&](int t0, uint16_t* vb, int buf) {
+  auto clean_tile = [&](int t0, bool holes, uint16_t* vb, int buf) {
+    u32x4_t x[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) x[u] = *reinterpret_cast<u32x4_t*>(vb + 8 * (256 * u + tid));
     bool odd = false;
-#pragma unroll 1
+#pragma unroll
     for (int u = 0; u < NU; ++u) {
-      u32x4_t x = *reinterpret_cast<u32x4_t*>(vb + 8 * (256 * u + tid));
-      const int key = t0 + u_row + u * (256 / UR);
-      if (page_id(a, w, t0 + 16 * group_of(u)) < 0 || key >= w.kv) x = u32x4_t{0u, 0u, 0u, 0u};
-      else odd |= clean<F16>(x);
-      *reinterpret_cast<u32x4_t*>(vb + 8 * (256 * u + tid)) = x;
+      const bool rest = t0 + u_row + u * (256 / UR) >= w.kv || (holes && page_id(a, w, t0 + 16 * group_of(u)) < 0);
+      if (rest) x[u] = u32x4_t{0u, 0u, 0u, 0u};
+      const bool any = !rest && clean<F16>(x[u]);
+      odd |= any;
+      if (rest || any) *reinterpret_cast<u32x4_t*>(vb + 8 * (256 * u + tid)) = x[u];
     }
     if (odd) s_odd[buf] = t0;
     __syncthreads();
@@ -496,8 +522,9 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
 
   const int k_at = l32 * D, k_sw = swizzle<D>(l32);
   const int v_row = 4 * half + ((lane & 15) >> 2), v_unit = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), v_el = 4 * (lane & 1);
-  auto compute = [&](int t0, bool masked, const uint16_t* kb_, const uint16_t* vb_, int buf) {
-    if (t0 >= any_hi || t0 + kTile <= any_lo) return;   // no row of the wave sees any of it
+  auto compute = [&](int t0, bool masked, bool holes, const uint16_t* kb_, const uint16_t* vb_, int buf) __attribute__((always_inline)) {
+    if (t0 >= any_hi) return;   // no row of the wave sees any of it
+
     f32x16_t s[2];
     {
       u32x4_t kf[2][KS];
@@ -512,6 +539,14 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
         for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) s[kb] = mfma_32x32x16<F16>(kf[kb][ks], qf[ks], s[kb]);
+      }
+      // four fragments ahead of the matrix instruction that takes them (2170 -> 2088 us at 2048 x 65536, 32/8 heads;
+      // all of them first: 2245)
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);   // LDS reads
+#pragma unroll
+      for (int i = 0; i < 2 * KS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // matrix instruction
+        if (i < 2 * KS - 4) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
     }
     const int key0 = t0 + 4 * half;   // element i of tile kb: key0 + 32 kb + 8 (i / 4) + i % 4
@@ -530,12 +565,14 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
           if (static_cast<unsigned>(32 * kb + 8 * (i >> 2) + (i & 3) - from) >= span) s[kb][i] = ninf;
           if ((i & 3) == 3) __builtin_amdgcn_sched_barrier(0);   // few lane masks live at a time
         }
+      if (holes) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        if (page_id(a, w, t0 + 16 * g) < 0) {   // a page the request does not have
+        for (int g = 0; g < 4; ++g)
+          if (page_id(a, w, t0 + 16 * g) < 0) {   // a page the request does not have
 #pragma unroll
-          for (int i = 0; i < 8; ++i) s[g >> 1][8 * (g & 1) + i] = ninf;
-        }
+            for (int i = 0; i < 8; ++i) s[g >> 1][8 * (g & 1) + i] = ninf;
+          }
+      }
     }
     float cm = s[0][0];
 #pragma unroll
@@ -543,7 +580,7 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
 #pragma unroll
       for (int i = 0; i < 16; ++i) cm = fmaxf(cm, s[kb][i]);
     cm = max_x32(cm);
-    const float sl = FORM ? 1.0f : a.scale_log2;
+    const float sl = a.unit_log2;
     cm = cm * sl - kShift<F16>;
     const float mn = fmaxf(m, cm);
     if (__ballot(mn > m + kLazyLog2)) {   // wave-uniform
@@ -585,15 +622,17 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
   };
 
   // One barrier a tile: the next tile's loads are issued before this one is computed, and have landed behind it.
-  auto turn = [&](int t0, const uint16_t* kb_, uint16_t* vb_, int buf, uint16_t* kn, uint16_t* vn) {
-    const bool masked = t0 < wg_all_lo || t0 + kTile > wg_all_hi || hole;
-    if (t0 + kTile < end) load(t0 + kTile, kn, vn);
-    if (masked) clean_tile(t0, vb_, buf);
-    compute(t0, masked, kb_, vb_, buf);
+  auto turn = [&](int t0, const uint16_t* kb_, uint16_t* vb_, int buf, uint16_t* kn, uint16_t* vn) __attribute__((always_inline)) {
+    const bool holes = hole, masked = t0 < wg_all_lo || t0 + kTile > wg_all_hi || holes;
+    const Pages next = pages_of(t0 + kTile);
+    if (masked) clean_tile(t0, holes, vb_, buf);
+    if (t0 + kTile < end) load(t0 + kTile, next, kn, vn);
+    compute(t0, masked, holes, kb_, vb_, buf);
     loads_landed();
   };
+  if (tid < 2) s_odd[tid] = -1;
   if (begin < end) {
-    load(begin, kbuf0, vbuf0);
+    load(begin, pages_of(begin), kbuf0, vbuf0);
     loads_landed();
     for (int t0 = begin; t0 < end; t0 += 2 * kTile) {
       turn(t0, kbuf0, vbuf0, 0, kbuf1, vbuf1);
@@ -603,16 +642,24 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
 
   l = sum_x32(l);
   if (w.n_split == 1) {
-    if (!r.on) return;
+    // by way of LDS (the wave's own part: the loop's last barrier has passed), so that whole rows are stored: 2.5 us a
+    // workgroup for 8-byte stores to 32 rows at a time
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* out = a.out + r.o_at + 4 * half;
+    uint16_t* mine = stage0 + wave * 32 * D;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const float x[4] = {o[d][4 * q] * inv, o[d][4 * q + 1] * inv, o[d][4 * q + 2] * inv, o[d][4 * q + 3] * inv};
-        *reinterpret_cast<u32x2_t*>(out + 32 * d + 8 * q) = pack4_half<F16>(x);
+        *reinterpret_cast<u32x2_t*>(mine + l32 * D + 8 * ((4 * d + q) ^ (l32 & (UR - 1))) + 4 * half) = pack4_half<F16>(x);
       }
+#pragma unroll
+    for (int i = 0; i < 32 * UR / 64; ++i) {
+      const int row = i * (64 / UR) + lane / UR, unit = lane % UR;
+      const u32x4_t x = *reinterpret_cast<const u32x4_t*>(mine + row * D + 8 * (unit ^ (row & (UR - 1))));
+      const Row ro = row_of<false>(a, c, w, 32 * wave + row);
+      if (ro.on) *reinterpret_cast<u32x4_t*>(a.out + ro.o_at + 8 * unit) = x;
+    }
     return;
   }
   const int64_t at = static_cast<int64_t>(w.part) * kRowsM + 32 * wave + l32;
@@ -741,7 +788,7 @@ __device__ __forceinline__ void token_body(const PagedArgs& a, const PagedClass&
     u32x4_t p[NQ];
     float mn[NQ];
     bool raise = false;
-    const float sl = FORM ? 1.0f : a.scale_log2;
+    const float sl = a.unit_log2;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       float cm = ninf;
@@ -906,7 +953,7 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedArgs a, PagedC
 }
 // Requests of both classes in one launch, the long ones first.
 template <int D, bool F16, bool FORM>
-__global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs a, PagedClass rows, PagedClass token, int n_rows) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_rows_kernel(PagedArgs a, PagedClass rows, PagedClass token, int n_rows) {
   __shared__ __attribute__((aligned(16))) uint16_t stage0[2 * kTile * D], stage1[2 * kTile * D];
   if (static_cast<int>(blockIdx.x) < n_rows) rows_body<D, F16, FORM>(a, rows, blockIdx.x, stage0, stage1);
   else token_body<D, F16, FORM, 2>(a, token, blockIdx.x - n_rows, stage0, stage1);
@@ -917,12 +964,12 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs a, PagedCl
 // on which workgroup was done first.  Tiles of the token kernel have few rows and up to a thousand parts (one row at a
 // time), those of the rows kernel many rows and few parts.
 template <int D, bool F16, int M, int R, int G>
-__device__ __forceinline__ void join_body(const PagedArgs& a, const PagedClass& c, int item) {
+__device__ __forceinline__ bool join_body(const PagedArgs& a, const PagedClass& c, int item) {
   constexpr int L = D / 4;             // lanes of a row, 4 values each
   constexpr int P = 256 / (R * L);
   __shared__ float s_acc[P][R][D], s_m[P][R], s_l[P][R];
   Where w;
-  if (!locate<true>(a, c, item / G, w)) return;
+  if (!locate<true>(a, c, item / G, w)) return false;
   const int in_tile = threadIdx.x / L % R, group = threadIdx.x / (L * R), d0 = 4 * (threadIdx.x % L);
   const int n_rows = min(c.tokens, w.n_rows - w.tile * c.tokens) * a.group;
   const float ninf = -__builtin_huge_valf();
@@ -976,12 +1023,18 @@ __device__ __forceinline__ void join_body(const PagedArgs& a, const PagedClass& 
     const float z[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
     *reinterpret_cast<u32x2_t*>(a.out + r.o_at + d0) = pack4_half<F16>(z);
   }
+  return true;
 }
 
 template <int D, bool F16, int NQ>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, PagedClass rows, PagedClass token, int n_rows) {
-  if (static_cast<int>(blockIdx.x) < n_rows) join_body<D, F16, kRowsM, 8, kRowsJoins>(a, rows, blockIdx.x);
-  else join_body<D, F16, NQ * kTokenM, 1, kTokenJoins>(a, token, blockIdx.x - n_rows);
+  // few workgroups for the many items there may be: a workgroup without work costs a microsecond, in rounds
+  if (static_cast<int>(blockIdx.x) < n_rows) {
+    for (int i = blockIdx.x; join_body<D, F16, kRowsM, 8, kRowsJoins>(a, rows, i); i += n_rows) __syncthreads();
+  } else {
+    for (int i = blockIdx.x - n_rows; join_body<D, F16, NQ * kTokenM, 1, kTokenJoins>(a, token, i); i += gridDim.x - n_rows)
+      __syncthreads();
+  }
 }
 
 // The launches of a call, from what the host knows: rows, requests, and the tokens a table row covers.
@@ -1051,14 +1104,15 @@ template <int D, bool F16, bool FORM>
 int launch(const PagedArgs& a, const Plan& p, hipStream_t st) {
   const auto n = [](int64_t x) { return static_cast<unsigned>(x); };
   if (p.rows.items) {
-    paged_rows_kernel<D, F16, FORM><<<n(p.rows.items + p.token.items), 256, 0, st>>>(a, p.rows.cls, p.token.cls,
-                                                                                   static_cast<int>(p.rows.items));
+    paged_rows_kernel<D, F16, FORM><<<n(p.rows.items + p.token.items), 256, 0, st>>>(
+        a, p.rows.cls, p.token.cls, static_cast<int>(p.rows.items));
   } else if (p.sets == 1) {
     paged_token_kernel<D, F16, FORM, 1><<<n(p.token.items), 256, 0, st>>>(a, p.token.cls);
   } else {
     paged_token_kernel<D, F16, FORM, 2><<<n(p.token.items), 256, 0, st>>>(a, p.token.cls);
   }
-  const int64_t joins = p.rows.tiles * kRowsJoins, all = joins + p.token.tiles * kTokenJoins;
+  const int64_t joins = std::min<int64_t>(p.rows.tiles * kRowsJoins, 2 * kRound);
+  const int64_t all = joins + std::min<int64_t>(p.token.tiles * kTokenJoins, 2 * kRound);
   if (all) {
     if (p.sets == 1)
       paged_join_kernel<D, F16, 1><<<n(all), 256, 0, st>>>(a, p.rows.cls, p.token.cls, static_cast<int>(joins));
@@ -1132,10 +1186,13 @@ QKV_EXPORT int qkv_paged_attention(const void* query, const int64_t* q_strides, 
   a.shift = __builtin_ctz(static_cast<unsigned>(page));
   a.requests = static_cast<int>(requests), a.rows = static_cast<int>(rows);
   a.kv_heads = static_cast<int>(kv_heads), a.group = static_cast<int>(group);
+  a.per_group = 65536 / a.group + 1;
   a.scale_log2 = scaling * kLog2e;
   a.tanh_scale = softcap > 0.0f ? 2.0f * kLog2e * scaling / softcap : 0.0f;
   a.cap_log2 = softcap * kLog2e;
   a.wide = softcap > kNearCap;
+  a.unit_log2 = softcap > 0.0f ? 1.0f : a.scale_log2;
+  a.slope_unit = softcap > 0.0f ? kLog2e : 1.0f / scaling;
   p.rows.cls.acc = static_cast<float*>(workspace);
   p.token.cls.acc = p.rows.cls.acc + head_dim * p.rows.parts * kRowsM;
   p.rows.cls.ml = p.token.cls.acc + head_dim * p.token.parts * p.sets * kTokenM;

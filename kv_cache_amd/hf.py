@@ -47,6 +47,16 @@ lagged modes (``lagtop2`` / ``lagrefresh{N}`` / ``qdrift…`` / ``pconf{T}`` +
 (K/V [B, Hkv, T, D] with the current token last).  As the reference's hook
 dispatches these modes only for one query per sequence (EV:6236, 6308,
 6414-6448), prefill stays dense SDPA.
+
+``PagedCache`` with the implementation of ``register_paged`` keeps K/V in pages
+(``paged``) and runs prompts, chunks and decode steps densely over them,
+left-padded batches included: padding takes no slot, and every sequence has
+its own length on the GPU.
+
+    hf.register_paged()                                   # attn_implementation "paged"
+    model.config._attn_implementation = "paged"
+    cache = hf.PagedCache(capacity=40960, page=64)
+    out = model.generate(**tokenizer(prompts, padding=True), past_key_values=cache)
 """
 
 from __future__ import annotations
@@ -58,6 +68,7 @@ import weakref
 import torch
 
 from . import int4 as K
+from . import paged
 
 # Cache layers by the address of their K buffer: the attention function gets
 # K as a view of that buffer and finds the layer's int4 state through it.
@@ -316,3 +327,161 @@ def register_mode(mode: str, capacity: int, *, name: str | None = None, **step_k
 
 
 ATTENTION_STEPS: dict = {}
+
+
+class _PagedState:
+    """What the layers of one PagedCache share: the page table, and the plan
+    of the step that the first layer to reach it made."""
+
+    def __init__(self, capacity: int, page: int):
+        self.capacity, self.page = int(capacity), int(page)
+        self.table = self.plan = None
+        self.length = 0          # columns stepped, padding included
+
+    def step(self, length: int, n: int, batch: int, device, attention_mask, window) -> paged.StepPlan:
+        """The plan of the step that brings the sequences to ``length``
+        columns with ``n`` new ones."""
+        if self.length == length:
+            return self.plan
+        if self.table is None:
+            pages = batch * -(-self.capacity // self.page)
+            self.table = paged.PageTable(batch, self.capacity, pages, self.page, device)
+        new = torch.full((batch,), n, dtype=torch.int32, device=device)
+        if attention_mask is not None and n > 1:
+            if window is not None and n > window:
+                raise RuntimeError(f"a masked chunk of {n} tokens on a layer with a sliding window of {window}: split it")
+            # the last query's view of the step's own columns: padding is hidden
+            seen = attention_mask[..., -1, length - n:length].reshape(-1, n)
+            seen = seen if seen.dtype == torch.bool else seen == 0
+            if not bool((seen[:, 1:] | ~seen[:, :-1]).all()):
+                raise RuntimeError("paged attention takes left-padded batches (padding before the tokens of a step)")
+            new = seen.sum(-1, dtype=torch.int32).expand(batch).contiguous()
+        self.plan = self.table.step(new, batch * n, padded=n)
+        self.length = length
+        return self.plan
+
+    def reset(self) -> None:
+        if self.table is not None and self.length:
+            self.table.release(torch.zeros_like(self.table.lens))
+        self.length = 0
+
+
+class PagedCacheLayer:
+    """One layer's K/V pages (bf16 or fp16).  ``update`` only counts the new
+    columns and hands the layer on to the attention function with their K/V;
+    that one knows the mask, and writes what is no padding into the pages."""
+
+    is_sliding = False
+    is_compileable = False
+    supports_early_init = False
+
+    def __init__(self, state: _PagedState):
+        self.state = state
+        self.keys = self.values = None        # no dense K/V exist
+        self.k_pages = self.v_pages = None
+        self.is_initialized = False
+        self.length = 0
+
+    def __repr__(self):
+        return f"PagedCacheLayer(length={self.length}, capacity={self.state.capacity}, page={self.state.page})"
+
+    # -- CacheLayerMixin protocol ------------------------------------------
+    def lazy_initialization(self, key_states: torch.Tensor, value_states: torch.Tensor) -> None:
+        b, h, _, d = key_states.shape
+        shape = (b * -(-self.state.capacity // self.state.page), h, self.state.page, d)
+        self.dtype, self.device = key_states.dtype, key_states.device
+        self.k_pages = torch.empty(shape, dtype=key_states.dtype, device=key_states.device)
+        self.v_pages = torch.empty(shape, dtype=value_states.dtype, device=key_states.device)
+        self.is_initialized = True
+
+    def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args, **kwargs):
+        if not self.is_initialized:
+            self.lazy_initialization(key_states, value_states)
+        n = key_states.size(-2)
+        if self.length + n > self.state.capacity:
+            raise RuntimeError(f"Paged cache capacity {self.state.capacity} exceeded ({self.length + n} tokens)")
+        self.length += n
+        key_states = key_states.view(key_states.shape)
+        key_states.paged_layer = self
+        return key_states, value_states
+
+    def get_mask_sizes(self, query_length: int):
+        return self.length + query_length, 0
+
+    def get_seq_length(self) -> int:
+        return self.length
+
+    def get_max_length(self) -> int:
+        return self.state.capacity
+
+    def reset(self) -> None:
+        self.length = 0
+        self.state.reset()
+
+    def crop(self, max_length: int) -> None:
+        raise RuntimeError("PagedCacheLayer cannot be cropped")
+
+    def reorder_cache(self, beam_idx) -> None:
+        raise RuntimeError("PagedCacheLayer cannot be reordered")
+
+    batch_repeat_interleave = batch_select_indices = reorder_cache
+
+    def offload(self):
+        raise RuntimeError("PagedCacheLayer cannot be offloaded")
+
+    prefetch = offload
+
+
+class PagedCache:
+    """A transformers ``Cache`` whose layers keep K/V in pages of ``page``
+    tokens under one page table; ``capacity`` bounds the columns (tokens and
+    padding) of a sequence."""
+
+    def __new__(cls, capacity: int, page: int = 64):
+        from transformers.cache_utils import Cache, CacheLayerMixin
+
+        if not (16 <= page <= 4096 and page & (page - 1) == 0):
+            raise RuntimeError(f"page must be a power of two in [16, 4096], got {page}")
+        return Cache(layer_class_to_replicate=functools.partial(_paged_layer_class(CacheLayerMixin),
+                                                               _PagedState(capacity, page)))
+
+
+@functools.lru_cache(maxsize=1)
+def _paged_layer_class(mixin):
+    return type("PagedCacheLayerHF", (PagedCacheLayer, mixin), {"__init__": PagedCacheLayer.__init__})
+
+
+def paged_attention_forward(module, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, attention_mask,
+                            scaling: float | None = None, dropout: float = 0.0, softcap: float | None = None,
+                            sliding_window: int | None = None, **kwargs):
+    """HF attention interface (query [B,Hq,n,D]; key/value [B,Hkv,n,D], the new
+    columns a PagedCache layer handed on) -> (out [B,n,Hq,D], None); columns of
+    padding get zeros.  Without a PagedCache: dense SDPA."""
+    from transformers.integrations.sdpa_attention import sdpa_attention_forward
+
+    layer = getattr(key, "paged_layer", None)
+    if layer is None:
+        return sdpa_attention_forward(module, query, key, value, attention_mask, dropout=dropout, scaling=scaling,
+                                      **kwargs)
+    if dropout:
+        raise RuntimeError("paged attention has no dropout")
+    b, hq, n, d = query.shape
+    state = layer.state
+    plan = state.step(layer.length, n, b, query.device, attention_mask, sliding_window)
+    rows = lambda x: x.transpose(1, 2).reshape(b * n, x.size(1), d)  # noqa: E731  (a view of what projections give)
+    paged.append(rows(key), rows(value), layer.k_pages, layer.v_pages, plan.slots)
+    first = None if sliding_window is None else plan.positions - (int(sliding_window) - 1)
+    out = paged.attention(rows(query), layer.k_pages, layer.v_pages, state.table.table, plan.cu_rows, plan.kv_lens,
+                          d ** -0.5 if scaling is None else float(scaling), max_rows=n,
+                          softcap=0.0 if softcap is None else float(softcap), first_keys=first)
+    return out.view(b, n, hq, d), None
+
+
+def register_paged(name: str = "paged") -> str:
+    """Register the paged attention function with transformers under ``name``."""
+    from transformers import AttentionInterface
+    from transformers.masking_utils import AttentionMaskInterface, sdpa_mask
+
+    AttentionInterface.register(name, paged_attention_forward)
+    AttentionMaskInterface.register(name, sdpa_mask)
+    return name

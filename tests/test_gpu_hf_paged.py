@@ -1,0 +1,128 @@
+"""The paged cache inside a transformers Qwen3 model (random init): prompts,
+chunks and decode steps against dense SDPA on a DynamicCache, left-padded
+batches included.  Logits agree within the bf16 tolerance of the int4 tests
+(two attention implementations, each rounded to bf16 in every layer)."""
+
+import pytest
+import torch
+
+from kv_cache_amd import hf
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _model(layers=2, head_dim=128, heads=4, dtype=torch.bfloat16):
+    from transformers import Qwen3Config, Qwen3ForCausalLM
+
+    torch.manual_seed(0)
+    cfg = Qwen3Config(vocab_size=512, hidden_size=256, intermediate_size=512, num_hidden_layers=layers,
+                      num_attention_heads=heads, num_key_value_heads=2, head_dim=head_dim, max_position_embeddings=4096,
+                      rope_theta=1.0e6)
+    return Qwen3ForCausalLM(cfg).to(DEV, dtype).eval()
+
+
+def _tokens(b, n, seed):
+    return torch.randint(1, 512, (b, n), generator=torch.Generator().manual_seed(seed)).to(DEV)
+
+
+def _run(model, impl, cache, chunks, masks):
+    """Logits of every chunk of tokens, fed one after the other."""
+    model.config._attn_implementation = impl
+    out = []
+    with torch.no_grad():
+        for ids, mask in zip(chunks, masks):
+            kw = {}
+            if mask is not None:
+                kw = dict(attention_mask=mask, position_ids=(mask.long().cumsum(-1) - 1).clamp(min=0)[:, -ids.size(1):])
+            out.append(model(ids, past_key_values=cache, use_cache=True, **kw).logits.float())
+    return out
+
+
+def _dense(model):
+    from transformers.cache_utils import DynamicCache
+
+    return DynamicCache(config=model.config)
+
+
+@pytest.mark.parametrize("head_dim,heads,page,dtype", [(128, 4, 64, torch.bfloat16), (64, 2, 16, torch.float16),
+                                                      (128, 8, 128, torch.bfloat16)])
+def test_prompt_chunks_and_steps_match_dense(head_dim, heads, page, dtype):
+    hf.register_paged()
+    model = _model(head_dim=head_dim, heads=heads, dtype=dtype)
+    chunks = [_tokens(2, n, 10 + i) for i, n in enumerate((130, 57, 1, 1, 5, 1))]
+    cache = hf.PagedCache(capacity=256, page=page)
+    got = _run(model, "paged", cache, chunks, [None] * 6)
+    want = _run(model, "sdpa", _dense(model), chunks, [None] * 6)
+    for g, w in zip(got, want):
+        torch.testing.assert_close(g, w, rtol=3e-2, atol=3e-2)
+    assert cache.get_seq_length() == 195
+    state = cache.layers[0].state
+    assert state.table.lens.tolist() == [195, 195]
+    assert all(layer.state is state for layer in cache.layers)
+
+
+def test_left_padded_batch_matches_each_alone():
+    hf.register_paged()
+    model = _model()
+    lens, n = [40, 7, 25], 40
+    alone = [_tokens(1, k + 3, 30 + k) for k in lens]
+    ids = torch.zeros((3, n), dtype=torch.long, device=DEV)
+    mask = torch.zeros((3, n + 3), dtype=torch.long, device=DEV)
+    for b, k in enumerate(lens):
+        ids[b, n - k:], mask[b, n - k:] = alone[b][0, :k], 1
+    chunks = [ids] + [torch.stack([alone[b][0, k + i] for b, k in enumerate(lens)])[:, None] for i in range(3)]
+    cache = hf.PagedCache(capacity=64, page=16)
+    got = _run(model, "paged", cache, chunks, [mask[:, : n + i] for i in range(4)])
+    state = cache.layers[0].state
+    assert state.table.lens.tolist() == [k + 3 for k in lens]
+    # padding takes no page: 3 + 1 + 2 of 16 tokens
+    assert int(state.table.count) == 12 - sum(-(-(k + 3) // 16) for k in lens)
+    for b, k in enumerate(lens):
+        want = _run(model, "sdpa", _dense(model), [alone[b]], [None])[0][0]
+        torch.testing.assert_close(got[0][b, n - k:], want[:k], rtol=3e-2, atol=3e-2)
+        for i in range(3):
+            torch.testing.assert_close(got[1 + i][b, 0], want[k + i], rtol=3e-2, atol=3e-2)
+
+
+def test_generate_and_reset():
+    hf.register_paged()
+    model = _model()
+    model.config._attn_implementation = "paged"
+    ids = _tokens(2, 50, 50)
+    mask = torch.ones_like(ids)
+    mask[1, :20] = 0
+    cache = hf.PagedCache(capacity=80, page=16)
+    with torch.no_grad():
+        a = model.generate(ids, attention_mask=mask, past_key_values=cache, max_new_tokens=8, do_sample=False)
+        assert a.shape == (2, 58)
+        cache.reset()
+        assert cache.get_seq_length() == 0
+        table = cache.layers[0].state.table
+        assert int(table.count) == table.pages and table.lens.tolist() == [0, 0]
+        b = model.generate(ids, attention_mask=mask, past_key_values=cache, max_new_tokens=8, do_sample=False)
+    assert torch.equal(a, b)
+
+
+def test_refusals():
+    hf.register_paged()
+    model = _model(layers=1)
+    with pytest.raises(RuntimeError, match="power of two"):
+        hf.PagedCache(capacity=64, page=20)
+    cache = hf.PagedCache(capacity=16, page=16)
+    with pytest.raises(RuntimeError, match="capacity 16 exceeded"):
+        _run(model, "paged", cache, [_tokens(1, 17, 1)], [None])
+    # padding behind the tokens
+    ids, mask = _tokens(2, 12, 2), torch.ones((2, 12), dtype=torch.long, device=DEV)
+    mask[1, 8:] = 0
+    with pytest.raises(RuntimeError, match="left-padded"):
+        _run(model, "paged", hf.PagedCache(capacity=64, page=16), [ids], [mask])
+
+
+def test_without_a_paged_cache_it_is_dense():
+    hf.register_paged()
+    model = _model(layers=1)
+    ids = _tokens(2, 33, 3)
+    got = _run(model, "paged", _dense(model), [ids], [None])
+    want = _run(model, "sdpa", _dense(model), [ids], [None])
+    assert torch.equal(got[0], want[0])
