@@ -957,7 +957,8 @@ int64_t qkv_paged_attention_workspace_bytes(int64_t rows, int64_t max_rows, int6
 /* Attention of a step's rows over the cache: single tokens, drafted tokens,
  * chunks of prompts and whole prompts, mixed as they come.  query / out
  * [rows, q_heads, head_dim] with strides {row, head}; pages as in
- * qkv_paged_append; table, cu_rows and kv_lens as in qkv_paged_plan.  Row i
+ * qkv_paged_append, of K and V with the same strides (a page's tokens within
+ * 2^30 elements); table, cu_rows and kv_lens as in qkv_paged_plan.  Row i
  * of request b is the token at p = kv_lens[b] - (cu_rows[b+1] - cu_rows[b])
  * + i and sees the keys j with first_keys[row] <= j < max(p + 1,
  * prefix_lens[b]), j < kv_lens[b]; a row with p < 0 or without a key gets
@@ -974,9 +975,8 @@ int64_t qkv_paged_attention_workspace_bytes(int64_t rows, int64_t max_rows, int6
  * the result does not depend on it.  head_dim 64 or 128, at most 128 query
  * heads per KV head, scaling > 0.  workspace: 16-byte aligned, contents
  * irrelevant; calls sharing one must not overlap in time. */
-int qkv_paged_attention(const void* query, const int64_t* q_strides, const void* k_pages, const int64_t* k_strides,
-                        const void* v_pages, const int64_t* v_strides, int64_t pages, int64_t page,
-                        const int32_t* table, int64_t table_ld, int64_t width, int64_t requests,
+int qkv_paged_attention(const void* query, const int64_t* q_strides, const void* k_pages, const void* v_pages,
+                        const int64_t* page_strides, int64_t pages, int64_t page, const int32_t* table, int64_t table_ld, int64_t width, int64_t requests,
                         const int32_t* cu_rows, const int32_t* kv_lens, int64_t rows, int64_t max_rows,
                         int64_t q_heads, int64_t kv_heads, int64_t head_dim, float scaling, float softcap,
                         const float* slopes, const int32_t* prefix_lens, const int32_t* first_keys, void* workspace,

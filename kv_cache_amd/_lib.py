@@ -146,7 +146,7 @@ _PROTOTYPES = {
     # strides by address: the callers lay all of a call's out in one array
     "qkv_paged_append": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
     "qkv_paged_attention_workspace_bytes": (_i64, [_i64] * 8),
-    "qkv_paged_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64,
+    "qkv_paged_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64,
                                    _i64, _i64, _i64, _i64, _f32, _f32, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i32,
                                    _vp]),
 }

@@ -40,7 +40,8 @@ constexpr uint32_t kOnes = F16 ? 0x3C003C00u : 0x3F803F80u;   // a pair of 1.0
 struct PagedArgs {
   const uint16_t *q, *k, *v;
   uint16_t* out;
-  int64_t q_row, q_head, k_page, k_head, k_tok, v_page, v_head, v_tok, o_row, o_head;
+  int64_t q_row, q_head, page, head, o_row, o_head;   // strides; pages of K and V share theirs
+  uint32_t tok;                                       // (page * tok fits 31 bits)
   const int32_t *table, *cu, *kv_lens, *prefix, *first;
   const float* slopes;
   int64_t table_ld;
@@ -449,14 +450,13 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
   // 16-key group, so in one page, and their address is a wave-uniform base and a constant offset.  LDS holds unit
   // tid of a pass at place tid, the swizzle is in which column is read.
   const int u_row = tid / UR, u_col = (tid % UR) ^ swizzle<D>(tid / UR);
-  const uint32_t k_off = 2 * ((u_row & 15) * static_cast<uint32_t>(a.k_tok) + 8 * u_col);
-  const uint32_t v_off = 2 * ((u_row & 15) * static_cast<uint32_t>(a.v_tok) + 8 * u_col);
-  const char* kh = reinterpret_cast<const char*>(a.k + w.head * a.k_head);
-  const char* vh = reinterpret_cast<const char*>(a.v + w.head * a.v_head);
+  const uint32_t off = 2 * ((u_row & 15) * a.tok + 8 * u_col);
+  const char* kh = reinterpret_cast<const char*>(a.k + w.head * a.head);
+  const char* vh = reinterpret_cast<const char*>(a.v + w.head * a.head);
   const int page_mask = (1 << a.shift) - 1;
   auto group_of = [&](int u) { return NU == 4 ? u : 2 * u + (wave >> 1); };   // of pass u and this wave
-  const int64_t k_page = 2 * a.k_page, v_page = 2 * a.v_page;
-  const uint32_t k_tok = 2 * static_cast<uint32_t>(a.k_tok), v_tok = 2 * static_cast<uint32_t>(a.v_tok);
+  const int64_t page_bytes = 2 * a.page;
+  const uint32_t tok_bytes = 2 * a.tok;
   const auto* table_row = (const __attribute__((address_space(4))) int32_t*)(a.table + w.b * a.table_ld);
   // The pages of a tile's four 16-key groups, -1 where there is none: the table's entries are read all at once (past
   // the request's end its last one), and before they are needed.
@@ -478,9 +478,9 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int id = max(NU == 4 ? p.id[u % 4] : wave >> 1 ? p.id[(2 * u + 1) % 4] : p.id[2 * u % 4], 0);
-      const uint32_t at = (t0 + 16 * group_of(u)) & page_mask;
-      load_lds16(kh + id * k_page + static_cast<uint64_t>(at) * k_tok + k_off, kb + 8 * (256 * u + 64 * wave));
-      load_lds16(vh + id * v_page + static_cast<uint64_t>(at) * v_tok + v_off, vb + 8 * (256 * u + 64 * wave));
+      const int64_t at = id * page_bytes + ((t0 + 16 * group_of(u)) & page_mask) * tok_bytes;
+      load_lds16(kh + at + off, kb + 8 * (256 * u + 64 * wave));
+      load_lds16(vh + at + off, vb + 8 * (256 * u + 64 * wave));
     }
   };
   // Where some row does not see all of a tile, what of V no row may read (a page's rest) becomes zero before it is
@@ -507,7 +507,7 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
     for (int j = 0; j < kTile; ++j) {
       const int key = t0 + j, id = page_id(a, w, key);
       if (id < 0) continue;
-      const uint16_t* vr = a.v + id * a.v_page + w.head * a.v_head + (key & page_mask) * a.v_tok + 4 * half;
+      const uint16_t* vr = a.v + id * a.page + w.head * a.head + (key & page_mask) * a.tok + 4 * half;
       if (!(r.on && key >= r.lo && key < r.hi)) continue;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
@@ -724,14 +724,14 @@ __device__ __forceinline__ void token_body(const PagedArgs& a, const PagedClass&
     for (int d = 0; d < DB; ++d) o[n][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
   const int page_mask = (1 << a.shift) - 1;
-  const int64_t k_page = 2 * a.k_page, v_page = 2 * a.v_page;
-  const uint32_t k_tok = 2 * static_cast<uint32_t>(a.k_tok), v_tok = 2 * static_cast<uint32_t>(a.v_tok);
-  const char* kh = reinterpret_cast<const char*>(a.k + w.head * a.k_head);
-  const char* vh = reinterpret_cast<const char*>(a.v + w.head * a.v_head);
-  const uint32_t k_off = c16 * k_tok + 16 * g4;
+  const int64_t page_bytes = 2 * a.page;
+  const uint32_t tok_bytes = 2 * a.tok;
+  const char* kh = reinterpret_cast<const char*>(a.k + w.head * a.head);
+  const char* vh = reinterpret_cast<const char*>(a.v + w.head * a.head);
+  const uint32_t k_off = c16 * tok_bytes + 16 * g4;
   // row u * PASS + lane / UR of V; its swizzle goes by the row's low bits, so by the parity of u where PASS is 4
-  const uint32_t v_off0 = lane / UR * v_tok + 16 * ((lane % UR) ^ swizzle<D>(lane / UR));
-  const uint32_t v_off1 = lane / UR * v_tok + 16 * ((lane % UR) ^ swizzle<D>(PASS + lane / UR));
+  const uint32_t v_off0 = lane / UR * tok_bytes + 16 * ((lane % UR) ^ swizzle<D>(lane / UR));
+  const uint32_t v_off1 = lane / UR * tok_bytes + 16 * ((lane % UR) ^ swizzle<D>(PASS + lane / UR));
   const auto* table_row = (const __attribute__((address_space(4))) int32_t*)(a.table + w.b * a.table_ld);
   struct Step {
     u32x4_t k[2][KS];
@@ -751,12 +751,12 @@ __device__ __forceinline__ void token_body(const PagedArgs& a, const PagedClass&
     for (int t = 0; t < 2; ++t) {
       const int key = t0 + 16 * t;
       x.id[t] = key < w.kv && static_cast<unsigned>(e.v[t]) < static_cast<unsigned>(a.pages) ? e.v[t] : -1;
-      const uint32_t at = key & page_mask;
-      const char* vp = vh + max(x.id[t], 0) * v_page + static_cast<uint64_t>(at) * v_tok;
+      const int64_t at = max(x.id[t], 0) * page_bytes + (key & page_mask) * tok_bytes;
+      const char* vp = vh + at;
 #pragma unroll
       for (int u = t * NV / 2; u < (t + 1) * NV / 2; ++u)
-        load_lds16(vp + u * PASS % 16 * v_tok + (u % 2 ? v_off1 : v_off0), vt + 8 * 64 * u);
-      const char* kp = kh + max(x.id[t], 0) * k_page + static_cast<uint64_t>(at) * k_tok;
+        load_lds16(vp + u * PASS % 16 * tok_bytes + (u % 2 ? v_off1 : v_off0), vt + 8 * 64 * u);
+      const char* kp = kh + at;
 #pragma unroll
       for (int s = 0; s < KS; ++s) x.k[t][s] = ld_nt4(reinterpret_cast<const uint16_t*>(kp + k_off + 64 * s));
     }
@@ -850,7 +850,7 @@ __device__ __forceinline__ void token_body(const PagedArgs& a, const PagedClass&
       for (int j = 0; j < kStep; ++j) {
         const int key = t0 + j, id = page_id(a, w, key);
         if (id < 0) continue;
-        const uint16_t* p0 = a.v + id * a.v_page + w.head * a.v_head + (key & page_mask) * a.v_tok + 4 * g4;
+        const uint16_t* p0 = a.v + id * a.page + w.head * a.head + (key & page_mask) * a.tok + 4 * g4;
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
           if (!(r[n].on && key >= r[n].lo && key < r[n].hi)) continue;
@@ -1136,15 +1136,14 @@ QKV_EXPORT int64_t qkv_paged_attention_workspace_bytes(int64_t rows, int64_t max
 }
 
 QKV_EXPORT int qkv_paged_attention(const void* query, const int64_t* q_strides, const void* k_pages,
-                                   const int64_t* k_strides, const void* v_pages, const int64_t* v_strides,
-                                   int64_t pages, int64_t page, const int32_t* table, int64_t table_ld, int64_t width,
+                                   const void* v_pages, const int64_t* page_strides, int64_t pages, int64_t page, const int32_t* table, int64_t table_ld, int64_t width,
                                    int64_t requests, const int32_t* cu_rows, const int32_t* kv_lens, int64_t rows,
                                    int64_t max_rows, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                    float scaling, float softcap, const float* slopes, const int32_t* prefix_lens,
                                    const int32_t* first_keys, void* workspace, int64_t workspace_bytes, void* out,
                                    const int64_t* out_strides, int dtype, void* stream) {
   const char* what = "qkv_paged_attention";
-  if (!q_strides || !k_pages || !k_strides || !v_pages || !v_strides || !table || !cu_rows || !kv_lens || !out_strides ||
+  if (!q_strides || !k_pages || !v_pages || !page_strides || !table || !cu_rows || !kv_lens || !out_strides ||
       (rows > 0 && (!query || !out)))
     return fail(QKV_ERR_INVALID, "%s: null pointer", what);
   bool f16;
@@ -1158,10 +1157,9 @@ QKV_EXPORT int qkv_paged_attention(const void* query, const int64_t* q_strides, 
   if (!aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(out, 16) || out_strides[0] % 8 || out_strides[1] % 8)
     return fail(QKV_ERR_INVALID, "%s: pages and output must be 16-byte aligned", what);
   for (int i = 0; i < 3; ++i)
-    if (k_strides[i] % 8 || v_strides[i] % 8)
-      return fail(QKV_ERR_INVALID, "%s: pages and output must be 16-byte aligned", what);
-  if (k_strides[2] < 0 || k_strides[2] >= (1 << 26) || v_strides[2] < 0 || v_strides[2] >= (1 << 26))
-    return fail(QKV_ERR_UNSUPPORTED, "%s: token strides must be below 2^26", what);
+    if (page_strides[i] % 8) return fail(QKV_ERR_INVALID, "%s: pages and output must be 16-byte aligned", what);
+  if (page_strides[2] < 0 || page_strides[2] >= (1 << 30) / page)
+    return fail(QKV_ERR_UNSUPPORTED, "%s: a page's tokens must lie within 2^30 elements", what);
   const int64_t group = q_heads / kv_heads;
   Plan p = plan_of(rows, max_rows, requests, width * page, kv_heads, group);
   if (p.rows.items + p.token.items > (1ll << 30)) return fail(QKV_ERR_UNSUPPORTED, "%s: too many rows", what);
@@ -1176,8 +1174,7 @@ QKV_EXPORT int qkv_paged_attention(const void* query, const int64_t* q_strides, 
   a.v = static_cast<const uint16_t*>(v_pages);
   a.out = static_cast<uint16_t*>(out);
   a.q_row = q_strides[0], a.q_head = q_strides[1];
-  a.k_page = k_strides[0], a.k_head = k_strides[1], a.k_tok = k_strides[2];
-  a.v_page = v_strides[0], a.v_head = v_strides[1], a.v_tok = v_strides[2];
+  a.page = page_strides[0], a.head = page_strides[1], a.tok = static_cast<uint32_t>(page_strides[2]);
   a.o_row = out_strides[0], a.o_head = out_strides[1];
   a.table = table, a.cu = cu_rows, a.kv_lens = kv_lens, a.prefix = prefix_lens, a.first = first_keys;
   a.slopes = slopes;

@@ -230,6 +230,7 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     if (query.dim() != 3 or query.size(2) != dim or query.dtype != k_pages.dtype or query.device != dev
             or query.stride(2) != 1):
         raise RuntimeError(f"query must be {k_pages.dtype} [rows, q_heads, {dim}] on {dev} with contiguous channels")
+    _require(v_pages.stride() == k_pages.stride(), "k_pages and v_pages must have the same strides")
     rows, q_heads = query.size(0), query.size(1)
     n, width = table.shape
     _require(table.device == dev, f"table must be on {dev}")
@@ -255,12 +256,12 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     else:
         _require(workspace.device == dev and workspace.is_contiguous(), f"workspace must be contiguous on {dev}")
     with _lib.on_device(dev):
-        st = _lib.strides(*query.stride()[:2], *k_pages.stride()[:3], *v_pages.stride()[:3], *out.stride()[:2])
+        st = _lib.strides(*query.stride()[:2], *k_pages.stride()[:3], *out.stride()[:2])
         at = ctypes.addressof(st)
         _lib.check(lib.qkv_paged_attention(
-            query.data_ptr(), at, k_pages.data_ptr(), at + 16, v_pages.data_ptr(), at + 40, pages, page,
+            query.data_ptr(), at, k_pages.data_ptr(), v_pages.data_ptr(), at + 16, pages, page,
             table.data_ptr(), table.stride(0), width, n, cu_rows.data_ptr(), kv_lens.data_ptr(), rows, most, q_heads,
             kv_heads, dim, scaling, softcap, _lib.ptr(slopes), _lib.ptr(prefix_lens), _lib.ptr(first_keys),
             _lib.ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
-            out.data_ptr(), at + 64, code, _lib.stream_of(query)))
+            out.data_ptr(), at + 40, code, _lib.stream_of(query)))
     return out

@@ -489,7 +489,8 @@ def test_refusals():
     for change, msg in ((dict(query=q.half()), "query must be"), (dict(query=q[..., ::2]), "query must be"),
                         (dict(query=q.cpu()), "query must be"), (dict(cu_rows=c["cu_rows"].long()), "cu_rows"),
                         (dict(kv_lens=c["cu_rows"]), "kv_lens"), (dict(table=c["table"].long()), "table"),
-                        (dict(v_pages=c["v_pages"][:, :1]), "one shape"), (dict(scaling=0.0), "scaling"),
+                        (dict(v_pages=c["v_pages"][:, :1]), "one shape"),
+                        (dict(v_pages=c["v_pages"].transpose(1, 2).contiguous().transpose(1, 2)), "same strides"), (dict(scaling=0.0), "scaling"),
                         (dict(query=q[:, :3]), "unsupported sizes")):
         with pytest.raises(RuntimeError, match=msg):
             paged.attention(**{**c, **change})

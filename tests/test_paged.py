@@ -27,7 +27,7 @@ def _append(key=P, kp=P, ks=S3, pages=4, page=16, heads=4, dim=64, rows=3, slots
 
 def _attend(q=P, kp=P, ks=S3, pages=4, page=16, ld=8, width=8, requests=2, rows=4, max_rows=4, hq=4, hkv=4, dim=64,
             scaling=1.0, cap=0.0, ws=P, ws_bytes=0, out=P, os=S2, dtype=0):
-    return lib.qkv_paged_attention(q, S2, kp, ks, P, S3, pages, page, P, ld, width, requests, P, P, rows, max_rows,
+    return lib.qkv_paged_attention(q, S2, kp, P, ks, pages, page, P, ld, width, requests, P, P, rows, max_rows,
                                    hq, hkv, dim, scaling, cap, None, None, None, ws, ws_bytes, out, os, dtype, None)
 
 
@@ -59,6 +59,7 @@ NAN, INF = float("nan"), float("inf")
     (lambda: _attend(kp=ctypes.c_void_p(264)), "16-byte aligned"), (lambda: _attend(out=ctypes.c_void_p(260)), "16-byte aligned"),
     (lambda: _attend(os=_lib.strides(256, 60)), "16-byte aligned"),
     (lambda: _attend(ks=_lib.strides(4096, 1020, 64)), "16-byte aligned"),
+    (lambda: _attend(ks=_lib.strides(4096, 1024, (1 << 26) + 8)), "within 2^30"),
     (lambda: _attend(width=100, ld=100), "workspace"),
     (lambda: _attend(width=100, ld=100, ws=ctypes.c_void_p(264), ws_bytes=1 << 40), "workspace"),
 ])
