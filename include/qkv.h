@@ -924,7 +924,7 @@ int qkv_prefill_block_topk(const float* bmax, int64_t rows, int64_t n, int64_t l
  * padded), its tokens last.  kv_lens int32 [requests]: tokens after the
  * step.  slots int64 [rows] = page id * page + t % page and positions int32
  * [rows] = t of each row's token, -1 for rows without one.
- * At most 4096 requests, 2^20 pages and 2^20 rows. */
+ * At most 4096 requests, 2^20 pages, 2^20 rows, 2^30 tokens a table row. */
 int qkv_paged_plan(const int32_t* new_lens, int32_t* table, int64_t table_ld, int32_t* lens, int32_t* free,
                    int32_t* count, int64_t requests, int64_t width, int64_t pages, int64_t page, int64_t rows,
                    int64_t padded, int32_t* cu_rows, int32_t* kv_lens, int64_t* slots, int32_t* positions,
@@ -973,8 +973,9 @@ int64_t qkv_paged_attention_workspace_bytes(int64_t rows, int64_t max_rows, int6
  * not see, do not reach it.  max_rows: a hint, the largest number of rows a
  * request has (up to 16 * kv_heads / q_heads the call takes fewer launches);
  * the result does not depend on it.  head_dim 64 or 128, at most 128 query
- * heads per KV head, scaling > 0.  workspace: 16-byte aligned, contents
- * irrelevant; calls sharing one must not overlap in time. */
+ * heads per KV head; scaling, and softcap where it is not 0, in [2^-60,
+ * 2^60]; a table row covers at most 2^30 tokens.  workspace: 16-byte
+ * aligned, contents irrelevant; calls sharing one must not overlap in time. */
 int qkv_paged_attention(const void* query, const int64_t* q_strides, const void* k_pages, const void* v_pages,
                         const int64_t* page_strides, int64_t pages, int64_t page, const int32_t* table, int64_t table_ld, int64_t width, int64_t requests,
                         const int32_t* cu_rows, const int32_t* kv_lens, int64_t rows, int64_t max_rows,

@@ -253,8 +253,7 @@ int check_table(const char* what, const void* table, int64_t table_ld, const voi
   if (requests > kMaxRequests)
     return fail(QKV_ERR_UNSUPPORTED, "%s: at most %d requests, got %lld", what, kMaxRequests,
                 static_cast<long long>(requests));
-  if (width * page > (1ll << 31) - page)
-    return fail(QKV_ERR_UNSUPPORTED, "%s: a table row covers at most 2^31 - page tokens", what);
+  if (width > (1ll << 30) / page) return fail(QKV_ERR_UNSUPPORTED, "%s: a table row covers at most 2^30 tokens", what);
   return QKV_OK;
 }
 

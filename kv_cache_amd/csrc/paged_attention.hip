@@ -9,8 +9,11 @@
 // Work.  The G query heads of a KV head share its K and V, so a tile holds the G heads of several tokens; a tile's
 // keys are split over several workgroups where there are few tiles.  How far is decided on the GPU from the lengths
 // (locate, below): no length is needed on the host.  Two kernels: `rows` for tiles of 128 (token, head) rows, whose
-// 4 waves hold 32 rows each and share tiles of 64 keys in LDS, bound by the matrix cores; `token` for requests of at
-// most 16 (token, head) rows, whose 4 waves walk different keys of the same rows, bound by memory.
+// 4 waves hold 32 rows each and share tiles of 64 keys in LDS, bound by the matrix cores (2048 tokens behind 63488, 32/8
+// heads: 2.09 ms, 1036 TFLOP/s, 83% of what a large library product reaches); `token` for requests of at most 16 or 32
+// (token, head) rows, whose 4 waves walk different keys of the same rows, bound by memory (32 requests of up to 32768
+// keys: 556 us, 5.85 TB/s).  Requests of 17 to 32 rows in the rows kernel leave three of its waves idle (7 drafts of 5
+// tokens, 4 heads: 70 us, 57 in the token kernel).
 //
 // Both take the scores transposed, S^T = K Q^T, so that a lane holds scores of one row: the softmax is in-lane but
 // for one lane swap, and P^T leaves the score accumulators in the layout that the matrix instruction of O^T = V^T P^T
@@ -55,11 +58,11 @@ struct PagedArgs {
 };
 
 // What one class of requests is worked by: tiles of `tokens` tokens, for requests of more than `above` and at most
-// `most` rows, split along the keys into chunks of at least `min_keys` for about `target` workgroups.
+// `most` rows, split along the keys into chunks of at least `min_keys`.
 struct PagedClass {
   int tokens, above, most, min_keys;
   float per_round;     // 1.0001 / kRound
-  int finer;
+  int finer;           // more than one round of chunks where one does not come out even
   int max_parts;       // parts the workspace holds
   float *acc, *ml;     // them: weighted values, then (maximum, sum)
 };
@@ -149,7 +152,8 @@ __device__ __forceinline__ bool locate(const PagedArgs& a, const PagedClass& c, 
     return s;
   };
   auto round_up = [&](float keys) {
-    const int least = max(c.min_keys, static_cast<int>(fminf(keys, 1.0e9f)) + 1);
+    const int least = max(c.min_keys, static_cast<int>(fminf(keys, 1073741824.0f)) + 1);   // no request has more than 2^30 keys
+ 
     return __builtin_amdgcn_readfirstlane((least + kTile - 1) & -kTile);
   };
   // `per` keys for each of the workgroups that run at once.  One round of them is best where it comes out even (one
@@ -374,9 +378,9 @@ __device__ __forceinline__ void load_lds16(const char* from, uint16_t* to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
                                    (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
-// Every load of the workgroup into LDS has landed, and every wave is done with the tile before.
-// Those of this wave have.
+// The wave's loads have landed.
 __device__ __forceinline__ void wave_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Those of the workgroup have, and every wave is done with the tile before.
 __device__ __forceinline__ void loads_landed() {
   __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
   __syncthreads();
@@ -395,8 +399,10 @@ __device__ __forceinline__ f32x16_t mfma_32x32x16(u32x4_t a, u32x4_t b, f32x16_t
 // ---------------------------------------------------------------------------
 // Tiles of 128 rows.  Wave w holds rows 32w .. 32w+31 as columns of S^T and O^T; a lane holds one row's scores of 16
 // of the 32 keys of a score tile (its other half-wave the others), and one row's outputs.  K and V of 64 keys lie in
-// LDS, double-buffered: the loads of the next tile are issued before this one is computed and stored behind it, one
-// barrier a tile.
+// LDS, double-buffered: the next tile's loads, straight into LDS, are issued before this one is computed and waited
+// for behind it, one barrier a tile.  Two workgroups a CU, so that one's softmax runs beside the other's products:
+// products of the next tile beside this one's softmax within a wave took more registers than there are for two
+// workgroups, and more time (2370 us at 2048 x 65536, 2600 in halves of a tile; 2180 as it was then).
 // ---------------------------------------------------------------------------
 template <int D, bool F16, bool FORM>
 __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& c, int item, uint16_t* stage0,
@@ -422,9 +428,9 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
   int wg_all_lo = 0, wg_lo = 0;
   if (a.first) {
     const int64_t at = w.row0 + w.tile * c.tokens;
-    const int f0 = a.first[at + min(lane, n_tok - 1)], f1 = a.first[at + min(lane + 64, n_tok - 1)];
-    wg_all_lo = max(0, wave_max_i(max(f0, f1)));
-    wg_lo = max(0, -wave_max_i(max(-f0, -f1)));
+    const int f0 = max(0, a.first[at + min(lane, n_tok - 1)]), f1 = max(0, a.first[at + min(lane + 64, n_tok - 1)]);
+    wg_all_lo = wave_max_i(max(f0, f1));
+    wg_lo = -wave_max_i(max(-f0, -f1));
   }
   const int wg_all_hi = hi_of(0), wg_hi = hi_of(n_tok - 1);
   const int tok_a = 32 * wave * a.per_group >> 16, tok_b = (32 * wave + 31) * a.per_group >> 16;
@@ -522,9 +528,9 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
 
   const int k_at = l32 * D, k_sw = swizzle<D>(l32);
   const int v_row = 4 * half + ((lane & 15) >> 2), v_unit = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), v_el = 4 * (lane & 1);
-  auto compute = [&](int t0, bool masked, bool holes, const uint16_t* kb_, const uint16_t* vb_, int buf) __attribute__((always_inline)) {
+  auto compute = [&](int t0, bool masked, bool holes, const uint16_t* kb_, const uint16_t* vb_, int buf)
+                     __attribute__((always_inline)) {
     if (t0 >= any_hi) return;   // no row of the wave sees any of it
-
     f32x16_t s[2];
     {
       u32x4_t kf[2][KS];
@@ -622,7 +628,8 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
   };
 
   // One barrier a tile: the next tile's loads are issued before this one is computed, and have landed behind it.
-  auto turn = [&](int t0, const uint16_t* kb_, uint16_t* vb_, int buf, uint16_t* kn, uint16_t* vn) __attribute__((always_inline)) {
+  auto turn = [&](int t0, const uint16_t* kb_, uint16_t* vb_, int buf, uint16_t* kn, uint16_t* vn)
+                  __attribute__((always_inline)) {
     const bool holes = hole, masked = t0 < wg_all_lo || t0 + kTile > wg_all_hi || holes;
     const Pages next = pages_of(t0 + kTile);
     if (masked) clean_tile(t0, holes, vb_, buf);
@@ -953,7 +960,8 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedArgs a, PagedC
 }
 // Requests of both classes in one launch, the long ones first.
 template <int D, bool F16, bool FORM>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_rows_kernel(PagedArgs a, PagedClass rows, PagedClass token, int n_rows) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_rows_kernel(PagedArgs a, PagedClass rows, PagedClass token,
+                                                                          int n_rows) {
   __shared__ __attribute__((aligned(16))) uint16_t stage0[2 * kTile * D], stage1[2 * kTile * D];
   if (static_cast<int>(blockIdx.x) < n_rows) rows_body<D, F16, FORM>(a, rows, blockIdx.x, stage0, stage1);
   else token_body<D, F16, FORM, 2>(a, token, blockIdx.x - n_rows, stage0, stage1);
@@ -1079,6 +1087,7 @@ struct Plan {
 Plan plan_of(int64_t rows, int64_t max_rows, int64_t requests, int64_t max_keys, int64_t kv_heads, int64_t group) {
   constexpr int64_t kAny = 0x7FFFFFFF;
   Plan p{};
+  max_rows = std::max<int64_t>(max_rows, 1);
   p.sets = max_rows * group <= kTokenM ? 1 : 2;
   const int64_t m = p.sets * kTokenM;
   if (max_rows * group <= m) {   // a longer request, if there is one after all, takes several tiles
@@ -1095,7 +1104,7 @@ int64_t part_floats(int64_t m, int64_t head_dim) { return m * (head_dim + 2); }
 bool good_sizes(int64_t rows, int64_t requests, int64_t width, int64_t page, int64_t q_heads, int64_t kv_heads,
                 int64_t head_dim) {
   return rows >= 0 && rows <= (1 << 30) && requests >= 1 && requests <= (1 << 20) && width >= 1 && page >= 16 &&
-         page <= 4096 && !(page & (page - 1)) && width <= ((1ll << 31) - page) / page && kv_heads >= 1 &&
+         page <= 4096 && !(page & (page - 1)) && width <= (1ll << 30) / page && kv_heads >= 1 &&
          q_heads >= kv_heads && q_heads % kv_heads == 0 && q_heads <= 65536 && q_heads / kv_heads <= kRowsM &&
          (head_dim == 64 || head_dim == 128);
 }
@@ -1152,8 +1161,10 @@ QKV_EXPORT int qkv_paged_attention(const void* query, const int64_t* q_strides, 
       pages > (1ll << 30) || max_rows < 0)
     return fail(QKV_ERR_UNSUPPORTED, "%s: unsupported sizes (head_dim 64 or 128, page a power of two in [16, 4096], "
                 "q_heads a multiple of kv_heads and at most %d times as many)", what, kRowsM);
-  if (!(scaling > 0.0f) || !(scaling < __builtin_huge_valf()) || !(softcap >= 0.0f) || !(softcap < __builtin_huge_valf()))
-    return fail(QKV_ERR_INVALID, "%s: scaling must be positive and softcap 0 or positive", what);
+  // so that scaling / softcap, and slopes / scaling, stay finite
+  const auto usable = [](float x) { return x >= 0x1p-60f && x <= 0x1p60f; };
+  if (!usable(scaling) || !(softcap == 0.0f || usable(softcap)))
+    return fail(QKV_ERR_INVALID, "%s: scaling must be in [2^-60, 2^60] and softcap 0 or there", what);
   if (!aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(out, 16) || out_strides[0] % 8 || out_strides[1] % 8)
     return fail(QKV_ERR_INVALID, "%s: pages and output must be 16-byte aligned", what);
   for (int i = 0; i < 3; ++i)

@@ -386,6 +386,24 @@ def test_rows_that_see_nothing():
     assert (got == 0).all()
 
 
+def test_first_keys_of_any_value():
+    # below zero (the least of all included) is zero, past the row is nothing
+    for rows in ([50, 3], [2, 1]):
+        c = _case([120, 90], rows, 8, 2, 128, 16, "bf16", seed=25)
+        n = sum(rows)
+        first = torch.full((n,), 40, dtype=torch.int32)
+        first[0], first[1], first[n - 1] = -2 ** 31, 2 ** 31 - 1, -7
+        _check(c, first_keys=first.to(DEV))
+
+
+def test_wrong_hints():
+    # the hint says less than there is, at group sizes that do not fit the smaller kernels' tiles
+    for hq, hkv in ((40, 2), (34, 1), (2, 2)):
+        c = _case([300, 70, 9], [1, 35, 4], hq, hkv, 64, 16, "bf16", seed=26)
+        for hint in (0, 1, 2, 1000):
+            _check(c, max_rows=hint)
+
+
 def test_left_padding_and_requests_without_tokens():
     # more rows than tokens: the first rows are padding and get zeros; a request not served has kv_lens 0
     for rows in ([40, 40, 40], [3, 3, 3]):

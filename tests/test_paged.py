@@ -41,7 +41,7 @@ NAN, INF = float("nan"), float("inf")
     (lambda: _plan(page=24), "power of two"), (lambda: _plan(page=8), "power of two"),
     (lambda: _plan(page=8192), "power of two"), (lambda: _plan(requests=4097), "at most 4096 requests"),
     (lambda: _plan(pages=(1 << 20) + 1), "at most 1048576 pages"), (lambda: _plan(rows=(1 << 20) + 1), "at most 1048576 rows"),
-    (lambda: _plan(width=1 << 27, ld=1 << 27), "2^31"),
+    (lambda: _plan(width=(1 << 26) + 1, ld=1 << 27), "2^30"),
     (lambda: _release(keep=None), "null pointer"), (lambda: _release(width=9), "bad sizes"),
     (lambda: _release(page=17), "power of two"),
     (lambda: _append(key=None), "null pointer"), (lambda: _append(slots=None), "null pointer"),
@@ -53,9 +53,11 @@ NAN, INF = float("nan"), float("inf")
     (lambda: _attend(dim=96), "unsupported sizes"), (lambda: _attend(page=20), "unsupported sizes"),
     (lambda: _attend(hq=6), "unsupported sizes"), (lambda: _attend(hq=129, hkv=1), "unsupported sizes"),
     (lambda: _attend(ld=7), "unsupported sizes"), (lambda: _attend(rows=-1), "unsupported sizes"),
-    (lambda: _attend(scaling=0.0), "scaling must be positive"), (lambda: _attend(scaling=-1.0), "scaling must be positive"),
-    (lambda: _attend(scaling=NAN), "scaling must be positive"), (lambda: _attend(scaling=INF), "scaling must be positive"),
+    (lambda: _attend(scaling=0.0), "scaling must be in"), (lambda: _attend(scaling=-1.0), "scaling must be in"),
+    (lambda: _attend(scaling=NAN), "scaling must be in"), (lambda: _attend(scaling=INF), "scaling must be in"),
     (lambda: _attend(cap=-1.0), "softcap"), (lambda: _attend(cap=NAN), "softcap"), (lambda: _attend(cap=INF), "softcap"),
+    (lambda: _attend(scaling=1e-30), "scaling must be in"), (lambda: _attend(cap=1e-30), "softcap"),
+    (lambda: _attend(width=(1 << 26) + 1, ld=1 << 27), "unsupported sizes"),
     (lambda: _attend(kp=ctypes.c_void_p(264)), "16-byte aligned"), (lambda: _attend(out=ctypes.c_void_p(260)), "16-byte aligned"),
     (lambda: _attend(os=_lib.strides(256, 60)), "16-byte aligned"),
     (lambda: _attend(ks=_lib.strides(4096, 1020, 64)), "16-byte aligned"),
