@@ -30,7 +30,7 @@ constexpr int kTile = 64;      // keys per step of the rows kernel; splits are m
 constexpr int kRowsM = 128;    // rows of a tile of the rows kernel
 constexpr int kTokenM = 16;    // rows of a column set of the token kernel, which has one or two
 constexpr int kRound = 512;    // workgroups that run at once: two a CU
-constexpr int kRowsJoins = 4, kTokenJoins = 8;   // workgroups that join the parts of such a tile
+constexpr int kRowsJoins = 8, kTokenJoins = 4;   // workgroups that join a tile's parts; of a column set's
 constexpr int kStep = 32;      // keys a wave of the token kernel takes at a time
 // fp16 weights are scaled by 2^6: they stay below 2^14 (lazy rescaling lets them reach 2^8) and normal down to 2^-20
 // of the row's largest, so that the small weights of long rows keep their bits.
@@ -1040,7 +1040,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, PagedClass
   if (static_cast<int>(blockIdx.x) < n_rows) {
     for (int i = blockIdx.x; join_body<D, F16, kRowsM, 8, kRowsJoins>(a, rows, i); i += n_rows) __syncthreads();
   } else {
-    for (int i = blockIdx.x - n_rows; join_body<D, F16, NQ * kTokenM, 1, kTokenJoins>(a, token, i); i += gridDim.x - n_rows)
+    for (int i = blockIdx.x - n_rows; join_body<D, F16, NQ * kTokenM, 1, NQ * kTokenJoins>(a, token, i); i += gridDim.x - n_rows)
       __syncthreads();
   }
 }
@@ -1121,7 +1121,7 @@ int launch(const PagedArgs& a, const Plan& p, hipStream_t st) {
     paged_token_kernel<D, F16, FORM, 2><<<n(p.token.items), 256, 0, st>>>(a, p.token.cls);
   }
   const int64_t joins = std::min<int64_t>(p.rows.tiles * kRowsJoins, 2 * kRound);
-  const int64_t all = joins + std::min<int64_t>(p.token.tiles * kTokenJoins, 2 * kRound);
+  const int64_t all = joins + std::min<int64_t>(p.token.tiles * p.sets * kTokenJoins, 2 * kRound);
   if (all) {
     if (p.sets == 1)
       paged_join_kernel<D, F16, 1><<<n(all), 256, 0, st>>>(a, p.rows.cls, p.token.cls, static_cast<int>(joins));
