@@ -12,7 +12,7 @@
 // 4 waves hold 32 rows each and share tiles of 64 keys in LDS, bound by the matrix cores (2048 tokens behind 63488, 32/8
 // heads: 2.09 ms, 1036 TFLOP/s, 83% of what a large library product reaches); `token` for requests of at most 16 or 32
 // (token, head) rows, whose 4 waves walk different keys of the same rows, bound by memory (32 requests of up to 32768
-// keys: 556 us, 5.85 TB/s).  Requests of 17 to 32 rows in the rows kernel leave three of its waves idle (7 drafts of 5
+// keys: 530 us, 6.14 TB/s).  Requests of 17 to 32 rows in the rows kernel leave three of its waves idle (7 drafts of 5
 // tokens, 4 heads: 70 us, 57 in the token kernel).
 //
 // Both take the scores transposed, S^T = K Q^T, so that a lane holds scores of one row: the softmax is in-lane but
@@ -373,10 +373,12 @@ __device__ __forceinline__ u32x2_t read_tr(const uint16_t* p) {
   return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)p));
 }
 
-// 16 bytes a lane from memory to LDS, at `to` (wave-uniform) + 16 bytes * lane, without registers.
+// 16 bytes a lane from memory to LDS, at `to` (wave-uniform) + 16 bytes * lane, without registers; ONCE: with the
+// non-temporal hint, for what no other workgroup reads.
+template <bool ONCE = false>
 __device__ __forceinline__ void load_lds16(const char* from, uint16_t* to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+                                   (__attribute__((address_space(3))) void*)to, 16, 0, ONCE ? 2 : 0);
 }
 // The wave's loads have landed.
 __device__ __forceinline__ void wave_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
@@ -686,7 +688,9 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
 // ---------------------------------------------------------------------------
 // Tiles of at most 16 NQ rows: NQ sets of 16 columns of 16-wide score tiles.  Wave w takes steps w, w + 4, ... of 32
 // keys of the workgroup's chunk; K goes from memory to the matrix instruction's registers, V through the wave's own
-// part of LDS (as it lies, read transposed), no barrier until the waves are joined at the end.
+// part of LDS (as it lies, read transposed), no barrier until the waves are joined at the end.  V is loaded with the
+// non-temporal hint, whole rows at a time; K without, since two loads share each of its 128-byte lines (32 requests of up
+// to 32768 keys: 530 us, 6.14 TB/s; both with the hint 548, neither 582, K alone 556).
 // ---------------------------------------------------------------------------
 template <int D, bool F16, bool FORM, int NQ>
 __device__ __forceinline__ void token_body(const PagedArgs& a, const PagedClass& c, int item, uint16_t* stage0,
@@ -762,10 +766,10 @@ __device__ __forceinline__ void token_body(const PagedArgs& a, const PagedClass&
       const char* vp = vh + at;
 #pragma unroll
       for (int u = t * NV / 2; u < (t + 1) * NV / 2; ++u)
-        load_lds16(vp + u * PASS % 16 * tok_bytes + (u % 2 ? v_off1 : v_off0), vt + 8 * 64 * u);
+        load_lds16<true>(vp + u * PASS % 16 * tok_bytes + (u % 2 ? v_off1 : v_off0), vt + 8 * 64 * u);
       const char* kp = kh + at;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) x.k[t][s] = ld_nt4(reinterpret_cast<const uint16_t*>(kp + k_off + 64 * s));
+      for (int s = 0; s < KS; ++s) x.k[t][s] = *reinterpret_cast<const u32x4_t*>(kp + k_off + 64 * s);
     }
   };
   auto compute = [&](int t0, Step& x, uint16_t* vt) __attribute__((always_inline)) {
