@@ -58,20 +58,30 @@ class StepPlan(NamedTuple):
 
     @classmethod
     def empty(cls, requests: int, rows: int, device) -> "StepPlan":
-        """Buffers for a step of ``rows`` rows (allocated as one)."""
-        words = torch.empty(2 * rows + rows + 2 * requests + 2, dtype=torch.int32, device=device)
-        slots, positions, cu, kv, failed = words.split_with_sizes([2 * rows, rows, requests + 1, requests, 1])
-        return cls(cu, kv, slots.view(torch.int64), positions, failed)
+        """Buffers for a step of ``rows`` rows."""
+        kv = torch.empty(requests, dtype=torch.int32, device=device)
+        return cls(kv.new_empty(requests + 1), kv, kv.new_empty(rows, dtype=torch.int64), kv.new_empty(rows),
+                   kv.new_empty(1))
 
 
-def _i32(name: str, t: torch.Tensor, n: int, device) -> None:
-    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous() or t.device != device:
-        raise RuntimeError(f"{name} must be contiguous int32 [{n}] on {device}")
+# The checks below run several times a call of ten microseconds: they ask tensors the cheapest way there is
+# (get_device() for the device, numel() and dim() for a shape of one axis).
 
 
-def _check_table(table: torch.Tensor) -> None:
-    if not table.is_cuda or table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1:
+def _i32(name: str, t: torch.Tensor, n: int, idx: int) -> None:
+    if (t.dtype is not torch.int32 or t.numel() != n or t.dim() != 1 or not t.is_contiguous()
+            or t.get_device() != idx):
+        raise RuntimeError(f"{name} must be contiguous int32 [{n}] on cuda:{idx}")
+
+
+def _check_table(table: torch.Tensor) -> tuple[int, int, int, int]:
+    """(device index, requests, width, row stride) of a page table."""
+    if not table.is_cuda or table.dtype is not torch.int32 or table.dim() != 2:
         raise RuntimeError("table must be CUDA int32 [requests, width] with contiguous rows")
+    ld, one = table.stride()
+    if one != 1:
+        raise RuntimeError("table must be CUDA int32 [requests, width] with contiguous rows")
+    return (table.get_device(), *table.shape, ld)
 
 
 def plan_step(new_lens: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, free: torch.Tensor,
@@ -88,25 +98,29 @@ def plan_step(new_lens: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, f
     is, with kv_lens 0, and counted in ``failed``.  At most 4096 requests,
     2^20 pages, 2^20 rows; ``page`` a power of two in [16, 4096]."""
     lib = _lib.load()
-    _check_table(table)
-    n, dev = table.size(0), table.device
-    _i32("new_lens", new_lens, n, dev)
-    _i32("lens", lens, n, dev)
-    _i32("free", free, free.numel(), dev)
-    _i32("count", count, 1, dev)
+    idx, n, width, ld = _check_table(table)
+    pages = free.numel()
+    _i32("new_lens", new_lens, n, idx)
+    _i32("lens", lens, n, idx)
+    _i32("free", free, pages, idx)
+    _i32("count", count, 1, idx)
     if out is None:
-        out = StepPlan.empty(n, rows, dev)
+        out = StepPlan.empty(n, rows, table.device)
     else:
-        _i32("out.cu_rows", out.cu_rows, n + 1, dev)
-        _i32("out.kv_lens", out.kv_lens, n, dev)
-        _i32("out.positions", out.positions, rows, dev)
-        _i32("out.failed", out.failed, 1, dev)
-        _check_slots(out.slots, rows, dev)
-    with _lib.on_device(dev):
-        _lib.check(lib.qkv_paged_plan(new_lens.data_ptr(), table.data_ptr(), table.stride(0), lens.data_ptr(),
-                                      free.data_ptr(), count.data_ptr(), n, table.size(1), free.size(0), page, rows,
-                                      padded, out.cu_rows.data_ptr(), out.kv_lens.data_ptr(), out.slots.data_ptr(),
-                                      out.positions.data_ptr(), out.failed.data_ptr(), _lib.stream_of(table)))
+        _i32("out.cu_rows", out.cu_rows, n + 1, idx)
+        _i32("out.kv_lens", out.kv_lens, n, idx)
+        _i32("out.positions", out.positions, rows, idx)
+        _i32("out.failed", out.failed, 1, idx)
+        _check_slots(out.slots, rows, idx)
+    cu, kv, slots, positions, failed = out
+    guard = _lib.enter_device(idx)
+    try:
+        rc = lib.qkv_paged_plan(new_lens.data_ptr(), table.data_ptr(), ld, lens.data_ptr(), free.data_ptr(),
+                                count.data_ptr(), n, width, pages, page, rows, padded, cu.data_ptr(), kv.data_ptr(),
+                                slots.data_ptr(), positions.data_ptr(), failed.data_ptr(), _lib.stream_on(idx))
+    finally:
+        _lib.leave_device(guard)
+    _lib.check(rc)
     return out
 
 
@@ -116,16 +130,19 @@ def release_pages(keep: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, f
     length or more leaves it) and gives the pages behind them back to
     ``free``; the last step's tokens released leave the stack as it was."""
     lib = _lib.load()
-    _check_table(table)
-    n, dev = table.size(0), table.device
-    _i32("keep", keep, n, dev)
-    _i32("lens", lens, n, dev)
-    _i32("free", free, free.numel(), dev)
-    _i32("count", count, 1, dev)
-    with _lib.on_device(dev):
-        _lib.check(lib.qkv_paged_release(keep.data_ptr(), table.data_ptr(), table.stride(0), lens.data_ptr(),
-                                         free.data_ptr(), count.data_ptr(), n, table.size(1), free.size(0), page,
-                                         _lib.stream_of(table)))
+    idx, n, width, ld = _check_table(table)
+    pages = free.numel()
+    _i32("keep", keep, n, idx)
+    _i32("lens", lens, n, idx)
+    _i32("free", free, pages, idx)
+    _i32("count", count, 1, idx)
+    guard = _lib.enter_device(idx)
+    try:
+        rc = lib.qkv_paged_release(keep.data_ptr(), table.data_ptr(), ld, lens.data_ptr(), free.data_ptr(),
+                                   count.data_ptr(), n, width, pages, page, _lib.stream_on(idx))
+    finally:
+        _lib.leave_device(guard)
+    _lib.check(rc)
 
 
 class PageTable:
@@ -153,19 +170,21 @@ class PageTable:
         release_pages(keep, self.table, self.lens, self.free, self.count, self.page)
 
 
-def _check_slots(slots: torch.Tensor, rows: int, device) -> None:
-    if slots.dtype is not torch.int64 or slots.shape != (rows,) or not slots.is_contiguous() or slots.device != device:
-        raise RuntimeError(f"slots must be contiguous int64 [{rows}] on {device}")
+def _check_slots(slots: torch.Tensor, rows: int, idx: int) -> None:
+    if (slots.dtype is not torch.int64 or slots.numel() != rows or slots.dim() != 1 or not slots.is_contiguous()
+            or slots.get_device() != idx):
+        raise RuntimeError(f"slots must be contiguous int64 [{rows}] on cuda:{idx}")
 
 
-def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor) -> int:
-    """Checks a layer's pages; returns their dtype code."""
+def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, tuple, tuple]:
+    """(dtype code, strides of k_pages, of v_pages) of a layer's pages, checked."""
     code = _lib.half_code("k_pages", k_pages)
-    if (not k_pages.is_cuda or k_pages.dim() != 4 or k_pages.shape != v_pages.shape or v_pages.dtype != k_pages.dtype
-            or v_pages.device != k_pages.device or k_pages.stride(3) != 1 or v_pages.stride(3) != 1):
+    if (not k_pages.is_cuda or k_pages.dim() != 4 or k_pages.shape != v_pages.shape
+            or v_pages.dtype is not k_pages.dtype or v_pages.get_device() != k_pages.get_device()
+            or k_pages.stride(3) != 1 or v_pages.stride(3) != 1):
         raise RuntimeError("k_pages and v_pages must be CUDA [pages, kv_heads, page, dim] of one shape, dtype and "
                            "device with contiguous channels")
-    return code
+    return code, k_pages.stride(), v_pages.stride()
 
 
 def append(key: torch.Tensor, value: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -174,22 +193,27 @@ def append(key: torch.Tensor, value: torch.Tensor, k_pages: torch.Tensor, v_page
     channels, to their ``slots`` (int64 [rows], as ``plan_step`` gives them;
     a row with -1 is skipped, no slot may come twice)."""
     lib = _lib.load()
-    _check_pages(k_pages, v_pages)
+    _, ks, vs = _check_pages(k_pages, v_pages)
     pages, heads, page, dim = k_pages.shape
+    idx = k_pages.get_device()
+    rows = slots.numel()
+    _check_slots(slots, rows, idx)
     for name, t in (("key", key), ("value", value)):
-        if (t.dim() != 3 or t.size(1) != heads or t.size(2) != dim or t.dtype != k_pages.dtype
-                or t.device != k_pages.device or t.stride(2) != 1):
-            raise RuntimeError(f"{name} must be {k_pages.dtype} [rows, {heads}, {dim}] on {k_pages.device} with "
-                               "contiguous channels")
-    rows = key.size(0)
-    _require(value.size(0) == rows, "key and value must have as many rows")
-    _check_slots(slots, rows, key.device)
-    with _lib.on_device(key.device):
-        st = _lib.strides(*key.stride()[:2], *value.stride()[:2], *k_pages.stride()[:3], *v_pages.stride()[:3])
-        at = ctypes.addressof(st)
-        _lib.check(lib.qkv_paged_append(key.data_ptr(), at, value.data_ptr(), at + 16, k_pages.data_ptr(), at + 32,
-                                        v_pages.data_ptr(), at + 56, pages, page, heads, dim, slots.data_ptr(), rows,
-                                        _lib.stream_of(key)))
+        if (t.shape != (rows, heads, dim) or t.dtype is not k_pages.dtype or t.get_device() != idx
+                or t.stride(2) != 1):
+            raise RuntimeError(f"{name} must be {k_pages.dtype} [{rows}, {heads}, {dim}] on {k_pages.device} with "
+                               "contiguous channels: key, value and slots have as many rows")
+    # row and head strides of the rows, page, head and token strides of the pages, in one array
+    st = _lib.strides(*key.stride()[:2], *value.stride()[:2], *ks[:3], *vs[:3])
+    at = ctypes.addressof(st)
+    guard = _lib.enter_device(idx)
+    try:
+        rc = lib.qkv_paged_append(key.data_ptr(), at, value.data_ptr(), at + 16, k_pages.data_ptr(), at + 32,
+                                  v_pages.data_ptr(), at + 56, pages, page, heads, dim, slots.data_ptr(), rows,
+                                  _lib.stream_on(idx))
+    finally:
+        _lib.leave_device(guard)
+    _lib.check(rc)
 
 
 def attention_workspace(rows: int, max_rows: int, requests: int, width: int, page: int, q_heads: int, kv_heads: int,
@@ -223,45 +247,55 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     [rows, Hq, D] in the query's dtype; rows of ``out`` behind the last
     request are left as they were."""
     lib = _lib.load()
-    code = _check_pages(k_pages, v_pages)
-    _check_table(table)
+    code, ks, vs = _check_pages(k_pages, v_pages)
+    idx, n, width, ld = _check_table(table)
     pages, kv_heads, page, dim = k_pages.shape
-    dev = k_pages.device
-    if (query.dim() != 3 or query.size(2) != dim or query.dtype != k_pages.dtype or query.device != dev
-            or query.stride(2) != 1):
-        raise RuntimeError(f"query must be {k_pages.dtype} [rows, q_heads, {dim}] on {dev} with contiguous channels")
-    _require(v_pages.stride() == k_pages.stride(), "k_pages and v_pages must have the same strides")
-    rows, q_heads = query.size(0), query.size(1)
-    n, width = table.shape
-    _require(table.device == dev, f"table must be on {dev}")
-    _i32("cu_rows", cu_rows, n + 1, dev)
-    _i32("kv_lens", kv_lens, n, dev)
+    if k_pages.get_device() != idx:
+        raise RuntimeError(f"table must be on {k_pages.device}")
+    if vs != ks:
+        raise RuntimeError("k_pages and v_pages must have the same strides")
+    if (query.dim() != 3 or query.dtype is not k_pages.dtype or query.get_device() != idx or query.stride(2) != 1
+            or query.size(2) != dim):
+        raise RuntimeError(f"query must be {k_pages.dtype} [rows, q_heads, {dim}] on {k_pages.device} with contiguous "
+                           "channels")
+    rows, q_heads, _ = query.shape
+    _i32("cu_rows", cu_rows, n + 1, idx)
+    _i32("kv_lens", kv_lens, n, idx)
     if prefix_lens is not None:
-        _i32("prefix_lens", prefix_lens, n, dev)
+        _i32("prefix_lens", prefix_lens, n, idx)
     if first_keys is not None:
-        _i32("first_keys", first_keys, rows, dev)
+        _i32("first_keys", first_keys, rows, idx)
     if slopes is not None:
-        _require(slopes.dtype == torch.float32 and slopes.device == dev and slopes.shape == (q_heads,)
-                 and slopes.is_contiguous(), f"slopes must be contiguous float32 [{q_heads}] on {dev}")
+        _require(slopes.dtype is torch.float32 and slopes.get_device() == idx and slopes.shape == (q_heads,)
+                 and slopes.is_contiguous(), f"slopes must be contiguous float32 [{q_heads}] on cuda:{idx}")
     if out is None:
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
     else:
-        _require(out.shape == query.shape and out.dtype == query.dtype and out.device == dev and out.stride(2) == 1,
-                 "out must have the query's shape, dtype and device with contiguous channels")
+        _require(out.shape == query.shape and out.dtype is query.dtype and out.get_device() == idx
+                 and out.stride(2) == 1, "out must have the query's shape, dtype and device with contiguous channels")
     most = rows if max_rows is None else max_rows
-    need = lib.qkv_paged_attention_workspace_bytes(rows, most, n, width, page, q_heads, kv_heads, dim)
+    ws_ptr, ws_bytes = None, 0
     if workspace is None:
-        if need > 0:
-            workspace = torch.empty(need // 4, dtype=torch.float32, device=dev)
+        ws_bytes = lib.qkv_paged_attention_workspace_bytes(rows, most, n, width, page, q_heads, kv_heads, dim)
+        if ws_bytes > 0:
+            workspace = torch.empty(ws_bytes // 4, dtype=torch.float32, device=query.device)
+            ws_ptr = workspace.data_ptr()
     else:
-        _require(workspace.device == dev and workspace.is_contiguous(), f"workspace must be contiguous on {dev}")
-    with _lib.on_device(dev):
-        st = _lib.strides(*query.stride()[:2], *k_pages.stride()[:3], *out.stride()[:2])
-        at = ctypes.addressof(st)
-        _lib.check(lib.qkv_paged_attention(
-            query.data_ptr(), at, k_pages.data_ptr(), v_pages.data_ptr(), at + 16, pages, page,
-            table.data_ptr(), table.stride(0), width, n, cu_rows.data_ptr(), kv_lens.data_ptr(), rows, most, q_heads,
-            kv_heads, dim, scaling, softcap, _lib.ptr(slopes), _lib.ptr(prefix_lens), _lib.ptr(first_keys),
-            _lib.ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
-            out.data_ptr(), at + 40, code, _lib.stream_of(query)))
+        _require(workspace.get_device() == idx and workspace.is_contiguous(),
+                 f"workspace must be contiguous on cuda:{idx}")
+        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    # row and head strides of the query, page, head and token strides of the pages, row and head strides of out
+    st = _lib.strides(*query.stride()[:2], *ks[:3], *out.stride()[:2])
+    at = ctypes.addressof(st)
+    guard = _lib.enter_device(idx)
+    try:
+        rc = lib.qkv_paged_attention(
+            query.data_ptr(), at, k_pages.data_ptr(), v_pages.data_ptr(), at + 16, pages, page, table.data_ptr(), ld,
+            width, n, cu_rows.data_ptr(), kv_lens.data_ptr(), rows, most, q_heads, kv_heads, dim, scaling, softcap,
+            None if slopes is None else slopes.data_ptr(), None if prefix_lens is None else prefix_lens.data_ptr(),
+            None if first_keys is None else first_keys.data_ptr(), ws_ptr, ws_bytes, out.data_ptr(), at + 40, code,
+            _lib.stream_on(idx))
+    finally:
+        _lib.leave_device(guard)
+    _lib.check(rc)
     return out
