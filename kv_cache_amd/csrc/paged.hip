@@ -324,7 +324,8 @@ QKV_EXPORT int qkv_paged_append(const void* key, const int64_t* key_strides, con
                slots, rows * units_row, pages * page, static_cast<int>(units_head), static_cast<int>(units_row),
                __builtin_ctz(static_cast<unsigned>(page))};
   const int64_t grid = cdiv(a.units, 256);
-  if (grid > (1ll << 31) - 1) return fail(QKV_ERR_UNSUPPORTED, "%s: too many rows", what);
+  // a grid has less than 2^32 threads
+  if (grid >= (1 << 24)) return fail(QKV_ERR_UNSUPPORTED, "%s: too many rows", what);
   append_kernel<<<static_cast<unsigned>(grid), 256, 0, static_cast<hipStream_t>(stream)>>>(a);
   return check_launch(what);
 }

@@ -64,6 +64,7 @@ struct PagedClass {
   float per_round;     // 1.0001 / kRound
   int finer;           // more than one round of chunks where one does not come out even
   int max_parts;       // parts the workspace holds
+  int max_joins;       // items of the kernel that joins them
   float *acc, *ml;     // them: weighted values, then (maximum, sum)
 };
 
@@ -380,8 +381,8 @@ __device__ __forceinline__ void load_lds16(const char* from, uint16_t* to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
                                    (__attribute__((address_space(3))) void*)to, 16, 0, ONCE ? 2 : 0);
 }
-// The wave's loads have landed.
-__device__ __forceinline__ void wave_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// The wave's loads have landed, and its reads of the step before have left LDS.
+__device__ __forceinline__ void wave_landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 // Those of the workgroup have, and every wave is done with the tile before.
 __device__ __forceinline__ void loads_landed() {
   __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
@@ -1042,9 +1043,12 @@ template <int D, bool F16, int NQ>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, PagedClass rows, PagedClass token, int n_rows) {
   // few workgroups for the many items there may be: a workgroup without work costs a microsecond, in rounds
   if (static_cast<int>(blockIdx.x) < n_rows) {
-    for (int i = blockIdx.x; join_body<D, F16, kRowsM, 8, kRowsJoins>(a, rows, i); i += n_rows) __syncthreads();
+    for (int i = blockIdx.x; i < rows.max_joins && join_body<D, F16, kRowsM, 8, kRowsJoins>(a, rows, i); i += n_rows)
+      __syncthreads();
   } else {
-    for (int i = blockIdx.x - n_rows; join_body<D, F16, NQ * kTokenM, 1, NQ * kTokenJoins>(a, token, i); i += gridDim.x - n_rows)
+    constexpr int G = NQ * kTokenJoins;
+    for (int i = blockIdx.x - n_rows; i < token.max_joins && join_body<D, F16, NQ * kTokenM, 1, G>(a, token, i);
+         i += gridDim.x - n_rows)
       __syncthreads();
   }
 }
@@ -1052,7 +1056,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, PagedClass
 // The launches of a call, from what the host knows: rows, requests, and the tokens a table row covers.
 struct Shape {
   PagedClass cls;
-  int64_t items, parts, tiles;   // workgroups; parts in the workspace; split tiles
+  int64_t items, parts;   // workgroups; parts in the workspace
 };
 
 // Tiles of m rows for requests of more than `above` and at most `most` rows.
@@ -1076,7 +1080,7 @@ Shape shape_of(bool token, int64_t m, int64_t above, int64_t most, int64_t rows,
     // ceil(keys / C) is at most 2 keys / C
     s.items = std::min(tiles + target, tiles * cdiv(max_keys, s.cls.min_keys));
     s.parts = std::min<int64_t>(2 * target, s.items);
-    s.tiles = std::min<int64_t>(target, tiles);
+    s.cls.max_joins = static_cast<int>(std::min<int64_t>(target, tiles) * (token ? m / kTokenM * kTokenJoins : kRowsJoins));
   }
   s.cls.max_parts = static_cast<int>(s.parts);
   return s;
@@ -1124,8 +1128,8 @@ int launch(const PagedArgs& a, const Plan& p, hipStream_t st) {
   } else {
     paged_token_kernel<D, F16, FORM, 2><<<n(p.token.items), 256, 0, st>>>(a, p.token.cls);
   }
-  const int64_t joins = std::min<int64_t>(p.rows.tiles * kRowsJoins, 2 * kRound);
-  const int64_t all = joins + std::min<int64_t>(p.token.tiles * p.sets * kTokenJoins, 2 * kRound);
+  const int64_t joins = std::min(p.rows.cls.max_joins, 2 * kRound);
+  const int64_t all = joins + std::min(p.token.cls.max_joins, 2 * kRound);
   if (all) {
     if (p.sets == 1)
       paged_join_kernel<D, F16, 1><<<n(all), 256, 0, st>>>(a, p.rows.cls, p.token.cls, static_cast<int>(joins));
@@ -1149,12 +1153,13 @@ QKV_EXPORT int64_t qkv_paged_attention_workspace_bytes(int64_t rows, int64_t max
 }
 
 QKV_EXPORT int qkv_paged_attention(const void* query, const int64_t* q_strides, const void* k_pages,
-                                   const void* v_pages, const int64_t* page_strides, int64_t pages, int64_t page, const int32_t* table, int64_t table_ld, int64_t width,
-                                   int64_t requests, const int32_t* cu_rows, const int32_t* kv_lens, int64_t rows,
-                                   int64_t max_rows, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
-                                   float scaling, float softcap, const float* slopes, const int32_t* prefix_lens,
-                                   const int32_t* first_keys, void* workspace, int64_t workspace_bytes, void* out,
-                                   const int64_t* out_strides, int dtype, void* stream) {
+                                   const void* v_pages, const int64_t* page_strides, int64_t pages, int64_t page,
+                                   const int32_t* table, int64_t table_ld, int64_t width, int64_t requests,
+                                   const int32_t* cu_rows, const int32_t* kv_lens, int64_t rows, int64_t max_rows,
+                                   int64_t q_heads, int64_t kv_heads, int64_t head_dim, float scaling, float softcap,
+                                   const float* slopes, const int32_t* prefix_lens, const int32_t* first_keys,
+                                   void* workspace, int64_t workspace_bytes, void* out, const int64_t* out_strides,
+                                   int dtype, void* stream) {
   const char* what = "qkv_paged_attention";
   if (!q_strides || !k_pages || !v_pages || !page_strides || !table || !cu_rows || !kv_lens || !out_strides ||
       (rows > 0 && (!query || !out)))
@@ -1177,7 +1182,8 @@ QKV_EXPORT int qkv_paged_attention(const void* query, const int64_t* q_strides, 
     return fail(QKV_ERR_UNSUPPORTED, "%s: a page's tokens must lie within 2^30 elements", what);
   const int64_t group = q_heads / kv_heads;
   Plan p = plan_of(rows, max_rows, requests, width * page, kv_heads, group);
-  if (p.rows.items + p.token.items > (1ll << 30)) return fail(QKV_ERR_UNSUPPORTED, "%s: too many rows", what);
+  // a grid has less than 2^32 threads
+  if (p.rows.items + p.token.items >= (1 << 24)) return fail(QKV_ERR_UNSUPPORTED, "%s: too many rows", what);
   const int64_t need = qkv_paged_attention_workspace_bytes(rows, max_rows, requests, width, page, q_heads, kv_heads, head_dim);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(QKV_ERR_INVALID, "%s: workspace must be 16-byte aligned and hold %lld bytes", what,

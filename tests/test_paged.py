@@ -121,3 +121,9 @@ def test_step_plan_buffers():
     p.slots.fill_(-1)
     p.positions.fill_(7)
     assert (p.slots == -1).all() and (p.positions == 7).all()
+
+
+def test_grids_have_less_than_2_32_threads():
+    for call in (lambda: _attend(rows=1 << 30, max_rows=1 << 30), lambda: _append(rows=1 << 30, heads=64)):
+        with pytest.raises(RuntimeError, match="too many rows"):
+            _lib.check(call())
