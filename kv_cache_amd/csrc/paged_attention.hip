@@ -383,11 +383,6 @@ __device__ __forceinline__ void load_lds16(const char* from, uint16_t* to) {
 }
 // The wave's loads have landed, and its reads of the step before have left LDS.
 __device__ __forceinline__ void wave_landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
-// Those of the workgroup have, and every wave is done with the tile before.
-__device__ __forceinline__ void loads_landed() {
-  __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
-  __syncthreads();
-}
 
 template <bool F16>
 __device__ __forceinline__ f32x16_t mfma_32x32x16(u32x4_t a, u32x4_t b, f32x16_t c) {
@@ -415,7 +410,7 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
   constexpr int UR = D / 8;                // 16-byte units of a row
   constexpr int NU = kTile * UR / 256;     // units a thread stages of K, and of V
   uint16_t *kbuf0 = stage0, *vbuf0 = stage0 + kTile * D, *kbuf1 = stage1, *vbuf1 = stage1 + kTile * D;
-  __shared__ int s_odd[2];
+  __shared__ int s_odd[2][4];
   Where w;
   if (!locate<false>(a, c, item, w)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -494,7 +489,7 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
   };
   // Where some row does not see all of a tile, what of V no row may read (a page's rest) becomes zero before it is
   // used, and so do infinities and NaN, which a zero weight would not hide; add_odd adds those to the rows that do
-  // see them.
+  // see them.  A wave cleans what it loaded itself, so that the barrier behind the loads serves for both.
   auto clean_tile = [&](int t0, bool holes, uint16_t* vb, int buf) {
     u32x4_t x[NU];
 #pragma unroll
@@ -508,8 +503,7 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
       odd |= any;
       if (rest || any) *reinterpret_cast<u32x4_t*>(vb + 8 * (256 * u + tid)) = x[u];
     }
-    if (odd) s_odd[buf] = t0;
-    __syncthreads();
+    s_odd[buf][wave] = __ballot(odd) != 0;
   };
   auto add_odd = [&](int t0) {
 #pragma unroll 1
@@ -627,23 +621,27 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
         const u32x2_t y = read_tr(vb_ + r1 * D + 8 * ((4 * d + v_unit) ^ swizzle<D>(r1)) + v_el);
         o[d] = mfma_32x32x16<F16>(u32x4_t{x[0], x[1], y[0], y[1]}, p[ks], o[d]);
       }
-    if (masked && s_odd[buf] == t0) add_odd(t0);
+    if (masked && (s_odd[buf][0] | s_odd[buf][1] | s_odd[buf][2] | s_odd[buf][3])) add_odd(t0);
   };
 
   // One barrier a tile: the next tile's loads are issued before this one is computed, and have landed behind it.
-  auto turn = [&](int t0, const uint16_t* kb_, uint16_t* vb_, int buf, uint16_t* kn, uint16_t* vn)
+  bool holes, masked;   // of the tile that has landed
+  auto landed = [&](int t0, uint16_t* vb, int buf) __attribute__((always_inline)) {
+    wave_landed();
+    holes = hole, masked = t0 < wg_all_lo || t0 + kTile > wg_all_hi || holes;
+    if (masked && t0 < end) clean_tile(t0, holes, vb, buf);
+    __syncthreads();
+  };
+  auto turn = [&](int t0, const uint16_t* kb_, const uint16_t* vb_, int buf, uint16_t* kn, uint16_t* vn)
                   __attribute__((always_inline)) {
-    const bool holes = hole, masked = t0 < wg_all_lo || t0 + kTile > wg_all_hi || holes;
     const Pages next = pages_of(t0 + kTile);
-    if (masked) clean_tile(t0, holes, vb_, buf);
     if (t0 + kTile < end) load(t0 + kTile, next, kn, vn);
     compute(t0, masked, holes, kb_, vb_, buf);
-    loads_landed();
+    landed(t0 + kTile, vn, buf ^ 1);
   };
-  if (tid < 2) s_odd[tid] = -1;
   if (begin < end) {
     load(begin, pages_of(begin), kbuf0, vbuf0);
-    loads_landed();
+    landed(begin, vbuf0, 0);
     for (int t0 = begin; t0 < end; t0 += 2 * kTile) {
       turn(t0, kbuf0, vbuf0, 0, kbuf1, vbuf1);
       if (t0 + kTile < end) turn(t0 + kTile, kbuf1, vbuf1, 1, kbuf0, vbuf0);
