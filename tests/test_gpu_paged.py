@@ -643,3 +643,40 @@ def test_offsets_past_32_bits():
     rows = torch.randn((2, hkv, dim), device=DEV).to(torch.bfloat16)
     paged.append(rows, rows, kp, vp, slots)
     assert torch.equal(kp[-1, :, -1], rows[0]) and torch.equal(vp[0, :, 5], rows[1])
+
+
+def test_calls_on_two_streams_at_once():
+    cases = [_case([2000, 90], [1, 30], 8, 2, 128, 16, "bf16", seed=27), _case([1500], [1], 8, 2, 64, 64, "fp16", seed=28)]
+    want = [paged.attention(**c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(6):
+        for c, s, g in zip(cases, streams, got):
+            with torch.cuda.stream(s):
+                g.append(paged.attention(**c))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    for w, g in zip(want, got):
+        assert all(torch.equal(x, w) for x in g)
+
+
+def test_two_graphs_share_a_workspace():
+    cases = [_case([2000, 90], [1, 30], 8, 2, 128, 16, "bf16", seed=29), _case([700, 1900], [1, 1], 8, 2, 128, 16, "bf16", seed=30)]
+    want = [paged.attention(**c) for c in cases]
+    size = max(paged.attention_workspace(c["query"].shape[0], c["query"].shape[0], *c["table"].shape, 16, 8, 2, 128,
+                                         DEV).numel() for c in cases)
+    ws = torch.empty(size, device=DEV)
+    outs = [torch.empty_like(w) for w in want]
+    graphs = []
+    for c, o in zip(cases, outs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            paged.attention(**c, workspace=ws, out=o)
+    for _ in range(4):
+        for g, o, w, c in zip(graphs, outs, want, cases):
+            ws.fill_(float("nan"))
+            o.zero_()
+            g.replay()
+            assert torch.equal(o, w) and torch.equal(paged.attention(**c), w)
