@@ -347,13 +347,13 @@ class _PagedState:
             pages = batch * -(-self.capacity // self.page)
             self.table = paged.PageTable(batch, self.capacity, pages, self.page, device)
         new = torch.full((batch,), n, dtype=torch.int32, device=device)
-        if attention_mask is not None and n > 1:
+        if attention_mask is not None:
             if window is not None and n > window:
                 raise RuntimeError(f"a masked chunk of {n} tokens on a layer with a sliding window of {window}: split it")
-            # the last query's view of the step's own columns: padding is hidden
+            # the last query's view of the step's own columns: padding is hidden, a single column like any other
             seen = attention_mask[..., -1, length - n:length].reshape(-1, n)
             seen = seen if seen.dtype == torch.bool else seen == 0
-            if not bool((seen[:, 1:] | ~seen[:, :-1]).all()):
+            if n > 1 and not bool((seen[:, 1:] | ~seen[:, :-1]).all()):
                 raise RuntimeError("paged attention takes left-padded batches (padding before the tokens of a step)")
             new = seen.sum(-1, dtype=torch.int32).expand(batch).contiguous()
         self.plan = self.table.step(new, batch * n, padded=n)
