@@ -329,41 +329,94 @@ def register_mode(mode: str, capacity: int, *, name: str | None = None, **step_k
 ATTENTION_STEPS: dict = {}
 
 
+# An additive mask hides a key with this or less: its weight is zero beside any score.
+_HIDDEN = -1.0e4
+
+
 class _PagedState:
-    """What the layers of one PagedCache share: the page table, and the plan
-    of the step that the first layer to reach it made."""
+    """What the layers of one PagedCache share: the page table, which columns
+    hold tokens, and the plan of the step that the first layer to reach it
+    made."""
 
     def __init__(self, capacity: int, page: int):
         self.capacity, self.page = int(capacity), int(page)
         self.table = self.plan = None
+        self.real = None         # bool [batch, capacity]: columns with a token; None while all have one
+        self.masks = []          # (mask, window) of the step's layers, compared with what the pages show
         self.length = 0          # columns stepped, padding included
 
     def step(self, length: int, n: int, batch: int, device, attention_mask, window) -> paged.StepPlan:
         """The plan of the step that brings the sequences to ``length``
-        columns with ``n`` new ones."""
-        if self.length == length:
+        columns with ``n`` new ones; raises where a layer's mask is not what
+        its attention over the pages shows."""
+        first = self.length != length
+        if first:
+            self.masks = []
+        # layers share a mask or two: one host read for each in a step
+        if attention_mask is not None and not any(m is attention_mask and w == window for m, w in self.masks):
+            self._compare(length, n, batch, device, attention_mask, window, first)
+            self.masks.append((attention_mask, window))
+        elif first and self.real is not None:
+            self.real[:, length - n:length] = True
+        if not first:
             return self.plan
         if self.table is None:
             pages = batch * -(-self.capacity // self.page)
             self.table = paged.PageTable(batch, self.capacity, pages, self.page, device)
-        new = torch.full((batch,), n, dtype=torch.int32, device=device)
-        if attention_mask is not None:
-            if window is not None and n > window:
-                raise RuntimeError(f"a masked chunk of {n} tokens on a layer with a sliding window of {window}: split it")
-            # the last query's view of the step's own columns: padding is hidden, a single column like any other
-            seen = attention_mask[..., -1, length - n:length].reshape(-1, n)
-            seen = seen if seen.dtype == torch.bool else seen == 0
-            if n > 1 and not bool((seen[:, 1:] | ~seen[:, :-1]).all()):
-                raise RuntimeError("paged attention takes left-padded batches (padding before the tokens of a step)")
-            new = seen.sum(-1, dtype=torch.int32).expand(batch).contiguous()
+        if attention_mask is None:
+            new = torch.full((batch,), n, dtype=torch.int32, device=device)
+        else:
+            new = self.real[:, length - n:length].sum(-1, dtype=torch.int32)
         self.plan = self.table.step(new, batch * n, padded=n)
         self.length = length
         return self.plan
 
+    def _compare(self, length: int, n: int, batch: int, device, mask, window, first: bool) -> None:
+        """Takes the padding of the step's columns from the mask (``first``)
+        and compares the rest of it: a token's query has to see its sequence's
+        tokens up to its own, within the window.  The rows of padding may see
+        anything."""
+        if (mask.dim() != 4 or mask.size(0) not in (1, batch) or mask.size(2) not in (1, n) or mask.size(3) < length
+                or not (mask.dtype == torch.bool or mask.is_floating_point())):
+            raise RuntimeError(f"paged attention takes bool or additive masks [{batch}, heads, {n}, {length} columns], "
+                               f"got {mask.dtype} {list(mask.shape)}")
+        mask = mask[..., :length].expand(batch, -1, n, -1)
+        if self.real is None:
+            real = torch.ones((batch, length), dtype=torch.bool, device=device)
+        else:
+            real = self.real[:, :length].clone()
+        if first:   # padding: a column that its own query does not see
+            own = mask[:, 0, :, length - n:].diagonal(dim1=-2, dim2=-1)
+            real[:, length - n:] = own if own.dtype == torch.bool else own == 0
+        fresh = real[:, length - n:]
+        at = torch.arange(length, device=device)
+        token = None if window is None else real.cumsum(-1)   # the window counts tokens, as the pages hold them
+        other = torch.zeros((), dtype=torch.bool, device=device)
+        rows = max(1, (1 << 26) // (batch * mask.size(1) * length))   # bounds what is compared at a time
+        for i in range(0, n, rows):
+            cols = slice(length - n + i, min(length - n + i + rows, length))
+            seen = real[:, None] & (at <= at[cols, None])
+            if window is not None:
+                seen &= token[:, None] > token[:, cols, None] - window
+            seen, m = seen[:, None], mask[:, :, i:i + rows]
+            same = m == seen if m.dtype == torch.bool else torch.where(seen, m == 0, m <= _HIDDEN)
+            other |= (~same & real[:, None, cols, None]).any()
+        order = (fresh[:, :-1] & ~fresh[:, 1:]).any()
+        other, order = torch.stack((other, order)).tolist()
+        if order:
+            raise RuntimeError("paged attention takes left-padded batches (padding before the tokens of a step)")
+        if other:
+            raise RuntimeError("paged attention takes causal masks, with the layer's sliding window and left padding; "
+                               "this mask shows or hides other keys")
+        if first:
+            if self.real is None:
+                self.real = torch.ones((batch, self.capacity), dtype=torch.bool, device=device)
+            self.real[:, length - n:length] = fresh
+
     def reset(self) -> None:
         if self.table is not None and self.length:
             self.table.release(torch.zeros_like(self.table.lens))
-        self.length = 0
+        self.length, self.real, self.masks = 0, None, []
 
 
 class PagedCacheLayer:

@@ -150,3 +150,140 @@ def test_a_sequence_without_a_token_in_a_single_step(taken):
     got = _run(model, "paged", hf.PagedCache(capacity=16, page=16), ids, mask, [4, 1, 1])
     assert taken == [[4, 4], [1, 0], [1, 1]]
     _near(got, _run(model, "sdpa", _dense(model), ids, mask, [4, 1, 1]), mask.bool())
+
+
+# -- masks that are not what the pages show ----------------------------------------
+
+
+def _causal(lens, n, total=None, window=None):
+    """bool [B, 1, n, total]: the mask of left-padded sequences, for the last n of total columns."""
+    total = n if total is None else total
+    own, j = torch.arange(total - n, total)[:, None], torch.arange(total)
+    m = j <= own
+    if window is not None:
+        m &= j > own - window
+    return torch.stack([m & (j >= total - k) for k in lens])[:, None]
+
+
+def _as_float(m, low):
+    return torch.where(m, 0.0, low)
+
+
+FOREIGN = ["two_sided", "prefix", "documents", "hidden_history", "one_head", "one_row", "soft", "a_later_column",
+           "integers", "two_axes", "too_narrow"]
+
+
+@pytest.mark.parametrize("form", FOREIGN)
+def test_masks_of_other_forms_are_refused(taken, form):
+    model, ids = _model(), _tokens(2, 6, 3)
+    m = _causal([6, 4], 6)
+    if form == "two_sided":
+        m = m | (torch.arange(6) >= 2)
+    elif form == "prefix":
+        m[:, :, :3, 2:3] = True
+    elif form == "documents":
+        m[:, :, 3:, :3] = False
+    elif form == "hidden_history":
+        m[1, 0, 5, 3] = False
+    elif form == "one_head":
+        m = m.expand(2, 4, 6, 6).clone()
+        m[0, 2, 4, 1] = False
+    elif form == "one_row":
+        m = m[:, :, -1:]
+    elif form == "soft":
+        m = _as_float(m, -1.0)
+    elif form == "a_later_column":
+        m[0, 0, 2, 3] = True
+    elif form == "integers":
+        m = m.long()
+    elif form == "two_axes":
+        m = m[0, 0]
+    elif form == "too_narrow":
+        m = m[..., :5]
+    cache = hf.PagedCache(capacity=16, page=16)
+    model.config._attn_implementation = "paged"
+    q, k = torch.randn(2, 4, 6, 16), torch.randn(2, 2, 6, 16)
+    key, value = cache.update(k, k, 0)
+    with pytest.raises(RuntimeError, match="mask"):
+        hf.paged_attention_forward(model.model.layers[0].self_attn, q, key, value, m)
+    assert taken == []
+
+
+def _attend(cache, m, n, layer=0, window=None, seed=0, **kw):
+    g = torch.Generator().manual_seed(seed)
+    q, k = torch.randn((2, 4, n, 16), generator=g), torch.randn((2, 2, n, 16), generator=g)
+    key, value = cache.update(k, k, layer)
+    return hf.paged_attention_forward(None, q, key, value, m, sliding_window=window, **kw)[0]
+
+
+@pytest.mark.parametrize("low", [None, -1.0e4, -1.0e9, torch.finfo(torch.float32).min, -torch.inf])
+def test_causal_masks_with_left_padding_are_taken(taken, low):
+    form = (lambda m: m) if low is None else (lambda m: _as_float(m, low))
+    a, b = hf.PagedCache(capacity=32, page=16), hf.PagedCache(capacity=32, page=16)
+    for i, (n, total) in enumerate(((6, 6), (1, 7), (3, 10))):
+        m = _causal([total, total - 2], n, total)
+        if n > 1 and total == n:
+            m[1, 0, :2] = True       # what rows of padding see does not matter, beyond their own column
+            m[1, 0, 0, 0] = m[1, 0, 1, 1] = False
+        got = _attend(a, form(m), n, seed=i)
+        assert torch.equal(got, _attend(b, form(m.expand(2, 4, n, total)), n, seed=i))
+    assert taken[0::2] == taken[1::2] == [[6, 4], [1, 1], [3, 3]]
+
+
+def test_one_column_that_hides_history_is_refused(taken):
+    cache = hf.PagedCache(capacity=32, page=16)
+    _attend(cache, _causal([5, 3], 5), 5)
+    m = _causal([6, 4], 1, 6)
+    m[0, 0, 0, 2] = False
+    with pytest.raises(RuntimeError, match="mask"):
+        _attend(cache, m, 1)
+    cache = hf.PagedCache(capacity=32, page=16)
+    _attend(cache, None, 5)
+    with pytest.raises(RuntimeError, match="mask"):
+        _attend(cache, m, 1)
+
+
+def test_every_layers_mask_is_looked_at(taken):
+    cache = hf.PagedCache(capacity=32, page=16)
+    m = _causal([5, 3], 5)
+    _attend(cache, m, 5, layer=0)
+    chunks = m & ((torch.arange(5)[:, None] // 2) == (torch.arange(5) // 2))
+    with pytest.raises(RuntimeError, match="mask"):
+        _attend(cache, chunks, 5, layer=1)
+    # a layer with a window, and one whose mask has another
+    cache = hf.PagedCache(capacity=32, page=16)
+    _attend(cache, m, 5, layer=0)
+    _attend(cache, _causal([5, 3], 5, window=2), 5, layer=1, window=2)
+    with pytest.raises(RuntimeError, match="mask"):
+        _attend(cache, _causal([5, 3], 5, window=3), 5, layer=2, window=2)
+
+
+@pytest.mark.parametrize("kinds", [["full_attention", "sliding_attention"], ["sliding_attention", "full_attention"]])
+@pytest.mark.parametrize("window", [3, 7])
+def test_windows_match_dense(taken, window, kinds):
+    # chunks longer than the window too, in left-padded batches and without a mask
+    extra = dict(use_sliding_window=True, sliding_window=window, layer_types=kinds)
+    model, widths = _model(**extra), [5, 1, 4, 1]
+    ids, mask = _tokens(2, 11, 4), torch.cat([_left_padded([5, 3], 5), torch.ones((2, 6), dtype=torch.long)], 1)
+    for m in (mask, None):
+        got = _run(model, "paged", hf.PagedCache(capacity=32, page=16), ids, m, widths)
+        # a dense cache without the sliding layers' own, which keeps fewer columns
+        from transformers.cache_utils import DynamicCache
+        want = _run(model, "sdpa", DynamicCache(), ids, m, widths)
+        _near(got, want, torch.ones((2, 11), dtype=torch.bool) if m is None else m.bool())
+
+
+def test_a_window_over_padding_between_tokens_is_refused(taken):
+    # the window counts columns in the mask, tokens in the pages
+    cache = hf.PagedCache(capacity=32, page=16)
+    _attend(cache, _causal([4, 4], 4, window=3), 4, window=3)
+    m = _causal([7, 7], 3, 7, window=3)
+    m[1, 0, :, 4:6] = False
+    with pytest.raises(RuntimeError, match="mask"):
+        _attend(cache, m, 3, window=3)
+    cache = hf.PagedCache(capacity=32, page=16)
+    _attend(cache, _causal([4, 4], 4), 4)
+    m = _causal([7, 7], 3, 7)
+    m[1, 0, :, 4:6] = False
+    _attend(cache, m, 3)
+    assert taken[-1] == [3, 1]
