@@ -504,6 +504,23 @@ def _paged_layer_class(mixin):
     return type("PagedCacheLayerHF", (PagedCacheLayer, mixin), {"__init__": PagedCacheLayer.__init__})
 
 
+# Arguments of the attention interface that hold a tensor and do not change what is attended to or how.
+_IGNORED = frozenset(("position_ids", "cache_position", "token_type_ids", "input_ids", "labels", "num_items_in_batch"))
+
+
+def _check_interface(module, n: int, key: torch.Tensor, attention_mask, arguments: dict) -> None:
+    """Raises for what the attention over the pages would leave out: scores
+    with sinks or biases, packed sequences, queries that see later keys."""
+    for name, x in arguments.items():
+        if isinstance(x, float) or (isinstance(x, torch.Tensor) and name not in _IGNORED):
+            raise RuntimeError(f"paged attention does not take {name}")
+    if key.size(2) != n:
+        raise RuntimeError(f"paged attention takes queries and keys of the same tokens, got {n} and {key.size(2)}")
+    causal = arguments.get("is_causal")
+    if n > 1 and attention_mask is None and not (getattr(module, "is_causal", True) if causal is None else causal):
+        raise RuntimeError("paged attention is causal: is_causal is False and there is no mask")
+
+
 def paged_attention_forward(module, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, attention_mask,
                             scaling: float | None = None, dropout: float = 0.0, softcap: float | None = None,
                             sliding_window: int | None = None, **kwargs):
@@ -519,6 +536,7 @@ def paged_attention_forward(module, query: torch.Tensor, key: torch.Tensor, valu
     if dropout:
         raise RuntimeError("paged attention has no dropout")
     b, hq, n, d = query.shape
+    _check_interface(module, n, key, attention_mask, kwargs)
     state = layer.state
     plan = state.step(layer.length, n, b, query.device, attention_mask, sliding_window)
     rows = lambda x: x.transpose(1, 2).reshape(b * n, x.size(1), d)  # noqa: E731  (a view of what projections give)

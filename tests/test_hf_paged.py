@@ -287,3 +287,53 @@ def test_a_window_over_padding_between_tokens_is_refused(taken):
     m[1, 0, :, 4:6] = False
     _attend(cache, m, 3)
     assert taken[-1] == [3, 1]
+
+
+# -- arguments of the attention interface ---------------------------------------------
+
+
+@pytest.mark.parametrize("name,value", [
+    ("s_aux", torch.zeros(4)), ("position_bias", torch.zeros(1, 4, 6, 6)), ("head_mask", torch.ones(4)),
+    ("cu_seq_lens_q", torch.tensor([0, 3, 6])), ("logit_cap", 30.0), ("is_causal", False)])
+def test_arguments_that_change_scores_are_refused(taken, name, value):
+    cache = hf.PagedCache(capacity=16, page=16)
+    with pytest.raises(RuntimeError, match=name):
+        _attend(cache, None, 6, **{name: value})
+    assert taken == []
+
+
+def test_arguments_that_change_nothing_are_taken(taken):
+    cache = hf.PagedCache(capacity=16, page=16)
+    got = _attend(cache, None, 6, position_ids=torch.arange(6)[None], cache_position=torch.arange(6), use_cache=True,
+                  output_attentions=False, s_aux=None, is_causal=True, logits_to_keep=1)
+    assert torch.equal(got, _attend(hf.PagedCache(capacity=16, page=16), None, 6))
+    # a mask says itself what is causal, a single query is last
+    _attend(cache, _causal([9, 9], 3, 9), 3, is_causal=False)
+    _attend(cache, None, 1, is_causal=False)
+
+
+def test_a_module_that_is_not_causal_is_refused(taken):
+    class Module(torch.nn.Module):
+        is_causal = False
+
+    key, value = hf.PagedCache(capacity=16, page=16).update(*[torch.randn(2, 2, 6, 16)] * 2, 0)
+    with pytest.raises(RuntimeError, match="is_causal"):
+        hf.paged_attention_forward(Module(), torch.randn(2, 4, 6, 16), key, value, None)
+
+
+def test_keys_of_another_sequence_are_refused(taken):
+    # cross attention: queries and keys are not of the same tokens
+    key, value = hf.PagedCache(capacity=16, page=16).update(*[torch.randn(2, 2, 6, 16)] * 2, 0)
+    with pytest.raises(RuntimeError, match="same tokens"):
+        hf.paged_attention_forward(None, torch.randn(2, 4, 3, 16), key, value, None)
+
+
+def test_attention_sinks_of_a_model_are_refused(taken):
+    from transformers import GptOssConfig, GptOssForCausalLM
+
+    torch.manual_seed(0)
+    model = GptOssForCausalLM(GptOssConfig(vocab_size=64, hidden_size=64, intermediate_size=64, num_hidden_layers=2,
+                                           num_attention_heads=4, num_key_value_heads=2, head_dim=16, sliding_window=8,
+                                           num_local_experts=2, num_experts_per_tok=1)).eval()
+    with pytest.raises(RuntimeError, match="s_aux"):
+        _run(model, "paged", hf.PagedCache(capacity=16, page=16), _tokens(2, 5, 5), None, [5])
