@@ -344,6 +344,14 @@ class _PagedState:
         self.real = None         # bool [batch, capacity]: columns with a token; None while all have one
         self.masks = []          # (mask, window) of the step's layers, compared with what the pages show
         self.length = 0          # columns stepped, padding included
+        self.open = False        # an update's columns have not been attended over yet
+
+    def check_closed(self) -> None:
+        """Raises if the attention function did not take an earlier update:
+        its columns are in no page."""
+        if self.open:
+            raise RuntimeError("K and V of an earlier update of this PagedCache were not taken: run the model with the "
+                               "attention implementation of register_paged, and reset() the cache")
 
     def step(self, length: int, n: int, batch: int, device, attention_mask, window) -> paged.StepPlan:
         """The plan of the step that brings the sequences to ``length``
@@ -416,13 +424,15 @@ class _PagedState:
     def reset(self) -> None:
         if self.table is not None and self.length:
             self.table.release(torch.zeros_like(self.table.lens))
-        self.length, self.real, self.masks = 0, None, []
+        self.length, self.real, self.masks, self.open = 0, None, [], False
 
 
 class PagedCacheLayer:
     """One layer's K/V pages (bf16 or fp16).  ``update`` only counts the new
     columns and hands the layer on to the attention function with their K/V;
-    that one knows the mask, and writes what is no padding into the pages."""
+    that one knows the mask, and writes what is no padding into the pages.
+    Another attention function would see the new columns alone: the next
+    update raises then."""
 
     is_sliding = False
     is_compileable = False
@@ -448,17 +458,20 @@ class PagedCacheLayer:
         self.is_initialized = True
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args, **kwargs):
+        self.state.check_closed()
         if not self.is_initialized:
             self.lazy_initialization(key_states, value_states)
         n = key_states.size(-2)
         if self.length + n > self.state.capacity:
             raise RuntimeError(f"Paged cache capacity {self.state.capacity} exceeded ({self.length + n} tokens)")
         self.length += n
+        self.state.open = True
         key_states = key_states.view(key_states.shape)
         key_states.paged_layer = self
         return key_states, value_states
 
     def get_mask_sizes(self, query_length: int):
+        self.state.check_closed()
         return self.length + query_length, 0
 
     def get_seq_length(self) -> int:
@@ -545,6 +558,7 @@ def paged_attention_forward(module, query: torch.Tensor, key: torch.Tensor, valu
     out = paged.attention(rows(query), layer.k_pages, layer.v_pages, state.table.table, plan.cu_rows, plan.kv_lens,
                           d ** -0.5 if scaling is None else float(scaling), max_rows=n,
                           softcap=0.0 if softcap is None else float(softcap), first_keys=first)
+    state.open = False
     return out.view(b, n, hq, d), None
 
 

@@ -337,3 +337,49 @@ def test_attention_sinks_of_a_model_are_refused(taken):
                                            num_local_experts=2, num_experts_per_tok=1)).eval()
     with pytest.raises(RuntimeError, match="s_aux"):
         _run(model, "paged", hf.PagedCache(capacity=16, page=16), _tokens(2, 5, 5), None, [5])
+
+
+# -- updates that the paged attention function did not take ------------------------------
+
+
+@pytest.mark.parametrize("layers", [1, 2])
+@pytest.mark.parametrize("impl", ["sdpa", "eager"])
+def test_another_implementation_raises(taken, layers, impl):
+    # it would see the step's own columns alone, and the pages would stay empty
+    model, ids = _model(layers=layers), _tokens(2, 7, 6)
+    with pytest.raises(RuntimeError, match="register_paged"):
+        _run(model, impl, hf.PagedCache(capacity=16, page=16), ids, None, [6, 1])
+
+
+def test_a_key_that_lost_its_layer_raises(taken):
+    cache = hf.PagedCache(capacity=16, page=16)
+    q, k = torch.randn(2, 4, 6, 16), torch.randn(2, 2, 6, 16)
+    key, value = cache.update(k, k, 0)
+    # dense over the new columns, as for any keys without a layer
+    module = torch.nn.Module()
+    module.num_key_value_groups = 2
+    hf.paged_attention_forward(module, q, key * 1.0, value, None)
+    with pytest.raises(RuntimeError, match="register_paged"):
+        cache.update(k, k, 1)
+    with pytest.raises(RuntimeError, match="register_paged"):
+        cache.layers[0].get_mask_sizes(1)
+    cache.reset()
+    assert cache.layers[0].get_mask_sizes(6) == (6, 0)
+    _attend(cache, None, 6)
+    assert taken == [[6, 6]]
+
+
+def test_a_step_that_fails_in_a_later_layer_has_to_be_reset(taken):
+    # the layers before hold the step's columns already
+    cache = hf.PagedCache(capacity=32, page=16)
+    m = _causal([5, 3], 5)
+    _attend(cache, m, 5, layer=0)
+    with pytest.raises(RuntimeError, match="mask"):
+        _attend(cache, m | True, 5, layer=1)
+    for layer in (0, 1):
+        with pytest.raises(RuntimeError, match="reset"):
+            _attend(cache, m, 5, layer=layer)
+    cache.reset()
+    _attend(cache, m, 5, layer=0)
+    _attend(cache, m, 5, layer=1)
+    assert taken == [[5, 3]] * 2
