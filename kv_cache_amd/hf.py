@@ -368,7 +368,7 @@ class _PagedState:
             self.real[:, length - n:length] = True
         if not first:
             return self.plan
-        if self.table is None:
+        if self.table is None or (self.length == 0 and self.table.lens.numel() != batch):
             pages = batch * -(-self.capacity // self.page)
             self.table = paged.PageTable(batch, self.capacity, pages, self.page, device)
         if attention_mask is None:
@@ -448,10 +448,25 @@ class PagedCacheLayer:
     def __repr__(self):
         return f"PagedCacheLayer(length={self.length}, capacity={self.state.capacity}, page={self.state.page})"
 
+    def page_shape(self, key_states: torch.Tensor) -> tuple:
+        b, h, _, d = key_states.shape
+        return b * -(-self.state.capacity // self.state.page), h, self.state.page, d
+
+    def holds(self, key_states: torch.Tensor) -> bool:
+        """Whether the pages are those of such keys."""
+        return (self.k_pages.shape == self.page_shape(key_states) and self.dtype == key_states.dtype
+                and self.device == key_states.device)
+
+    def take_back(self, n: int) -> None:
+        """Undoes an update whose step was refused before anything was written;
+        a step that other layers have made stays open."""
+        if self.state.length != self.length:
+            self.length -= n
+            self.state.open = False
+
     # -- CacheLayerMixin protocol ------------------------------------------
     def lazy_initialization(self, key_states: torch.Tensor, value_states: torch.Tensor) -> None:
-        b, h, _, d = key_states.shape
-        shape = (b * -(-self.state.capacity // self.state.page), h, self.state.page, d)
+        shape = self.page_shape(key_states)
         self.dtype, self.device = key_states.dtype, key_states.device
         self.k_pages = torch.empty(shape, dtype=key_states.dtype, device=key_states.device)
         self.v_pages = torch.empty(shape, dtype=value_states.dtype, device=key_states.device)
@@ -459,11 +474,12 @@ class PagedCacheLayer:
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args, **kwargs):
         self.state.check_closed()
-        if not self.is_initialized:
-            self.lazy_initialization(key_states, value_states)
         n = key_states.size(-2)
         if self.length + n > self.state.capacity:
             raise RuntimeError(f"Paged cache capacity {self.state.capacity} exceeded ({self.length + n} tokens)")
+        # an empty layer takes any batch, whatever it held before
+        if not self.is_initialized or (self.length == 0 and not self.holds(key_states)):
+            self.lazy_initialization(key_states, value_states)
         self.length += n
         self.state.open = True
         key_states = key_states.view(key_states.shape)
@@ -521,9 +537,12 @@ def _paged_layer_class(mixin):
 _IGNORED = frozenset(("position_ids", "cache_position", "token_type_ids", "input_ids", "labels", "num_items_in_batch"))
 
 
-def _check_interface(module, n: int, key: torch.Tensor, attention_mask, arguments: dict) -> None:
-    """Raises for what the attention over the pages would leave out: scores
-    with sinks or biases, packed sequences, queries that see later keys."""
+def _check_interface(module, n: int, key: torch.Tensor, attention_mask, dropout: float, arguments: dict) -> None:
+    """Raises for what the attention over the pages would leave out: dropout,
+    scores with sinks or biases, packed sequences, queries that see later
+    keys."""
+    if dropout:
+        raise RuntimeError("paged attention has no dropout")
     for name, x in arguments.items():
         if isinstance(x, float) or (isinstance(x, torch.Tensor) and name not in _IGNORED):
             raise RuntimeError(f"paged attention does not take {name}")
@@ -546,12 +565,14 @@ def paged_attention_forward(module, query: torch.Tensor, key: torch.Tensor, valu
     if layer is None:
         return sdpa_attention_forward(module, query, key, value, attention_mask, dropout=dropout, scaling=scaling,
                                       **kwargs)
-    if dropout:
-        raise RuntimeError("paged attention has no dropout")
     b, hq, n, d = query.shape
-    _check_interface(module, n, key, attention_mask, kwargs)
     state = layer.state
-    plan = state.step(layer.length, n, b, query.device, attention_mask, sliding_window)
+    try:
+        _check_interface(module, n, key, attention_mask, dropout, kwargs)
+        plan = state.step(layer.length, n, b, query.device, attention_mask, sliding_window)
+    except RuntimeError:
+        layer.take_back(key.size(2))
+        raise
     rows = lambda x: x.transpose(1, 2).reshape(b * n, x.size(1), d)  # noqa: E731  (a view of what projections give)
     paged.append(rows(key), rows(value), layer.k_pages, layer.v_pages, plan.slots)
     first = None if sliding_window is None else plan.positions - (int(sliding_window) - 1)

@@ -369,6 +369,36 @@ def test_a_key_that_lost_its_layer_raises(taken):
     assert taken == [[6, 6]]
 
 
+def test_a_refused_step_leaves_the_cache_as_it_was(taken):
+    cache = hf.PagedCache(capacity=32, page=16)
+    first = _attend(cache, _causal([5, 3], 5), 5, seed=1)
+    wrong = _causal([8, 6], 3, 8)
+    wrong[0, 0, 2, 4] = False
+    for bad in (dict(m=wrong), dict(m=None, s_aux=torch.zeros(4))):
+        with pytest.raises(RuntimeError):
+            _attend(cache, n=3, **bad)
+        assert cache.get_seq_length() == 5 and cache.layers[0].get_mask_sizes(3) == (8, 0)
+    with pytest.raises(RuntimeError, match="exceeded"):
+        _attend(cache, None, 28)
+    got = _attend(cache, _causal([8, 6], 3, 8), 3, seed=2)
+    other = hf.PagedCache(capacity=32, page=16)
+    assert torch.equal(first, _attend(other, _causal([5, 3], 5), 5, seed=1))
+    assert torch.equal(got, _attend(other, _causal([8, 6], 3, 8), 3, seed=2))
+    assert taken == [[5, 3], [3, 3]] * 2
+
+
+def test_a_refused_first_step_binds_the_cache_to_nothing(taken):
+    # its batch, heads and dtype were never taken
+    cache = hf.PagedCache(capacity=32, page=16)
+    wrong = _causal([6, 6], 6) | True
+    with pytest.raises(RuntimeError, match="mask"):
+        _attend(cache, wrong, 6)
+    k = torch.randn(3, 1, 4, 8, dtype=torch.float64)
+    key, value = cache.update(k, k, 0)
+    out, _ = hf.paged_attention_forward(None, torch.randn(3, 2, 4, 8, dtype=torch.float64), key, value, None)
+    assert out.shape == (3, 4, 2, 8) and taken == [[4, 4, 4]]
+
+
 def test_a_step_that_fails_in_a_later_layer_has_to_be_reset(taken):
     # the layers before hold the step's columns already
     cache = hf.PagedCache(capacity=32, page=16)
