@@ -343,7 +343,7 @@ class _PagedState:
         self.table = self.plan = None
         self.real = None         # bool [batch, capacity]: columns with a token; None while all have one
         self.masks = []          # (mask, window) of the step's layers, compared with what the pages show
-        self.length = 0          # columns stepped, padding included
+        self.length = self.new = 0   # columns stepped, padding included; of the last step
         self.open = False        # an update's columns have not been attended over yet
 
     def check_closed(self) -> None:
@@ -358,6 +358,9 @@ class _PagedState:
         columns with ``n`` new ones; raises where a layer's mask is not what
         its attention over the pages shows."""
         first = self.length != length
+        if length - n != (self.length if first else self.length - self.new):
+            raise RuntimeError(f"the layers of a PagedCache step together: a layer steps from {length - n} columns to "
+                               f"{length}, the cache holds {self.length}")
         if first:
             self.masks = []
         # layers share a mask or two: one host read for each in a step
@@ -376,7 +379,7 @@ class _PagedState:
         else:
             new = self.real[:, length - n:length].sum(-1, dtype=torch.int32)
         self.plan = self.table.step(new, batch * n, padded=n)
-        self.length = length
+        self.length, self.new = length, n
         return self.plan
 
     def _compare(self, length: int, n: int, batch: int, device, mask, window, first: bool) -> None:

@@ -413,3 +413,14 @@ def test_a_step_that_fails_in_a_later_layer_has_to_be_reset(taken):
     _attend(cache, m, 5, layer=0)
     _attend(cache, m, 5, layer=1)
     assert taken == [[5, 3]] * 2
+
+
+@pytest.mark.parametrize("n", [1, 5, 6])
+def test_layers_that_step_apart_are_refused(taken, n):
+    # one plan serves all layers of a step: a layer that left one out is behind
+    cache = hf.PagedCache(capacity=32, page=16)
+    _attend(cache, None, 5, layer=0)
+    _attend(cache, None, 1, layer=0)
+    with pytest.raises(RuntimeError, match="together"):
+        _attend(cache, None, n, layer=1)
+    assert taken == [[5, 5], [1, 1]]
