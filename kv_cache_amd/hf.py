@@ -556,6 +556,20 @@ def _check_interface(module, n: int, key: torch.Tensor, attention_mask, dropout:
         raise RuntimeError("paged attention is causal: is_causal is False and there is no mask")
 
 
+class _NoBackward(torch.autograd.Function):
+    """Ties an output to the inputs it has no gradients for: a backward pass
+    raises, where it would leave their part out."""
+
+    @staticmethod
+    def forward(ctx, out, *inputs):
+        return out.view_as(out)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("paged attention has no backward: run the model under torch.no_grad(), or train it without a "
+                           "PagedCache")
+
+
 def paged_attention_forward(module, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, attention_mask,
                             scaling: float | None = None, dropout: float = 0.0, softcap: float | None = None,
                             sliding_window: int | None = None, **kwargs):
@@ -583,6 +597,8 @@ def paged_attention_forward(module, query: torch.Tensor, key: torch.Tensor, valu
                           d ** -0.5 if scaling is None else float(scaling), max_rows=n,
                           softcap=0.0 if softcap is None else float(softcap), first_keys=first)
     state.open = False
+    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
+        out = _NoBackward.apply(out, query, key, value)
     return out.view(b, n, hq, d), None
 
 

@@ -424,3 +424,17 @@ def test_layers_that_step_apart_are_refused(taken, n):
     with pytest.raises(RuntimeError, match="together"):
         _attend(cache, None, n, layer=1)
     assert taken == [[5, 5], [1, 1]]
+
+
+# -- gradients ---------------------------------------------------------------------------
+
+
+def test_a_backward_pass_raises(taken):
+    # the pages hold no graph: gradients through them would be left out of those of the parameters
+    model, ids = _model(), _tokens(2, 6, 7)
+    model.config._attn_implementation = "paged"
+    want = _run(model, "paged", hf.PagedCache(capacity=16, page=16), ids, None, [6])
+    got = model(ids, past_key_values=hf.PagedCache(capacity=16, page=16), use_cache=True).logits
+    assert torch.equal(got, want)
+    with pytest.raises(RuntimeError, match="no backward"):
+        got.sum().backward()
