@@ -680,3 +680,16 @@ def test_two_graphs_share_a_workspace():
             o.zero_()
             g.replay()
             assert torch.equal(o, w) and torch.equal(paged.attention(**c), w)
+
+
+def test_lengths_past_the_table_row_are_its_end():
+    # 7 pages of 16 keys: kv_lens beyond them is read as 112 keys, its rows see all of those (p counts from kv_lens)
+    for rows, hq in ((1, 4), (40, 8)):
+        c = _case([112], [rows], hq, 2, 64, 16, "bf16", seed=31)
+        c["table"] = c["table"][:, :7].contiguous()
+        all_seen = {**c, "kv_lens": _i32([112])}
+        want, tol = _reference(all_seen, prefix_lens=_i32([112]))   # every row sees the 112 keys
+        got = paged.attention(**{**c, "kv_lens": _i32([10 ** 6])})
+        _within(got, want, tol)
+        got = paged.attention(**{**c, "kv_lens": _i32([2 ** 31 - 1])})
+        _within(got, want, tol)
