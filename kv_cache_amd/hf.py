@@ -341,7 +341,7 @@ class _PagedState:
     def __init__(self, capacity: int, page: int):
         self.capacity, self.page = int(capacity), int(page)
         self.table = self.plan = None
-        self.real = None         # bool [batch, capacity]: columns with a token; None while all have one
+        self.real = None         # bool [batch, capacity]: columns with a token; None while no step had a mask
         self.masks = []          # (mask, window) of the step's layers, compared with what the pages show
         self.length = self.new = 0   # columns stepped, padding included; of the last step
         self.open = False        # an update's columns have not been attended over yet
@@ -363,6 +363,8 @@ class _PagedState:
                                f"{length}, the cache holds {self.length}")
         if first:
             self.masks = []
+            if self.length == 0:
+                self.real = None     # a refused step's, of whatever batch
         # layers share a mask or two: one host read for each in a step
         if attention_mask is not None and not any(m is attention_mask and w == window for m, w in self.masks):
             self._compare(length, n, batch, device, attention_mask, window, first)
@@ -393,36 +395,34 @@ class _PagedState:
                                f"got {mask.dtype} {list(mask.shape)}")
         mask = mask[..., :length].expand(batch, -1, n, -1)
         if self.real is None:
-            real = torch.ones((batch, length), dtype=torch.bool, device=device)
-        else:
-            real = self.real[:, :length].clone()
-        if first:   # padding: a column that its own query does not see
+            self.real = torch.ones((batch, self.capacity), dtype=torch.bool, device=device)
+        real = self.real[:, :length]
+        if first:   # padding: a column that its own query does not see (a refused step's columns are written again)
             own = mask[:, 0, :, length - n:].diagonal(dim1=-2, dim2=-1)
             real[:, length - n:] = own if own.dtype == torch.bool else own == 0
-        fresh = real[:, length - n:]
-        at = torch.arange(length, device=device)
-        token = None if window is None else real.cumsum(-1)   # the window counts tokens, as the pages hold them
-        other = torch.zeros((), dtype=torch.bool, device=device)
+        # the window counts tokens, as the pages hold them
+        token = None if window is None else real.cumsum(-1)
+        at = torch.arange(length, device=device) if n > 1 else None   # a single query is behind all columns
         rows = max(1, (1 << 26) // (batch * mask.size(1) * length))   # bounds what is compared at a time
+        other = []
         for i in range(0, n, rows):
             cols = slice(length - n + i, min(length - n + i + rows, length))
-            seen = real[:, None] & (at <= at[cols, None])
+            seen = real[:, None]
+            if n > 1:
+                seen = seen & (at <= at[cols, None])
             if window is not None:
-                seen &= token[:, None] > token[:, cols, None] - window
+                seen = seen & (token[:, None] > token[:, cols, None] - window)
             seen, m = seen[:, None], mask[:, :, i:i + rows]
-            same = m == seen if m.dtype == torch.bool else torch.where(seen, m == 0, m <= _HIDDEN)
-            other |= (~same & real[:, None, cols, None]).any()
-        order = (fresh[:, :-1] & ~fresh[:, 1:]).any()
-        other, order = torch.stack((other, order)).tolist()
-        if order:
-            raise RuntimeError("paged attention takes left-padded batches (padding before the tokens of a step)")
-        if other:
+            differs = m != seen if m.dtype == torch.bool else torch.where(seen, m != 0, ~(m <= _HIDDEN))
+            other.append((differs & real[:, None, cols, None]).any())
+        if n > 1:
+            fresh = real[:, length - n:]
+            other.append((fresh[:, :-1] & ~fresh[:, 1:]).any())
+            if other.pop():
+                raise RuntimeError("paged attention takes left-padded batches (padding before the tokens of a step)")
+        if other[0] if len(other) == 1 else torch.stack(other).any():
             raise RuntimeError("paged attention takes causal masks, with the layer's sliding window and left padding; "
                                "this mask shows or hides other keys")
-        if first:
-            if self.real is None:
-                self.real = torch.ones((batch, self.capacity), dtype=torch.bool, device=device)
-            self.real[:, length - n:length] = fresh
 
     def reset(self) -> None:
         if self.table is not None and self.length:

@@ -399,6 +399,16 @@ def test_a_refused_first_step_binds_the_cache_to_nothing(taken):
     assert out.shape == (3, 4, 2, 8) and taken == [[4, 4, 4]]
 
 
+def test_a_refused_first_step_of_another_batch(taken):
+    cache = hf.PagedCache(capacity=32, page=16)
+    with pytest.raises(RuntimeError, match="mask"):
+        _attend(cache, _causal([6, 6], 6) | True, 6)
+    k = torch.randn(3, 2, 4, 16)
+    key, value = cache.update(k, k, 0)
+    hf.paged_attention_forward(None, torch.randn(3, 4, 4, 16), key, value, _causal([4, 1, 3], 4))
+    assert taken == [[4, 1, 3]]
+
+
 def test_a_step_that_fails_in_a_later_layer_has_to_be_reset(taken):
     # the layers before hold the step's columns already
     cache = hf.PagedCache(capacity=32, page=16)
