@@ -970,17 +970,22 @@ int64_t qkv_paged_attention_workspace_bytes(int64_t rows, int64_t max_rows, int6
  * dtype for the product with V.  Rows of out outside all requests are left
  * as they were.  Keys whose table entry is not in [0, pages) are not seen;
  * what pages hold behind kv_lens, and infinities and NaN at keys a row does
- * not see, do not reach it.  max_rows: a hint, the largest number of rows a
- * request has (up to 16 * kv_heads / q_heads the call takes fewer launches);
- * the result does not depend on it.  head_dim 64 or 128, at most 128 query
- * heads per KV head; scaling, and softcap where it is not 0, in [2^-60,
- * 2^60]; a table row covers at most 2^30 tokens.  workspace: 16-byte
- * aligned, contents irrelevant; calls sharing one must not overlap in time. */
+ * not see, do not reach it.  first_keys hides a prefix's keys like others:
+ * rows of a later document see a prefix of all documents only with first_keys
+ * 0.  max_rows: a hint, the largest number of rows a request has.  Where its
+ * (row, head) pairs, max_rows * q_heads / kv_heads, are at most 16 or 32 the
+ * call takes smaller tiles, fewer workgroups and a smaller workspace; where it
+ * says less than there is, the result is the same up to its rounding.
+ * head_dim 64 or 128, at most 128 query heads per KV head; scaling, and
+ * softcap where it is not 0, in [2^-60, 2^60]; a table row covers at most
+ * 2^30 tokens.  workspace: 16-byte aligned, contents irrelevant; calls sharing
+ * one must not overlap in time. */
 int qkv_paged_attention(const void* query, const int64_t* q_strides, const void* k_pages, const void* v_pages,
-                        const int64_t* page_strides, int64_t pages, int64_t page, const int32_t* table, int64_t table_ld, int64_t width, int64_t requests,
-                        const int32_t* cu_rows, const int32_t* kv_lens, int64_t rows, int64_t max_rows,
-                        int64_t q_heads, int64_t kv_heads, int64_t head_dim, float scaling, float softcap,
-                        const float* slopes, const int32_t* prefix_lens, const int32_t* first_keys, void* workspace,
+                        const int64_t* page_strides, int64_t pages, int64_t page, const int32_t* table,
+                        int64_t table_ld, int64_t width, int64_t requests, const int32_t* cu_rows,
+                        const int32_t* kv_lens, int64_t rows, int64_t max_rows, int64_t q_heads, int64_t kv_heads,
+                        int64_t head_dim, float scaling, float softcap, const float* slopes,
+                        const int32_t* prefix_lens, const int32_t* first_keys, void* workspace,
                         int64_t workspace_bytes, void* out, const int64_t* out_strides, int dtype, void* stream);
 
 #ifdef __cplusplus

@@ -13,7 +13,7 @@
 // heads: 2.09 ms, 1036 TFLOP/s, 83% of what a large library product reaches); `token` for requests of at most 16 or 32
 // (token, head) rows, whose 4 waves walk different keys of the same rows, bound by memory (32 requests of up to 32768
 // keys: 530 us, 6.14 TB/s).  Requests of 17 to 32 rows in the rows kernel leave three of its waves idle (7 drafts of 5
-// tokens, 4 heads: 70 us, 57 in the token kernel).
+// tokens, 4 heads: 57 us, 47 in the token kernel).
 //
 // Both take the scores transposed, S^T = K Q^T, so that a lane holds scores of one row: the softmax is in-lane but
 // for one lane swap, and P^T leaves the score accumulators in the layout that the matrix instruction of O^T = V^T P^T
@@ -32,6 +32,11 @@ constexpr int kTokenM = 16;    // rows of a column set of the token kernel, whic
 constexpr int kRound = 512;    // workgroups that run at once: two a CU
 constexpr int kRowsJoins = 8, kTokenJoins = 4;   // workgroups that join a tile's parts; of a column set's
 constexpr int kStep = 32;      // keys a wave of the token kernel takes at a time
+// The weights exp(s - m) are rounded to the dtype for the product with V, half a step each (2^-8 in bf16, 2^-11 in
+// fp16): the matrix instruction takes both operands in one 16-bit type, and a second product for what the rounding took
+// would double that half of the matrix work.  The sums are of the rounded weights, so that V is weighted by a partition
+// of one.  Scores, maxima, sums and outputs stay in 32 bits (one token over 500 keys, bf16, against 64 bits: off by 2.8e-4
+// on average, 2.0e-4 with weights in 32 bits; by 6.1e-3 at most either way, the output's own rounding).
 // fp16 weights are scaled by 2^6: they stay below 2^14 (lazy rescaling lets them reach 2^8) and normal down to 2^-20
 // of the row's largest, so that the small weights of long rows keep their bits.
 template <bool F16>
@@ -154,13 +159,12 @@ __device__ __forceinline__ bool locate(const PagedArgs& a, const PagedClass& c, 
   };
   auto round_up = [&](float keys) {
     const int least = max(c.min_keys, static_cast<int>(fminf(keys, 1073741824.0f)) + 1);   // no request has more than 2^30 keys
- 
     return __builtin_amdgcn_readfirstlane((least + kTile - 1) & -kTile);
   };
   // `per` keys for each of the workgroups that run at once.  One round of them is best where it comes out even (one
-  // request of 131011 keys: 94 us, 100 in two rounds).  The last chunks of several requests differ, and a second round
+  // request of 131011 keys: 92 us, 97 in two rounds).  The last chunks of several requests differ, and a second round
   // of a few workgroups costs as much as a full one: then two rounds, or three where chunks stay above 2048 keys (32
-  // requests of up to 32768: 625, 574, 554 us with one, two, three; 8 of up to 16384: three 88, two 85.5).
+  // requests of up to 32768: 574, 543, 527 us with one, two, three; 8 of up to 16384: two 82, three 85).
   auto chunk_of = [&](float per) { return round_up(fmaxf(per * (1.0f / 3.0f), fminf(per * 0.5f, 2048.0f))); };
   auto splits_of = [&](const Share& s, int chunk) { return s.keys > chunk ? (s.keys + chunk - 1) / chunk : 1; };
   int at, part, nt;
@@ -169,8 +173,8 @@ __device__ __forceinline__ bool locate(const PagedArgs& a, const PagedClass& c, 
     const float per = wave_total(static_cast<float>(s.nt) * static_cast<float>(s.keys)) * a.kv_heads * c.per_round;
     w.chunk = round_up(per);
     if (c.finer) {
-      // the shortest chunks, up to a fifth longer, that make one round (4 requests of up to 30000 keys: 60 us, 66 in
-      // two; a third longer, as 32 of up to 32768 would need, 615 instead of 554)
+      // the shortest chunks, up to a fifth longer, that make one round (4 requests of up to 30000 keys: 70 us, 74 in
+      // two; 8 of up to 16384: 77, 80 with chunks that make a little more than one)
       const int tiles = s.nt * a.kv_heads;
       int i = 0;
       for (; i < 4; ++i) {
@@ -298,7 +302,7 @@ __device__ __forceinline__ Row row_of(const PagedArgs& a, const PagedClass& c, c
 
 // cap * tanh(x / cap) in log2 units, of a product q.k.  Near: 1 - 2 / (exp(2x) + 1), in error by 2^-22 of the cap or
 // so, which for caps up to kNearCap is below 2^-14.  For larger ones that error would show, and small x take the odd
-// polynomial (next term x^11 / 113: below 2^-27 of x at 0.25).
+// polynomial (next term x^11 / 113: below 2^-26 of x at 0.25).
 constexpr float kNearCap = 256.0f;
 __device__ __forceinline__ float near_cap(const PagedArgs& a, float qk) {
   const float t = __builtin_amdgcn_exp2f(qk * a.tanh_scale);
@@ -877,8 +881,8 @@ __device__ __forceinline__ void token_body(const PagedArgs& a, const PagedClass&
   };
 
   // A step's loads are issued when those of the step before have landed, and land while that one is computed.  (Issued
-  // before that wait, two steps deep, 32 requests of up to 32768 keys take the same 580 us: eight waves a CU with 16 KB
-  // each on its way are enough.)
+  // before that wait, two steps deep, 32 requests of up to 32768 keys take 547 us instead of 529: eight waves a CU with
+  // 16 KB each on its way are enough.)
   Step x0, x1;
   Entries e;
   uint16_t *vt0 = stage0 + wave * kStep * D, *vt1 = stage1 + wave * kStep * D;
@@ -1064,7 +1068,7 @@ Shape shape_of(bool token, int64_t m, int64_t above, int64_t most, int64_t rows,
   s.cls.tokens = static_cast<int>(m / group);
   s.cls.above = static_cast<int>(above);
   s.cls.most = static_cast<int>(most);
-  // up to 512 keys the launch that joins parts costs more than a split gives (one request of 500 keys: 15.7 us, 20 split)
+  // up to 512 keys the launch that joins parts costs more than a split gives (one request of 500 keys: 12.8 us, 17.1 split)
   s.cls.min_keys = token && max_keys <= 512 ? 512 : 256;
   const int64_t target = token && requests > 1 ? 3 * kRound : kRound;   // the most that chunk_of asks for
   s.cls.per_round = 1.0001f / static_cast<float>(kRound);

@@ -51,7 +51,8 @@ dispatches these modes only for one query per sequence (EV:6236, 6308,
 ``PagedCache`` with the implementation of ``register_paged`` keeps K/V in pages
 (``paged``) and runs prompts, chunks and decode steps densely over them,
 left-padded batches included: padding takes no slot, and every sequence has
-its own length on the GPU.
+its own length on the GPU.  Masks are compared with what the pages show: any
+other than causal with left padding and the layer's window raises.
 
     hf.register_paged()                                   # attn_implementation "paged"
     model.config._attn_implementation = "paged"
@@ -574,8 +575,10 @@ def paged_attention_forward(module, query: torch.Tensor, key: torch.Tensor, valu
                             scaling: float | None = None, dropout: float = 0.0, softcap: float | None = None,
                             sliding_window: int | None = None, **kwargs):
     """HF attention interface (query [B,Hq,n,D]; key/value [B,Hkv,n,D], the new
-    columns a PagedCache layer handed on) -> (out [B,n,Hq,D], None); columns of
-    padding get zeros.  Without a PagedCache: dense SDPA."""
+    columns a PagedCache layer handed on) -> (out [B,n,Hq,D], None).  What
+    columns of padding get is for nobody: zeros before a sequence's first
+    token, attention over its earlier tokens later.  Without a PagedCache:
+    dense SDPA."""
     from transformers.integrations.sdpa_attention import sdpa_attention_forward
 
     layer = getattr(key, "paged_layer", None)
@@ -587,7 +590,7 @@ def paged_attention_forward(module, query: torch.Tensor, key: torch.Tensor, valu
     try:
         _check_interface(module, n, key, attention_mask, dropout, kwargs)
         plan = state.step(layer.length, n, b, query.device, attention_mask, sliding_window)
-    except RuntimeError:
+    except Exception:
         layer.take_back(key.size(2))
         raise
     rows = lambda x: x.transpose(1, 2).reshape(b * n, x.size(1), d)  # noqa: E731  (a view of what projections give)

@@ -25,7 +25,8 @@ captured into a graph and replayed while the requests grow.
 No reference counterpart: the reference keeps HF's dense cache, every
 sequence of a batch at one length, and prefills with dense attention
 (evaluate_qwen3_top2_head_limit3_ppl.py:7079-7111).  Everything runs on the
-GPU on the current stream and raises RuntimeError on bad input.
+GPU on the current stream and raises RuntimeError on bad input.  The pages
+hold no graph: there are no gradients.
 """
 
 from __future__ import annotations
@@ -93,7 +94,9 @@ def plan_step(new_lens: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, f
 
     Rows are packed, ``new_lens[b]`` for each request, or, with ``padded`` =
     n, n for each with its tokens last (a left-padded batch; ``rows`` is then
-    requests * n).  Rows behind the last request's have no token.  A request
+    requests * n).  The rows before them have slot and position -1; over the
+    cache they are queries of the request's earlier tokens, so ``attention``
+    gives zeros only where there are none.  Rows behind the last request's have no token.  A request
     whose tokens do not fit its table row, the pool or ``rows`` is left as it
     is, with kv_lens 0, and counted in ``failed``.  At most 4096 requests,
     2^20 pages, 2^20 rows; ``page`` a power of two in [16, 4096]."""
@@ -240,9 +243,10 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     ``softcap`` > 0 caps scores to softcap * tanh(scaling * q.k / softcap);
     ``slopes`` f32 [Hq] then takes slopes[h] * |p - j| off; ``prefix_lens``
     int32 [requests] opens the first keys to every row; ``first_keys`` int32
-    [rows] hides the keys before a row's document (or window: p + 1 - w).
-    ``max_rows``, the most rows a request has where the caller knows it,
-    spares launches (1 in a decode step); the result does not depend on it.
+    [rows] hides the keys before a row's document (or window: p + 1 - w), a
+    prefix's among them.  ``max_rows``, the most rows a request has where the
+    caller knows it (1 in a decode step), spares workgroups and workspace;
+    saying less than there is changes the result by its rounding at most.
     ``workspace`` (``attention_workspace``) spares an allocation.  Returns
     [rows, Hq, D] in the query's dtype; rows of ``out`` behind the last
     request are left as they were."""
