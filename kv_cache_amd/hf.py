@@ -342,7 +342,7 @@ class _PagedState:
     def __init__(self, capacity: int, page: int):
         self.capacity, self.page = int(capacity), int(page)
         self.table = self.plan = None
-        self.real = None         # bool [batch, capacity]: columns with a token; None while no step had a mask
+        self.real = None         # bool [batch, columns]: those with a token; None while no step had a mask
         self.masks = []          # (mask, window) of the step's layers, compared with what the pages show
         self.length = self.new = 0   # columns stepped, padding included; of the last step
         self.open = False        # an update's columns have not been attended over yet
@@ -371,7 +371,7 @@ class _PagedState:
             self._compare(length, n, batch, device, attention_mask, window, first)
             self.masks.append((attention_mask, window))
         elif first and self.real is not None:
-            self.real[:, length - n:length] = True
+            self.real = torch.cat((self.real[:, :self.length], self.real.new_ones((batch, n))), 1)
         if not first:
             return self.plan
         if self.table is None or (self.length == 0 and self.table.lens.numel() != batch):
@@ -395,12 +395,12 @@ class _PagedState:
             raise RuntimeError(f"paged attention takes bool or additive masks [{batch}, heads, {n}, {length} columns], "
                                f"got {mask.dtype} {list(mask.shape)}")
         mask = mask[..., :length].expand(batch, -1, n, -1)
-        if self.real is None:
-            self.real = torch.ones((batch, self.capacity), dtype=torch.bool, device=device)
-        real = self.real[:, :length]
-        if first:   # padding: a column that its own query does not see (a refused step's columns are written again)
+        real = self.real
+        if real is None:
+            real = torch.ones((batch, length), dtype=torch.bool, device=device)
+        if first:   # padding: a column that its own query does not see
             own = mask[:, 0, :, length - n:].diagonal(dim1=-2, dim2=-1)
-            real[:, length - n:] = own if own.dtype == torch.bool else own == 0
+            real = torch.cat((real[:, :length - n], own if own.dtype == torch.bool else own == 0), 1)
         # the window counts tokens, as the pages hold them
         token = None if window is None else real.cumsum(-1)
         at = torch.arange(length, device=device) if n > 1 else None   # a single query is behind all columns
@@ -424,6 +424,7 @@ class _PagedState:
         if other[0] if len(other) == 1 else torch.stack(other).any():
             raise RuntimeError("paged attention takes causal masks, with the layer's sliding window and left padding; "
                                "this mask shows or hides other keys")
+        self.real = real
 
     def reset(self) -> None:
         if self.table is not None and self.length:
@@ -567,8 +568,8 @@ class _NoBackward(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
-        raise RuntimeError("paged attention has no backward: run the model under torch.no_grad(), or train it without a "
-                           "PagedCache")
+        raise RuntimeError("paged attention has no backward: run the model under torch.no_grad(), or train it without "
+                           "a PagedCache")
 
 
 def paged_attention_forward(module, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, attention_mask,

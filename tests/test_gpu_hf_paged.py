@@ -238,3 +238,19 @@ def test_a_backward_pass_raises():
     logits = model(_tokens(1, 9, 110), past_key_values=hf.PagedCache(capacity=32, page=16), use_cache=True).logits
     with pytest.raises(RuntimeError, match="no backward"):
         logits.float().sum().backward()
+
+
+def test_steps_under_inference_mode_and_outside():
+    hf.register_paged()
+    model = _model(layers=1)
+    model.config._attn_implementation = "paged"
+    ids, mask = _tokens(2, 12, 120), torch.ones((2, 12), dtype=torch.long, device=DEV)
+    mask[1, :4] = 0
+    caches, out = (hf.PagedCache(capacity=32, page=16), hf.PagedCache(capacity=32, page=16)), ([], [])
+    for i, (a, e) in enumerate(((0, 9), (9, 10), (10, 12))):
+        for c, inside, got in zip(caches, (i % 2 == 0, False), out):
+            with torch.inference_mode() if inside else torch.no_grad():
+                got.append(model(ids[:, a:e], attention_mask=mask[:, :e], past_key_values=c, use_cache=True).logits.clone())
+    for x, y in zip(*out):
+        assert torch.equal(x, y)
+    assert caches[0].layers[0].state.table.lens.tolist() == [12, 8]

@@ -448,3 +448,16 @@ def test_a_backward_pass_raises(taken):
     assert torch.equal(got, want)
     with pytest.raises(RuntimeError, match="no backward"):
         got.sum().backward()
+
+
+def test_steps_under_inference_mode_and_outside(monkeypatch):
+    # what the state keeps between steps is not written in place
+    monkeypatch.setattr(paged.PageTable, "step", lambda t, new, rows, padded: new.tolist())
+    state, at = hf._PagedState(32, 16), 0
+    steps = [(_causal([5, 3], 5), 5), (_causal([6, 4], 1, 6), 1), (None, 1), (_causal([9, 7], 2, 9), 2)]
+    for i, (m, n) in enumerate(steps):
+        at += n
+        with torch.inference_mode(i % 2 == 0):
+            got = state.step(at, n, 2, "cpu", m, None)
+        assert got == ([5, 3] if i == 0 else [n, n])
+    assert state.real.tolist() == [[True] * 9, [False] * 2 + [True] * 7]
