@@ -693,3 +693,33 @@ def test_lengths_past_the_table_row_are_its_end():
         _within(got, want, tol)
         got = paged.attention(**{**c, "kv_lens": _i32([2 ** 31 - 1])})
         _within(got, want, tol)
+
+
+@pytest.mark.parametrize("dt,hq,hkv,dim", [("bf16", 8, 2, 128), ("fp16", 6, 2, 64)])
+def test_windows_over_long_caches(dt, hq, hkv, dim):
+    # most parts of the split keys see nothing: single tokens, drafts and chunks, windows across parts' borders
+    kv = [5000, 4097, 3, 2600]
+    for rows in ([1, 1, 1, 1], [4, 2, 3, 5], [150, 1, 3, 40]):
+        c = _case(kv, rows, hq, hkv, dim, 16, dt, seed=32)
+        at = torch.cat([torch.arange(n - m, n) for n, m in zip(kv, rows)])
+        for window in (1, 100, 1024):
+            _check(c, first_keys=(at - (window - 1)).int().to(DEV))
+
+
+def test_short_requests_in_a_wide_table():
+    # the table row covers far more keys than the requests hold
+    kv = [500, 1, 300, 0, 513]
+    c = _case(kv, [1] * 5, 8, 2, 128, 64, "bf16", seed=33)
+    wide = torch.full((5, 640), -1, dtype=torch.int32, device=DEV)
+    wide[:, : c["table"].shape[1]] = c["table"]
+    _check({**c, "table": wide}, max_rows=1)
+    _check({**c, "table": wide})
+
+
+def test_in_place_of_the_query():
+    for kv, rows in (([300, 90], [40, 1]), ([3000, 90], [1, 2]), ([5000], [130])):
+        c = _case(kv, rows, 8, 2, 128, 16, "bf16", seed=34)
+        want = paged.attention(**c)
+        q = c["query"].clone()
+        assert paged.attention(**{**c, "query": q}, out=q) is q
+        assert torch.equal(q, want)
