@@ -32,6 +32,9 @@ extern "C" {
 #define QKV_DTYPE_BF16 0
 #define QKV_DTYPE_FP16 1
 #define QKV_DTYPE_FP32 2
+/* What a code of a quantised page is: e4m3 or e2m1. */
+#define QKV_CODE_FP8 1
+#define QKV_CODE_FP4 2
 
 /* Block-metadata selector kinds (qkv_block_*). */
 #define QKV_BLOCK_QBB 0  /* Quest-style per-block channel min/max bounds */
@@ -987,6 +990,55 @@ int qkv_paged_attention(const void* query, const int64_t* q_strides, const void*
                         int64_t head_dim, float scaling, float softcap, const float* slopes,
                         const int32_t* prefix_lens, const int32_t* first_keys, void* workspace,
                         int64_t workspace_bytes, void* out, const int64_t* out_strides, int dtype, void* stream);
+
+/* Quantised pages: K and V as codes of QKV_CODE_FP8 (e4m3, one byte) or
+ * QKV_CODE_FP4 (e2m1, two channels a byte, the even one in the low half),
+ * with one scale byte s for each 32 channels of a token's head: a code stands
+ * for its value times 2^(s - 127), s = 255 for NaN.  k_pages / v_pages
+ * [pages, kv_heads, page, head_dim or head_dim / 2] bytes with page_strides
+ * {page, head, token}, multiples of 16; k_scales / v_scales [pages, kv_heads,
+ * page, head_dim / 32] bytes with scale_strides {page, head}, the last two
+ * axes without gaps, 4-byte aligned.  K and V share their strides. */
+
+/* qkv_paged_append into quantised pages.  key / value of `dtype` (bf16 or
+ * fp16); head_dim a multiple of 32.  A block's scale is 2^e, e >= -100 the
+ * least with amax <= 464 * 2^e (fp8) or 7 * 2^e (fp4); values are rounded to
+ * the nearest code, halves to the even one.  A magnitude whose code would
+ * stand for more than the dtype holds is stored as 1.875 (fp8) or 1.5 (fp4)
+ * times 2^15 (fp16) or 2^127 (bf16).  A block with an infinity or NaN is
+ * stored as NaN. */
+int qkv_paged_append_codes(const void* key, const int64_t* key_strides, const void* value,
+                           const int64_t* value_strides, void* k_pages, void* v_pages, const int64_t* page_strides,
+                           void* k_scales, void* v_scales, const int64_t* scale_strides, int code, int64_t pages,
+                           int64_t page, int64_t kv_heads, int64_t head_dim, const int64_t* slots, int64_t rows,
+                           int dtype, void* stream);
+
+/* Reads tokens back as rows of `dtype`: row i of request b (cu_rows as in
+ * qkv_paged_plan) is the token at kv_lens[b] - (cu_rows[b+1] - cu_rows[b]) +
+ * i; zeros where the request has none there (before its first, or without a
+ * page in [0, pages)).  Rows outside all requests are left as they were.
+ * code 0 for 16-bit pages (of `dtype`, strides in elements and multiples of
+ * 8; the scales NULL).  key / value [rows, kv_heads, head_dim] with strides
+ * {row, head}, rows 16-byte aligned; head_dim a multiple of 32; at most 2^20
+ * requests. */
+int qkv_paged_read(const void* k_pages, const void* v_pages, const int64_t* page_strides, const void* k_scales,
+                   const void* v_scales, const int64_t* scale_strides, int code, int64_t pages, int64_t page,
+                   int64_t kv_heads, int64_t head_dim, const int32_t* table, int64_t table_ld, int64_t width,
+                   int64_t requests, const int32_t* cu_rows, const int32_t* kv_lens, int64_t rows, void* key,
+                   const int64_t* key_strides, void* value, const int64_t* value_strides, int dtype, void* stream);
+
+/* qkv_paged_attention over quantised pages, of the values that they stand
+ * for in `dtype`, the query's (fp16: values past 65504 are infinities).  The
+ * same workspace. */
+int qkv_paged_attention_codes(const void* query, const int64_t* q_strides, const void* k_pages, const void* v_pages,
+                              const int64_t* page_strides, const void* k_scales, const void* v_scales,
+                              const int64_t* scale_strides, int code, int64_t pages, int64_t page,
+                              const int32_t* table, int64_t table_ld, int64_t width, int64_t requests,
+                              const int32_t* cu_rows, const int32_t* kv_lens, int64_t rows, int64_t max_rows,
+                              int64_t q_heads, int64_t kv_heads, int64_t head_dim, float scaling, float softcap,
+                              const float* slopes, const int32_t* prefix_lens, const int32_t* first_keys,
+                              void* workspace, int64_t workspace_bytes, void* out, const int64_t* out_strides,
+                              int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -149,6 +149,12 @@ _PROTOTYPES = {
     "qkv_paged_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64,
                                    _i64, _i64, _i64, _i64, _f32, _f32, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i32,
                                    _vp]),
+    "qkv_paged_append_codes": (_i32, [_vp] * 10 + [_i32, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _vp]),
+    "qkv_paged_read": (_i32, [_vp] * 6 + [_i32, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp,
+                              _vp, _vp, _i32, _vp]),
+    "qkv_paged_attention_codes": (_i32, [_vp] * 8 + [_i32, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64,
+                                                     _i64, _i64, _f32, _f32, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i32,
+                                                     _vp]),
 }
 
 _LIB = None

@@ -190,11 +190,71 @@ def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, tup
     return code, k_pages.stride(), v_pages.stride()
 
 
+# Quantised pages: codes of 8 bits (e4m3) or of 4 (e2m1, two to a byte, the even channel in the low half), and one scale
+# byte s for each 32 channels of a token's head, under which a code stands for its value times 2^(s - 127).
+_CODES = {torch.float8_e4m3fn: 1, torch.uint8: 2}
+_BLOCK = 32
+_HALF = (torch.bfloat16, torch.float16)
+
+
+def quantized_pages(pages: int, kv_heads: int, page: int, head_dim: int, kind: str,
+                    device) -> tuple[torch.Tensor, torch.Tensor]:
+    """Quantised pages of K or of V for a layer, and their scales: ``kind``
+    "fp8" (float8_e4m3fn [pages, Hkv, page, D]) or "fp4" (uint8 [pages, Hkv,
+    page, D / 2]), scales uint8 [pages, Hkv, page, D / 32]; contents as the
+    allocator gives them."""
+    _require(kind in ("fp8", "fp4"), f"kind must be fp8 or fp4, got {kind!r}")
+    _require(head_dim % _BLOCK == 0, f"head_dim must be a multiple of {_BLOCK}, got {head_dim}")
+    scales = torch.empty((pages, kv_heads, page, head_dim // _BLOCK), dtype=torch.uint8, device=device)
+    if kind == "fp8":
+        return scales.new_empty((pages, kv_heads, page, head_dim), dtype=torch.float8_e4m3fn), scales
+    return scales.new_empty((pages, kv_heads, page, head_dim // 2)), scales
+
+
+def _check_codes(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales, v_scales) -> tuple[int, int, tuple, tuple]:
+    """(code, head dim, strides of the pages, strides of the scales) of a
+    layer's quantised pages, checked."""
+    code = _CODES.get(k_pages.dtype)
+    if code is None:
+        raise RuntimeError(f"quantised pages must be float8_e4m3fn or uint8, got {k_pages.dtype}")
+    if (not k_pages.is_cuda or k_pages.dim() != 4 or k_pages.shape != v_pages.shape
+            or v_pages.dtype is not k_pages.dtype or v_pages.get_device() != k_pages.get_device()):
+        raise RuntimeError("k_pages and v_pages must be CUDA [pages, kv_heads, page, dim] of one shape, dtype and "
+                           "device with contiguous channels")
+    ps = k_pages.stride()
+    if ps != v_pages.stride() or ps[3] != 1:
+        raise RuntimeError("k_pages and v_pages must have the same strides, with contiguous channels")
+    pages, heads, page, dim = k_pages.shape
+    dim *= code   # two to a byte
+    shape = (pages, heads, page, dim // _BLOCK)
+    if dim % _BLOCK or k_scales is None or v_scales is None:
+        raise RuntimeError(f"quantised pages have k_scales and v_scales and a multiple of {_BLOCK} channels")
+    ss = k_scales.stride()
+    for t in (k_scales, v_scales):
+        if (t.dtype is not torch.uint8 or t.shape != shape or t.get_device() != k_pages.get_device()
+                or t.stride() != ss or ss[3] != 1 or ss[2] != shape[3]):
+            raise RuntimeError(f"k_scales and v_scales must be uint8 {list(shape)} on {k_pages.device} of the same "
+                               "strides, a head's tokens without gaps")
+    return code, dim, ps, ss
+
+
 def append(key: torch.Tensor, value: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
-           slots: torch.Tensor) -> None:
+           slots: torch.Tensor, *, k_scales: torch.Tensor | None = None,
+           v_scales: torch.Tensor | None = None) -> None:
     """Writes the rows' K and V, [rows, Hkv, D] at any strides with contiguous
     channels, to their ``slots`` (int64 [rows], as ``plan_step`` gives them;
-    a row with -1 is skipped, no slot may come twice)."""
+    a row with -1 is skipped, no slot may come twice).
+
+    Into quantised pages (``quantized_pages``, with their scales), bf16 or
+    fp16 rows are rounded to the nearest code, halves to the even one, under
+    the smallest power of two (from 2^-100 on) that keeps a block's largest
+    magnitude within half a step: an fp8 value is off by at most 2^-4 of
+    itself or 2^-10 of the scale, an fp4 one by 2^-2 or 2^-2.  A block with an
+    infinity or NaN is stored as NaN; magnitudes that would read back as more
+    than the dtype holds (fp16 over 61440, in fp4 over 49152) are stored as
+    that."""
+    if k_scales is not None or v_scales is not None or k_pages.dtype in _CODES:
+        return _append_codes(key, value, k_pages, v_pages, slots, k_scales, v_scales)
     lib = _lib.load()
     _, ks, vs = _check_pages(k_pages, v_pages)
     pages, heads, page, dim = k_pages.shape
@@ -219,6 +279,82 @@ def append(key: torch.Tensor, value: torch.Tensor, k_pages: torch.Tensor, v_page
     _lib.check(rc)
 
 
+def _append_codes(key, value, k_pages, v_pages, slots, k_scales, v_scales) -> None:
+    lib = _lib.load()
+    code, dim, ps, ss = _check_codes(k_pages, v_pages, k_scales, v_scales)
+    pages, heads, page, _ = k_pages.shape
+    idx = k_pages.get_device()
+    rows = slots.numel()
+    _check_slots(slots, rows, idx)
+    dtype = _lib.half_code("key", key)
+    for name, t in (("key", key), ("value", value)):
+        if t.shape != (rows, heads, dim) or t.dtype is not key.dtype or t.get_device() != idx or t.stride(2) != 1:
+            raise RuntimeError(f"{name} must be {key.dtype} [{rows}, {heads}, {dim}] on {k_pages.device} with "
+                               "contiguous channels: key, value and slots have as many rows")
+    # row and head strides of the rows, page, head and token strides of the pages, page and head strides of the scales
+    st = _lib.strides(*key.stride()[:2], *value.stride()[:2], *ps[:3], *ss[:2])
+    at = ctypes.addressof(st)
+    guard = _lib.enter_device(idx)
+    try:
+        rc = lib.qkv_paged_append_codes(key.data_ptr(), at, value.data_ptr(), at + 16, k_pages.data_ptr(),
+                                        v_pages.data_ptr(), at + 32, k_scales.data_ptr(), v_scales.data_ptr(), at + 56,
+                                        code, pages, page, heads, dim, slots.data_ptr(), rows, dtype,
+                                        _lib.stream_on(idx))
+    finally:
+        _lib.leave_device(guard)
+    _lib.check(rc)
+
+
+def read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, cu_rows: torch.Tensor,
+         kv_lens: torch.Tensor, rows: int, *, k_scales: torch.Tensor | None = None,
+         v_scales: torch.Tensor | None = None, dtype: torch.dtype | None = None,
+         out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """K and V of cached tokens, [rows, Hkv, D] each: row i of request b is
+    the token at kv_lens[b] - (cu_rows[b + 1] - cu_rows[b]) + i, so that
+    cu_rows = the sums of kv_lens reads whole requests; zeros where a request
+    has no token.  Quantised pages give ``dtype`` (bf16 if not said), which
+    holds what they stand for without a rounding (fp16 below 2^-14 with fewer
+    bits, and infinities past 65504); others their own.  Rows of ``out`` (two
+    tensors, any row and head strides of 16 bytes) behind the last request are
+    left as they were."""
+    lib = _lib.load()
+    if k_scales is not None or v_scales is not None or k_pages.dtype in _CODES:
+        code, dim, ps, ss = _check_codes(k_pages, v_pages, k_scales, v_scales)
+        dtype = torch.bfloat16 if dtype is None else dtype
+        _require(dtype in _HALF, f"dtype must be bfloat16 or float16, got {dtype}")
+    else:
+        _, ps, vs = _check_pages(k_pages, v_pages)
+        _require(vs == ps, "k_pages and v_pages must have the same strides")
+        _require(dtype is None or dtype is k_pages.dtype, f"pages of {k_pages.dtype} are not read as {dtype}")
+        code, dim, ss, dtype = 0, k_pages.size(3), (0, 0), k_pages.dtype
+    pages, heads, page, _ = k_pages.shape
+    idx, n, width, ld = _check_table(table)
+    _require(k_pages.get_device() == idx, f"table must be on {k_pages.device}")
+    _i32("cu_rows", cu_rows, n + 1, idx)
+    _i32("kv_lens", kv_lens, n, idx)
+    _require(rows >= 0, "rows must not be negative")
+    if out is None:
+        key = torch.empty((rows, heads, dim), dtype=dtype, device=k_pages.device)
+        value = torch.empty_like(key)
+    else:
+        key, value = out
+        for t in out:
+            _require(t.shape == (rows, heads, dim) and t.dtype is dtype and t.get_device() == idx and t.stride(2) == 1,
+                     f"out must be two {dtype} [{rows}, {heads}, {dim}] on {k_pages.device} with contiguous channels")
+    st = _lib.strides(*ps[:3], *ss[:2], *key.stride()[:2], *value.stride()[:2])
+    at = ctypes.addressof(st)
+    guard = _lib.enter_device(idx)
+    try:
+        rc = lib.qkv_paged_read(k_pages.data_ptr(), v_pages.data_ptr(), at, _lib.ptr(k_scales), _lib.ptr(v_scales),
+                                at + 24, code, pages, page, heads, dim, table.data_ptr(), ld, width, n,
+                                cu_rows.data_ptr(), kv_lens.data_ptr(), rows, key.data_ptr(), at + 40,
+                                value.data_ptr(), at + 56, _lib.DTYPE_CODES[dtype], _lib.stream_on(idx))
+    finally:
+        _lib.leave_device(guard)
+    _lib.check(rc)
+    return key, value
+
+
 def attention_workspace(rows: int, max_rows: int, requests: int, width: int, page: int, q_heads: int, kv_heads: int,
                         head_dim: int, device) -> torch.Tensor:
     """A workspace for ``attention`` calls of these sizes (contents
@@ -233,7 +369,8 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
               cu_rows: torch.Tensor, kv_lens: torch.Tensor, scaling: float, *, max_rows: int | None = None,
               softcap: float = 0.0, slopes: torch.Tensor | None = None, prefix_lens: torch.Tensor | None = None,
               first_keys: torch.Tensor | None = None, out: torch.Tensor | None = None,
-              workspace: torch.Tensor | None = None) -> torch.Tensor:
+              workspace: torch.Tensor | None = None, k_scales: torch.Tensor | None = None,
+              v_scales: torch.Tensor | None = None) -> torch.Tensor:
     """query [rows, Hq, D] over the cached keys of the rows' requests, whose
     own K and V were appended before.  Row i of request b is the token at
     p = kv_lens[b] - (cu_rows[b + 1] - cu_rows[b]) + i and sees the keys j
@@ -247,20 +384,29 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     prefix's among them.  ``max_rows``, the most rows a request has where the
     caller knows it (1 in a decode step), spares workgroups and workspace;
     saying less than there is changes the result by its rounding at most.
-    ``workspace`` (``attention_workspace``) spares an allocation.  Returns
-    [rows, Hq, D] in the query's dtype; rows of ``out`` behind the last
-    request are left as they were."""
+    ``workspace`` (``attention_workspace``) spares an allocation.  Quantised
+    pages come with ``k_scales`` and ``v_scales`` (``quantized_pages``) and
+    are attended to as the values of the query's dtype that they stand for.
+    Returns [rows, Hq, D] in the query's dtype; rows of ``out`` behind the
+    last request are left as they were."""
     lib = _lib.load()
-    code, ks, vs = _check_pages(k_pages, v_pages)
+    if k_scales is not None or v_scales is not None or k_pages.dtype in _CODES:
+        code, dim, ks, ss = _check_codes(k_pages, v_pages, k_scales, v_scales)
+        dtype = _lib.half_code("query", query)
+    else:
+        dtype, ks, vs = _check_pages(k_pages, v_pages)
+        if vs != ks:
+            raise RuntimeError("k_pages and v_pages must have the same strides")
+        if query.dtype is not k_pages.dtype:
+            raise RuntimeError(f"query must be {k_pages.dtype} [rows, q_heads, dim] on {k_pages.device} with contiguous "
+                               "channels")
+        code, dim, ss = 0, k_pages.size(3), (0, 0)
     idx, n, width, ld = _check_table(table)
-    pages, kv_heads, page, dim = k_pages.shape
+    pages, kv_heads, page, _ = k_pages.shape
     if k_pages.get_device() != idx:
         raise RuntimeError(f"table must be on {k_pages.device}")
-    if vs != ks:
-        raise RuntimeError("k_pages and v_pages must have the same strides")
-    if (query.dim() != 3 or query.dtype is not k_pages.dtype or query.get_device() != idx or query.stride(2) != 1
-            or query.size(2) != dim):
-        raise RuntimeError(f"query must be {k_pages.dtype} [rows, q_heads, {dim}] on {k_pages.device} with contiguous "
+    if query.dim() != 3 or query.get_device() != idx or query.stride(2) != 1 or query.size(2) != dim:
+        raise RuntimeError(f"query must be {query.dtype} [rows, q_heads, {dim}] on {k_pages.device} with contiguous "
                            "channels")
     rows, q_heads, _ = query.shape
     _i32("cu_rows", cu_rows, n + 1, idx)
@@ -288,17 +434,24 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         _require(workspace.get_device() == idx and workspace.is_contiguous(),
                  f"workspace must be contiguous on cuda:{idx}")
         ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    # row and head strides of the query, page, head and token strides of the pages, row and head strides of out
-    st = _lib.strides(*query.stride()[:2], *ks[:3], *out.stride()[:2])
+    # row and head strides of the query, page, head and token strides of the pages, row and head strides of out, page
+    # and head strides of the scales
+    st = _lib.strides(*query.stride()[:2], *ks[:3], *out.stride()[:2], *ss[:2])
     at = ctypes.addressof(st)
+    # what the three calls share, before and behind the pages' own
+    rest = (pages, page, table.data_ptr(), ld, width, n, cu_rows.data_ptr(), kv_lens.data_ptr(), rows, most, q_heads,
+            kv_heads, dim, scaling, softcap, None if slopes is None else slopes.data_ptr(),
+            None if prefix_lens is None else prefix_lens.data_ptr(),
+            None if first_keys is None else first_keys.data_ptr(), ws_ptr, ws_bytes, out.data_ptr(), at + 40, dtype)
     guard = _lib.enter_device(idx)
     try:
-        rc = lib.qkv_paged_attention(
-            query.data_ptr(), at, k_pages.data_ptr(), v_pages.data_ptr(), at + 16, pages, page, table.data_ptr(), ld,
-            width, n, cu_rows.data_ptr(), kv_lens.data_ptr(), rows, most, q_heads, kv_heads, dim, scaling, softcap,
-            None if slopes is None else slopes.data_ptr(), None if prefix_lens is None else prefix_lens.data_ptr(),
-            None if first_keys is None else first_keys.data_ptr(), ws_ptr, ws_bytes, out.data_ptr(), at + 40, code,
-            _lib.stream_on(idx))
+        if code:
+            rc = lib.qkv_paged_attention_codes(query.data_ptr(), at, k_pages.data_ptr(), v_pages.data_ptr(), at + 16,
+                                               k_scales.data_ptr(), v_scales.data_ptr(), at + 56, code, *rest,
+                                               _lib.stream_on(idx))
+        else:
+            rc = lib.qkv_paged_attention(query.data_ptr(), at, k_pages.data_ptr(), v_pages.data_ptr(), at + 16, *rest,
+                                         _lib.stream_on(idx))
     finally:
         _lib.leave_device(guard)
     _lib.check(rc)
