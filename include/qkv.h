@@ -1040,6 +1040,45 @@ int qkv_paged_attention_codes(const void* query, const int64_t* q_strides, const
                               void* workspace, int64_t workspace_bytes, void* out, const int64_t* out_strides,
                               int dtype, void* stream);
 
+/* Words of the plan that qkv_paged_share writes; -1 for sizes it does not
+ * take. */
+int64_t qkv_paged_share_words(int64_t rows, int64_t requests);
+
+/* A step whose requests may continue the tokens of another one, their parent:
+ * parents int32 [requests], a request of the same page table or anything
+ * outside [0, requests) for none; lens int32 [requests], the tokens that
+ * requests hold as parents.  A request with tokens (kv_lens[b] > 0) then
+ * stands behind all lens[parents[b]] tokens of its parent (one without any,
+ * and the request itself, are none; a parent's own parent does not count).
+ * shared int32 [qkv_paged_share_words] receives the rows gathered by parent;
+ * its first `rows` words are the rows' positions, with the parent's tokens
+ * before a request's own (-1 for rows without a token).  cu_rows, kv_lens as
+ * in qkv_paged_plan, cu_rows ascending.  At most 4096 requests, 2^20 rows. */
+int qkv_paged_share(const int32_t* parents, const int32_t* cu_rows, const int32_t* kv_lens, const int32_t* lens,
+                    int64_t requests, int64_t rows, int32_t* shared, void* stream);
+
+/* Bytes of workspace for qkv_paged_attention_shared; -1 for sizes it does not
+ * take. */
+int64_t qkv_paged_attention_shared_workspace_bytes(int64_t rows, int64_t max_rows, int64_t requests, int64_t width,
+                                                   int64_t page, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
+
+/* qkv_paged_attention (code 0) or qkv_paged_attention_codes of such a step,
+ * `shared` its plan for the same cu_rows, kv_lens, rows and requests.  With n
+ * = its parent's tokens, row i of request b is the token at p = n +
+ * kv_lens[b] - (cu_rows[b+1] - cu_rows[b]) + i of the parent's tokens and its
+ * own behind them, and sees the keys first_keys[row] <= j < max(p + 1,
+ * prefix_lens[b]) of them; rows before its own first token, and rows that see
+ * none, get zeros.  A parent's keys are read once for all rows behind it. */
+int qkv_paged_attention_shared(const void* query, const int64_t* q_strides, const void* k_pages, const void* v_pages,
+                               const int64_t* page_strides, const void* k_scales, const void* v_scales,
+                               const int64_t* scale_strides, int code, const int32_t* shared, int64_t pages,
+                               int64_t page, const int32_t* table, int64_t table_ld, int64_t width,
+                               int64_t requests, const int32_t* cu_rows, const int32_t* kv_lens, int64_t rows,
+                               int64_t max_rows, int64_t q_heads, int64_t kv_heads, int64_t head_dim, float scaling,
+                               float softcap, const float* slopes, const int32_t* prefix_lens,
+                               const int32_t* first_keys, void* workspace, int64_t workspace_bytes, void* out,
+                               const int64_t* out_strides, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

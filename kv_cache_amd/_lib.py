@@ -155,6 +155,12 @@ _PROTOTYPES = {
     "qkv_paged_attention_codes": (_i32, [_vp] * 8 + [_i32, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64,
                                                      _i64, _i64, _f32, _f32, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i32,
                                                      _vp]),
+    "qkv_paged_share_words": (_i64, [_i64, _i64]),
+    "qkv_paged_share": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp]),
+    "qkv_paged_attention_shared_workspace_bytes": (_i64, [_i64] * 8),
+    "qkv_paged_attention_shared": (_i32, [_vp] * 8 + [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64,
+                                                      _i64, _i64, _i64, _f32, _f32, _vp, _vp, _vp, _vp, _i64, _vp, _vp,
+                                                      _i32, _vp]),
 }
 
 _LIB = None

@@ -5,14 +5,15 @@
 // entries, top last.  A step adds new_lens[b] tokens to every request; its rows lie one request after another (packed,
 // or `padded` rows each with the tokens at the end).  All of it is decided here from the lengths on the GPU, so that a
 // step can be captured and needs no length on the host.
-#include "common.h"
+#include "paged_tiles.h"
 
 namespace qkv {
 namespace {
 
-constexpr int kMaxRequests = 4096;   // a request's four words of step state lie in LDS (64 KB)
+// a request's four words of step state lie in LDS (64 KB); sums over kPlanThreads of pages, or rows, fit an int
+constexpr int kMaxRequests = kMaxPlanned;
 constexpr int kPlanThreads = 1024;
-constexpr int64_t kMaxCount = 1 << 20;   // pages, and rows of a step: sums over kPlanThreads of them fit an int
+constexpr int64_t kMaxCount = kMaxPlannedRows;
 
 __device__ __forceinline__ int ceil_pages(int64_t tokens, int shift) {
   return static_cast<int>((tokens + ((1 << shift) - 1)) >> shift);
@@ -211,6 +212,126 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(ReleaseArgs a) {
   }
 }
 
+struct ShareArgs {
+  const int32_t *parents, *cu, *kv_lens, *lens;
+  int requests, rows;
+  SharedPlan p;
+};
+constexpr uint32_t kNobody = 0xFFFFFFFFu;
+
+// Request b's parent, or -1; its rows, and how many of them, the last ones, have a token.
+struct Heir {
+  int parent, end, rows, tokens;
+};
+__device__ __forceinline__ Heir heir_of(const ShareArgs& a, int b) {
+  const int row0 = min(max(a.cu[b], 0), a.rows);
+  Heir h;
+  h.end = min(max(a.cu[b + 1], row0), a.rows);
+  h.rows = h.end - row0;
+  h.tokens = min(h.rows, max(a.kv_lens[b], 0));
+  h.parent = a.parents[b];
+  // a parent without tokens is none, nor is a request's own
+  if (static_cast<unsigned>(h.parent) >= static_cast<unsigned>(a.requests) || h.parent == b || a.lens[h.parent] <= 0 ||
+      a.kv_lens[b] <= 0)
+    h.parent = -1;
+  return h;
+}
+
+// What is known of a row: its position, its place among its parent's heirs, the heir at that place.
+__device__ __forceinline__ void put_shared_row(const ShareArgs& a, const int* cu, int row) {
+  int pos = -1, rank = -2;
+  const int b = last_at_most(cu, a.requests - 1, row);
+  if (row >= cu[0] && row < cu[a.requests]) {
+    const Heir h = heir_of(a, b);
+    rank = -1;
+    const int nth = row - (h.end - h.tokens);
+    if (nth >= 0 && row < h.end) {
+      pos = a.p.before[b] + max(a.kv_lens[b], 0) - (h.end - row);
+      if (h.parent >= 0 && a.p.starts[b] + nth < a.rows) {   // always so where cu_rows ascends
+        rank = a.p.starts[b] + nth;
+        a.p.order[rank] = row;
+      }
+    }
+  }
+  a.p.positions[row] = pos;
+  a.p.rank[row] = rank;
+}
+
+// One workgroup sorts the requests by parent, then by themselves (keys differ, so the order is one whatever runs first),
+// and prefix sums of their tokens give every heir its place.
+template <bool WITH_ROWS>
+__global__ __launch_bounds__(kPlanThreads) void share_kernel(ShareArgs a) {
+  __shared__ uint32_t s_key[kMaxRequests];
+  __shared__ int s_start[kMaxRequests], s_cu[kMaxRequests + 1];
+  __shared__ int part[2 * kPlanThreads / 64];
+  const int tid = threadIdx.x;
+  int n = 1;
+  while (n < a.requests) n <<= 1;
+  for (int b = tid; b < n; b += kPlanThreads) {
+    uint32_t key = kNobody;
+    if (b < a.requests) {
+      const Heir h = heir_of(a, b);
+      if (h.parent >= 0 && h.tokens > 0) key = static_cast<uint32_t>(h.parent) << 12 | static_cast<uint32_t>(b);
+      s_cu[b] = h.end - h.rows;
+      if (b == a.requests - 1) s_cu[a.requests] = h.end;
+      a.p.before[b] = h.parent >= 0 ? a.lens[h.parent] : 0;
+      a.p.parent_lens[b] = max(a.lens[b], 0);
+      a.p.starts[b] = 0;
+    }
+    s_key[b] = key;
+  }
+  __syncthreads();
+  for (int k = 2; k <= n; k <<= 1)   // bitonic: ascending runs of k keys
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int i = tid; i < n; i += kPlanThreads) {
+        const int other = i ^ j;
+        if (other > i) {
+          const uint32_t x = s_key[i], y = s_key[other];
+          if ((x > y) == ((i & k) == 0)) {
+            s_key[i] = y;
+            s_key[other] = x;
+          }
+        }
+      }
+      __syncthreads();
+    }
+  int carry = 0;
+  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    const uint32_t key = i < n ? s_key[i] : kNobody;
+    const int b = static_cast<int>(key & 4095u);
+    const int m = key == kNobody ? 0 : heir_of(a, b).tokens;
+    int up = m, none = 0, tot, tot_none;
+    block_scan2(up, none, tot, tot_none, part);
+    if (i < n) s_start[i] = carry + up - m;
+    if (key != kNobody) a.p.starts[b] = carry + up - m;
+    carry += tot;
+  }
+  __syncthreads();
+  for (int p = tid; p <= a.requests; p += kPlanThreads) {
+    int lo = 0, hi = n;   // the first key of parent p or a later one
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (s_key[mid] != kNobody && s_key[mid] >> 12 < static_cast<uint32_t>(p)) lo = mid + 1;
+      else hi = mid;
+    }
+    a.p.heirs_cu[p] = lo < n && s_key[lo] != kNobody ? s_start[lo] : carry;
+  }
+  if constexpr (WITH_ROWS) {
+    __threadfence_block();
+    __syncthreads();   // before and starts, which this workgroup wrote
+    for (int row = tid; row < a.rows; row += kPlanThreads) put_shared_row(a, s_cu, row);
+  }
+}
+
+__global__ __launch_bounds__(256) void share_rows_kernel(ShareArgs a) {
+  __shared__ int s_cu[kMaxRequests + 1];
+  for (int i = threadIdx.x; i <= a.requests; i += 256) s_cu[i] = min(max(a.cu[i], 0), a.rows);
+  __syncthreads();
+  const int row = blockIdx.x * 256 + threadIdx.x;
+  if (row < a.rows) put_shared_row(a, s_cu, row);
+}
+
 struct AppendArgs {
   const uint16_t *k, *v;
   uint16_t *kp, *vp;
@@ -327,5 +448,29 @@ QKV_EXPORT int qkv_paged_append(const void* key, const int64_t* key_strides, con
   // a grid has less than 2^32 threads
   if (grid >= (1 << 24)) return fail(QKV_ERR_UNSUPPORTED, "%s: too many rows", what);
   append_kernel<<<static_cast<unsigned>(grid), 256, 0, static_cast<hipStream_t>(stream)>>>(a);
+  return check_launch(what);
+}
+
+QKV_EXPORT int64_t qkv_paged_share_words(int64_t rows, int64_t requests) {
+  if (rows < 1 || rows > kMaxCount || requests < 1 || requests > kMaxRequests) return -1;
+  return SharedPlan::words(rows, requests);
+}
+
+QKV_EXPORT int qkv_paged_share(const int32_t* parents, const int32_t* cu_rows, const int32_t* kv_lens,
+                               const int32_t* lens, int64_t requests, int64_t rows, int32_t* shared, void* stream) {
+  const char* what = "qkv_paged_share";
+  if (!parents || !cu_rows || !kv_lens || !lens || !shared) return fail(QKV_ERR_INVALID, "%s: null pointer", what);
+  if (qkv_paged_share_words(rows, requests) < 0)
+    return fail(QKV_ERR_UNSUPPORTED, "%s: 1 to %d requests and 1 to %lld rows, got %lld and %lld", what, kMaxRequests,
+                static_cast<long long>(kMaxCount), static_cast<long long>(requests), static_cast<long long>(rows));
+  ShareArgs a{parents, cu_rows, kv_lens, lens, static_cast<int>(requests), static_cast<int>(rows),
+              SharedPlan(shared, rows, requests)};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (rows <= kPlanRowsInOne) {
+    share_kernel<true><<<1, kPlanThreads, 0, st>>>(a);
+  } else {
+    share_kernel<false><<<1, kPlanThreads, 0, st>>>(a);
+    share_rows_kernel<<<static_cast<unsigned>(cdiv(rows, 256)), 256, 0, st>>>(a);
+  }
   return check_launch(what);
 }

@@ -7,6 +7,22 @@
 
 namespace qkv {
 
+constexpr int kMaxPlanned = 4096;             // requests of a planned step
+constexpr int64_t kMaxPlannedRows = 1 << 20;   // and its rows (or pages)
+
+// The rows of requests that continue another request's tokens, their parent's, gathered by parent (paged.hip writes it,
+// int32 words from one address).  Row order[i] of heirs_cu[a] <= i < heirs_cu[a + 1] is a's heir and sees its
+// parent_lens[a] tokens; rank is order's inverse (-1: a row without a parent or token, -2: no request's row).  before[b]
+// tokens come before request b's own, so that its row is at positions[row] (-1 without a token).  starts[b]: the place
+// of b's first heir.
+struct SharedPlan {
+  int32_t *positions, *rank, *order, *heirs_cu, *starts, *parent_lens, *before;
+  SharedPlan(int32_t* at, int64_t rows, int64_t requests)
+      : positions(at), rank(at + rows), order(at + 2 * rows), heirs_cu(at + 3 * rows), starts(heirs_cu + requests + 1),
+        parent_lens(starts + requests), before(parent_lens + requests) {}
+  static int64_t words(int64_t rows, int64_t requests) { return 3 * rows + 4 * requests + 1; }
+};
+
 // A call of the attention over pages as the C interface takes it.
 struct PagedCall {
   const void* query;
@@ -33,6 +49,8 @@ struct PagedCall {
 // Over codes: the kernels of each format are compiled in a file of their own.
 int paged_call_fp8(const PagedCall& c, const char* what);
 int paged_call_fp4(const PagedCall& c, const char* what);
+int shared_call_fp8(const PagedCall& c, const int32_t* plan, const char* what);
+int shared_call_fp4(const PagedCall& c, const int32_t* plan, const char* what);
 
 namespace {
 
@@ -80,10 +98,9 @@ struct PagedArgs {
   int wide;                                 // the cap is larger than kNearCap
   const uint8_t *k_scales, *v_scales;       // of codes: [pages][head][token][block], the last two without gaps
   int64_t s_page, s_head;                   // their strides
-  // Requests that continue another's tokens: the heirs of request a are rows order[heirs_cu[a] .. heirs_cu[a+1]-1] and
-  // see its parent_lens[a] first keys; before[b] is how many a request's own tokens come behind, positions[row] where a
-  // row then is.  at: for every (row, KV head), then for every (place in order, KV head), where its parts lie.
-  const int32_t *order, *heirs_cu, *parent_lens, *before, *positions;
+  // Requests that continue another's tokens (SharedPlan).  at: for every (row, KV head), then for every (place in order,
+  // KV head), where its parts lie.
+  const int32_t *order, *rank, *heirs_cu, *parent_lens, *before, *positions;
   int2* at;
 };
 

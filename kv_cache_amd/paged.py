@@ -190,6 +190,53 @@ def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, tup
     return code, k_pages.stride(), v_pages.stride()
 
 
+class SharedRows:
+    """What ``share_rows`` decides of a step, one int32 ``buffer`` for all of
+    it; ``positions`` [rows] is where each row's token is, its parent's
+    tokens before its request's own (-1 where a row has no token)."""
+
+    __slots__ = ("buffer", "rows", "requests", "positions")
+
+    def __init__(self, requests: int, rows: int, device):
+        words = _lib.load().qkv_paged_share_words(rows, requests)
+        _require(words >= 0, f"share_rows takes 1 to 4096 requests and 1 to 2^20 rows, got {requests} and {rows}")
+        self.buffer = torch.empty(words, dtype=torch.int32, device=device)
+        self.rows, self.requests, self.positions = rows, requests, self.buffer[:rows]
+
+
+def share_rows(parents: torch.Tensor, cu_rows: torch.Tensor, kv_lens: torch.Tensor, lens: torch.Tensor, rows: int, *,
+               out: SharedRows | None = None) -> SharedRows:
+    """Of a step whose requests may continue the tokens of another one: the
+    rows gathered by parent, for ``attention(..., shared=...)`` of every
+    layer.  ``parents`` int32 [requests] is each request's parent, a request
+    of the same page table, or -1; ``lens`` int32 [requests] the tokens that
+    requests hold as parents (``PageTable.lens``); ``cu_rows`` and ``kv_lens``
+    are the step's (``plan_step``).  A request then stands behind all tokens
+    of its parent, wherever their last page ends; its own pages hold only its
+    own tokens.  The parent's own parent does not count.  Release a parent
+    after its last child."""
+    lib = _lib.load()
+    _require(parents.is_cuda, "parents must be CUDA")
+    n, idx = parents.numel(), parents.get_device()
+    _i32("parents", parents, n, idx)
+    _i32("cu_rows", cu_rows, n + 1, idx)
+    _i32("kv_lens", kv_lens, n, idx)
+    _i32("lens", lens, n, idx)
+    if out is None:
+        out = SharedRows(n, rows, parents.device)
+    else:
+        _require(out.rows == rows and out.requests == n and out.buffer.get_device() == idx,
+                 f"out must be SharedRows({n}, {rows}) on cuda:{idx}")
+    guard = _lib.enter_device(idx)
+    try:
+        rc = lib.qkv_paged_share(parents.data_ptr(), cu_rows.data_ptr(), kv_lens.data_ptr(), lens.data_ptr(), n, rows,
+                                 out.buffer.data_ptr(), _lib.stream_on(idx))
+    finally:
+        _lib.leave_device(guard)
+    _lib.check(rc)
+    return out
+
+
 # Quantised pages: codes of 8 bits (e4m3) or of 4 (e2m1, two to a byte, the even channel in the low half), and one scale
 # byte s for each 32 channels of a token's head, under which a code stands for its value times 2^(s - 127).
 _CODES = {torch.float8_e4m3fn: 1, torch.uint8: 2}
@@ -356,11 +403,13 @@ def read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, cu_r
 
 
 def attention_workspace(rows: int, max_rows: int, requests: int, width: int, page: int, q_heads: int, kv_heads: int,
-                        head_dim: int, device) -> torch.Tensor:
-    """A workspace for ``attention`` calls of these sizes (contents
-    irrelevant).  Calls that share one must not overlap in time."""
-    need = _lib.load().qkv_paged_attention_workspace_bytes(rows, max_rows, requests, width, page, q_heads, kv_heads,
-                                                           head_dim)
+                        head_dim: int, device, *, shared: bool = False) -> torch.Tensor:
+    """A workspace for ``attention`` calls of these sizes, with ``shared``
+    rows or without (contents irrelevant).  Calls that share one must not
+    overlap in time."""
+    lib = _lib.load()
+    size = lib.qkv_paged_attention_shared_workspace_bytes if shared else lib.qkv_paged_attention_workspace_bytes
+    need = size(rows, max_rows, requests, width, page, q_heads, kv_heads, head_dim)
     _require(need >= 0, "attention_workspace: sizes that attention does not take")
     return torch.empty(need // 4, dtype=torch.float32, device=device)
 
@@ -370,7 +419,7 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
               softcap: float = 0.0, slopes: torch.Tensor | None = None, prefix_lens: torch.Tensor | None = None,
               first_keys: torch.Tensor | None = None, out: torch.Tensor | None = None,
               workspace: torch.Tensor | None = None, k_scales: torch.Tensor | None = None,
-              v_scales: torch.Tensor | None = None) -> torch.Tensor:
+              v_scales: torch.Tensor | None = None, shared: SharedRows | None = None) -> torch.Tensor:
     """query [rows, Hq, D] over the cached keys of the rows' requests, whose
     own K and V were appended before.  Row i of request b is the token at
     p = kv_lens[b] - (cu_rows[b + 1] - cu_rows[b]) + i and sees the keys j
@@ -387,6 +436,14 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     ``workspace`` (``attention_workspace``) spares an allocation.  Quantised
     pages come with ``k_scales`` and ``v_scales`` (``quantized_pages``) and
     are attended to as the values of the query's dtype that they stand for.
+
+    ``shared`` (``share_rows`` of the same step) puts requests behind their
+    parents: with n = the parent's tokens, row i of request b is the token at
+    p = n + kv_lens[b] - (cu_rows[b + 1] - cu_rows[b]) + i of the parent's
+    tokens and its own behind them, first_keys and prefix_lens count from the
+    parent's first, and rows before a request's own first token get zeros.  A
+    parent's keys are read once for all rows behind it.
+
     Returns [rows, Hq, D] in the query's dtype; rows of ``out`` behind the
     last request are left as they were."""
     lib = _lib.load()
@@ -425,8 +482,11 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                  and out.stride(2) == 1, "out must have the query's shape, dtype and device with contiguous channels")
     most = rows if max_rows is None else max_rows
     ws_ptr, ws_bytes = None, 0
+    if shared is not None and (shared.rows != rows or shared.requests != n or shared.buffer.get_device() != idx):
+        raise RuntimeError(f"shared must be share_rows of {n} requests and {rows} rows on cuda:{idx}")
     if workspace is None:
-        ws_bytes = lib.qkv_paged_attention_workspace_bytes(rows, most, n, width, page, q_heads, kv_heads, dim)
+        size = lib.qkv_paged_attention_workspace_bytes if shared is None else lib.qkv_paged_attention_shared_workspace_bytes
+        ws_bytes = size(rows, most, n, width, page, q_heads, kv_heads, dim)
         if ws_bytes > 0:
             workspace = torch.empty(ws_bytes // 4, dtype=torch.float32, device=query.device)
             ws_ptr = workspace.data_ptr()
@@ -445,7 +505,11 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
             None if first_keys is None else first_keys.data_ptr(), ws_ptr, ws_bytes, out.data_ptr(), at + 40, dtype)
     guard = _lib.enter_device(idx)
     try:
-        if code:
+        if shared is not None:
+            rc = lib.qkv_paged_attention_shared(query.data_ptr(), at, k_pages.data_ptr(), v_pages.data_ptr(), at + 16,
+                                                _lib.ptr(k_scales), _lib.ptr(v_scales), at + 56, code,
+                                                shared.buffer.data_ptr(), *rest, _lib.stream_on(idx))
+        elif code:
             rc = lib.qkv_paged_attention_codes(query.data_ptr(), at, k_pages.data_ptr(), v_pages.data_ptr(), at + 16,
                                                k_scales.data_ptr(), v_scales.data_ptr(), at + 56, code, *rest,
                                                _lib.stream_on(idx))
