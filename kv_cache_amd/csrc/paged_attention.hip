@@ -26,7 +26,10 @@ QKV_EXPORT int64_t qkv_paged_attention_workspace_bytes(int64_t rows, int64_t max
                                                        int64_t page, int64_t q_heads, int64_t kv_heads,
                                                        int64_t head_dim) {
   if (!good_sizes(rows, requests, width, page, q_heads, kv_heads, head_dim)) return -1;
-  return workspace_bytes(plan_of(rows, max_rows, requests, width * page, kv_heads, q_heads / kv_heads), head_dim);
+  int64_t most = 0;   // over 16-bit pages and over codes
+  for (const int64_t row_bytes : {2 * head_dim, head_dim, head_dim / 2})
+    most = std::max(most, workspace_bytes(plan_of(rows, max_rows, requests, width * page, kv_heads, q_heads / kv_heads, row_bytes), head_dim));
+  return most;
 }
 
 QKV_EXPORT int qkv_paged_attention(const void* query, const int64_t* q_strides, const void* k_pages,

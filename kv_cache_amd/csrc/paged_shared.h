@@ -160,7 +160,7 @@ __device__ __forceinline__ int locate_shared(const PagedArgs& a, const SharedArg
 }
 
 template <int D, bool F16, bool FORM, int FMT, int NQ>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_shared_kernel(PagedArgs a, SharedArgs c) {
+__global__ __launch_bounds__(256, D == 64 && !FORM ? 3 : 2) void paged_shared_kernel(PagedArgs a, SharedArgs c) {
   __shared__ __attribute__((aligned(16))) uint16_t stage0[2 * kTile * D], stage1[2 * kTile * D];
   Where w;
   const int kind = locate_shared(a, c, blockIdx.x, w);
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(256) void paged_shared_join_kernel(PagedArgs a, Sha
         step[i] = (e.y & 15) * kPartUnit;
         from[i] = e.x + head - kv * a.group;
         // always so where the rows ascend
-        if (n[i] < 0 || e.x < 0 || from[i] + static_cast<int64_t>(max(n[i] - 1, 0)) * step[i] >= static_cast<int64_t>(c.max_units) * kPartUnit)
+        if (n[i] < 0 || e.x < 0 || step[i] == 0 || from[i] + static_cast<int64_t>(max(n[i] - 1, 0)) * step[i] >= static_cast<int64_t>(c.max_units) * kPartUnit)
           n[i] = 0;
         if (i == 0) on = n[0] > 0;   // else the output is written already
       }

@@ -61,6 +61,9 @@ constexpr int kTile = 64;      // keys per step of the rows kernel; splits are m
 constexpr int kRowsM = 128;    // rows of a tile of the rows kernel
 constexpr int kTokenM = 16;    // rows of a column set of the token kernel, which has one or two
 constexpr int kRound = 512;    // workgroups that run at once: two a CU
+// Three a CU of the token kernel with one column set over rows of at most 64 bytes (29 requests of up to 32001 keys in fp4:
+// 152 us, 170 with two; over the 128 bytes of fp8 two are as fast or faster, 8 requests of up to 16384 keys 46.8 and 49.9).
+constexpr int kShortRound = 768, kShortRow = 64;
 constexpr int kRowsJoins = 8, kTokenJoins = 4;   // workgroups that join a tile's parts; of a column set's
 constexpr int kStep = 32;      // keys a wave of the token kernel takes at a time
 // The weights exp(s - m) are rounded to the dtype for the product with V, half a step each (2^-8 in bf16, 2^-11 in
@@ -108,7 +111,8 @@ struct PagedArgs {
 // `most` rows, split along the keys into chunks of at least `min_keys`.
 struct PagedClass {
   int tokens, above, most, min_keys;
-  float per_round;     // 1.0001 / kRound
+  int round;           // workgroups that run at once
+  float per_round;     // 1.0001 / round
   int finer;           // more than one round of chunks where one does not come out even
   int max_parts;       // parts the workspace holds
   int max_joins;       // items of the kernel that joins them
@@ -224,7 +228,7 @@ __device__ __forceinline__ bool locate(const PagedArgs& a, const PagedClass& c, 
         w.chunk = round_up(per * (1.0f + 0.0667f * i));
         // without a division: one more or less is near enough to choose by
         const int ns = static_cast<int>(static_cast<float>(s.keys - 1) * __builtin_amdgcn_rcpf(static_cast<float>(w.chunk))) + 1;
-        if (__builtin_amdgcn_readlane(wave_scan(tiles * ns), 63) <= kRound) break;
+        if (__builtin_amdgcn_readlane(wave_scan(tiles * ns), 63) <= c.round) break;
       }
       if (i == 4) w.chunk = chunk_of(per);
     }
@@ -477,6 +481,16 @@ template <bool F16, int FMT>
 __device__ __forceinline__ u32x4_t unit_of(u32x4_t codes, int j, uint32_t scale) {
   return FMT == kFp8Pages ? values8<F16, FMT>(codes[2 * j], codes[2 * j + 1], scale) : values8<F16, FMT>(codes[j], 0, scale);
 }
+// Rows kernel: a thread that converts 16 bytes of a row has several units of 8 channels.  It writes the j-th of them to
+// LDS behind the j-th ones of the row's other threads, so that these lie side by side: unit u of a row holds the channels
+// of unit unit_at(u), in Q's order for the products with K and in the outputs' for those with V.  (A thread's own units
+// side by side: half of the LDS cycles were conflicts, 2048 x 65536 in fp8 2293 us.)
+template <int D, int FMT>
+__device__ __forceinline__ constexpr int unit_at(int u) {
+  if (FMT == kHalfPages) return u;
+  const int threads = (FMT == kFp8Pages ? D : D / 2) / 16, each = D / 8 / threads;
+  return each * (u % threads) + u / threads;
+}
 template <int D, int FMT>
 constexpr int kRowBytes = FMT == kHalfPages ? 2 * D : FMT == kFp8Pages ? D : D / 2;
 
@@ -564,7 +578,7 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
   u32x4_t qf[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
-    const uint4 x = load16u(a.q + r.q_at + 16 * s + 8 * half);
+    const uint4 x = load16u(a.q + r.q_at + 8 * (unit_at<D, FMT>(2 * s) + half * unit_at<D, FMT>(1)));
     qf[s] = r.on ? u32x4_t{x.x, x.y, x.z, x.w} : u32x4_t{0u, 0u, 0u, 0u};
   }
 
@@ -607,11 +621,10 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
     u32x4_t k[QP], v[QP];
     uint32_t ks[QP], vs[QP];
   };
-  Staged staged;
   const int q_row = tid / QU, q_unit = tid % QU;
   const uint32_t q_off = (q_row & 15) * tok_bytes + 16 * q_unit;
   const uint32_t qs_off = (q_row & 15) * (D / kScaleBlock) + q_unit * QC / kScaleBlock;
-  auto load = [&](int t0, Pages p, uint16_t* kb, uint16_t* vb) __attribute__((always_inline)) {
+  auto load = [&](int t0, Pages p, uint16_t* kb, uint16_t* vb, Staged& staged) __attribute__((always_inline)) {
 #pragma unroll
     for (int g = 0; g < 4; ++g)
       if (static_cast<unsigned>(p.id[g]) >= static_cast<unsigned>(a.pages)) p.id[g] = -1;
@@ -645,7 +658,8 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
   // Where some row does not see all of a tile, what of V no row may read (a page's rest) becomes zero before it is
   // used, and so do infinities and NaN, which a zero weight would not hide; add_odd adds those to the rows that do
   // see them.  A wave cleans what it loaded itself, so that the barrier behind the loads serves for both.
-  auto put_codes = [&](int t0, bool masked, bool holes, uint16_t* kb, uint16_t* vb, int buf) __attribute__((always_inline)) {
+  auto put_codes = [&](int t0, bool masked, bool holes, uint16_t* kb, uint16_t* vb, int buf, const Staged& staged)
+                       __attribute__((always_inline)) {
     bool odd = false;
     if (kTile * QU >= 256 || q_row < kTile) {
 #pragma unroll
@@ -654,12 +668,12 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
         const bool rest = masked && (t0 + row >= w.kv || (holes && page_id(a, w, t0 + (row & -16)) < 0));
 #pragma unroll
         for (int j = 0; j < QC / 8; ++j) {
-          const int to = row * D + 8 * ((q_unit * (QC / 8) + j) ^ swizzle<D>(row));
+          const int to = row * D + 8 * ((q_unit + QU * j) ^ swizzle<D>(row));
           *reinterpret_cast<u32x4_t*>(kb + to) = unit_of<F16, FMT>(staged.k[u], j, staged.ks[u]);
           u32x4_t x = unit_of<F16, FMT>(staged.v[u], j, staged.vs[u]);
           if (masked) {
-            if (rest) x = u32x4_t{0u, 0u, 0u, 0u};
-            else odd |= clean<F16>(x);
+            x = u32x4_t{rest ? 0u : x[0], rest ? 0u : x[1], rest ? 0u : x[2], rest ? 0u : x[3]};
+            odd |= clean<F16>(x);
           }
           *reinterpret_cast<u32x4_t*>(vb + to) = x;
         }
@@ -692,7 +706,7 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
       for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const uint16_t x = value_at<D, F16, FMT>(a, w.head, id, key & page_mask, 4 * half + 32 * d + 8 * (i >> 2) + (i & 3));
+          const uint16_t x = value_at<D, F16, FMT>(a, w.head, id, key & page_mask, 4 * half + 8 * unit_at<D, FMT>(4 * d + (i >> 2)) + (i & 3));
           if (not_finite<F16>(x)) o[d][i] += half_to_f32<F16>(x);
           if ((i & 3) == 3) __builtin_amdgcn_sched_barrier(0);
         }
@@ -701,9 +715,12 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
 
   const int k_at = l32 * D, k_sw = swizzle<D>(l32);
   const int v_row = 4 * half + ((lane & 15) >> 2), v_unit = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), v_el = 4 * (lane & 1);
-  auto compute = [&](int t0, bool masked, bool holes, const uint16_t* kb_, const uint16_t* vb_, int buf)
+  auto compute = [&](int t0, bool masked, bool holes, const uint16_t* kb_, const uint16_t* vb_, int buf, auto&& between)
                      __attribute__((always_inline)) {
-    if (t0 >= any_hi) return;   // no row of the wave sees any of it
+    if (t0 >= any_hi) {   // no row of the wave sees any of it
+      between();
+      return;
+    }
     f32x16_t s[2];
     {
       u32x4_t kf[2][KS];
@@ -727,6 +744,10 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // matrix instruction
         if (i < 2 * KS - 4) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
+    }
+    if constexpr (FMT != kHalfPages && !FORM) {
+      __builtin_amdgcn_sched_barrier(0);
+      between();
     }
     const int key0 = t0 + 4 * half;   // element i of tile kb: key0 + 32 kb + 8 (i / 4) + i % 4
     if constexpr (FORM) {
@@ -788,6 +809,10 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
         p[2 * kb + (q >> 1)][2 * (q & 1) + 1] = x[1];
       }
     l += sum0 + sum1;
+    if constexpr (FMT != kHalfPages && FORM) {   // (behind the first product, the score forms would spill registers)
+      __builtin_amdgcn_sched_barrier(0);
+      between();
+    }
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
@@ -802,11 +827,11 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
 
   // One barrier a tile: the next tile's loads are issued before this one is computed, and have landed behind it.
   bool holes, masked;   // of the tile that has landed
-  auto landed = [&](int t0, uint16_t* kb, uint16_t* vb, int buf) __attribute__((always_inline)) {
+  auto landed = [&](int t0, uint16_t* kb, uint16_t* vb, int buf, const Staged& staged) __attribute__((always_inline)) {
     if constexpr (FMT == kHalfPages) wave_landed();
     holes = hole, masked = t0 < wg_all_lo || t0 + kTile > wg_all_hi || holes;
     if constexpr (FMT != kHalfPages) {
-      if (t0 < end) put_codes(t0, masked, holes, kb, vb, buf);
+      if (t0 < end) put_codes(t0, masked, holes, kb, vb, buf, staged);
     } else {
       if (masked && t0 < end) clean_tile(t0, holes, vb, buf);
     }
@@ -815,13 +840,21 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
   auto turn = [&](int t0, const uint16_t* kb_, const uint16_t* vb_, int buf, uint16_t* kn, uint16_t* vn)
                   __attribute__((always_inline)) {
     const Pages next = pages_of(t0 + kTile);
-    if (t0 + kTile < end) load(t0 + kTile, next, kn, vn);
-    compute(t0, masked, holes, kb_, vb_, buf);
-    landed(t0 + kTile, kn, vn, buf ^ 1);
+    Staged staged;
+    const auto ahead = [&]() __attribute__((always_inline)) {
+      if (t0 + kTile < end) load(t0 + kTile, next, kn, vn, staged);
+    };
+    // codes go to registers, which the first product has most need of: they are loaded behind it
+    if constexpr (FMT == kHalfPages) ahead();
+    compute(t0, masked, holes, kb_, vb_, buf, [&]() __attribute__((always_inline)) {
+      if constexpr (FMT != kHalfPages) ahead();
+    });
+    landed(t0 + kTile, kn, vn, buf ^ 1, staged);
   };
   if (begin < end) {
-    load(begin, pages_of(begin), kbuf0, vbuf0);
-    landed(begin, kbuf0, vbuf0, 0);
+    Staged staged;
+    load(begin, pages_of(begin), kbuf0, vbuf0, staged);
+    landed(begin, kbuf0, vbuf0, 0, staged);
     for (int t0 = begin; t0 < end; t0 += 2 * kTile) {
       turn(t0, kbuf0, vbuf0, 0, kbuf1, vbuf1);
       if (t0 + kTile < end) turn(t0 + kTile, kbuf1, vbuf1, 1, kbuf0, vbuf0);
@@ -840,7 +873,7 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const float x[4] = {o[d][4 * q] * inv, o[d][4 * q + 1] * inv, o[d][4 * q + 2] * inv, o[d][4 * q + 3] * inv};
-        *reinterpret_cast<u32x2_t*>(mine + l32 * D + 8 * ((4 * d + q) ^ (l32 & (UR - 1))) + 4 * half) = pack4_half<F16>(x);
+        *reinterpret_cast<u32x2_t*>(mine + l32 * D + 8 * (unit_at<D, FMT>(4 * d + q) ^ (l32 & (UR - 1))) + 4 * half) = pack4_half<F16>(x);
       }
 #pragma unroll
     for (int i = 0; i < 32 * UR / 64; ++i) {
@@ -861,7 +894,7 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      *reinterpret_cast<float4*>(c.acc + at * D + 4 * half + 32 * d + 8 * q) =
+      *reinterpret_cast<float4*>(c.acc + at * D + 4 * half + 8 * unit_at<D, FMT>(4 * d + q)) =
           make_float4(o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]);
 }
 
@@ -962,7 +995,11 @@ __device__ __forceinline__ void token_body(const PagedArgs& a, const PagedClass&
       const char* kp = kh + at[t] + c16 * tok_bytes;
       if constexpr (KW >= 4) {
 #pragma unroll
-        for (int s = 0; s < KW / 4; ++s) x.k[t][s] = *reinterpret_cast<const u32x4_t*>(kp + 16 * g4 + 64 * s);
+        for (int s = 0; s < KW / 4; ++s) {
+          // once where one load takes a whole row (fp8, D 128: two loads share its line)
+          const auto* from = reinterpret_cast<const u32x4_t*>(kp + 16 * g4 + 64 * s);
+          x.k[t][s] = KW == 4 ? __builtin_nontemporal_load(from) : *from;
+        }
       } else {
         const u32x2_t y = *reinterpret_cast<const u32x2_t*>(kp + 8 * g4);
         x.k[t][0] = u32x4_t{y[0], y[1], 0u, 0u};
@@ -999,8 +1036,10 @@ __device__ __forceinline__ void token_body(const PagedArgs& a, const PagedClass&
       for (int s = 0; s < KS; ++s) x.k[t][s] = *reinterpret_cast<const u32x4_t*>(kp + k_off + 64 * s);
     }
   };
-  auto compute = [&](int t0, Step& x, uint16_t* vt) __attribute__((always_inline)) {
-    const bool masked = t0 < all_lo || t0 + kStep > all_hi || (x.id[0] | x.id[1]) < 0;
+  // `ahead` is called when the codes in x are used up.
+  auto compute = [&](int t0, Step& x, uint16_t* vt, auto&& ahead) __attribute__((always_inline)) {
+    const int id[2] = {x.id[0], x.id[1]};
+    const bool masked = t0 < all_lo || t0 + kStep > all_hi || (id[0] | id[1]) < 0;
     bool odd = false;
     u32x4_t kf[2][KS];
     if constexpr (FMT != kHalfPages) {
@@ -1019,23 +1058,24 @@ __device__ __forceinline__ void token_body(const PagedArgs& a, const PagedClass&
 #pragma unroll
       for (int u = 0; u < QP; ++u) {
         const int row = u * QR + q_row;
-        const bool rest = masked && (t0 + row >= w.kv || (row >= 16 ? x.id[1] : x.id[0]) < 0);
+        const bool rest = masked && (t0 + row >= w.kv || (row >= 16 ? id[1] : id[0]) < 0);
 #pragma unroll
         for (int j = 0; j < QC / 8; ++j) {
           u32x4_t y = unit_of<F16, FMT>(x.v[u], j, x.vs[u]);
           if (masked) {
-            if (rest) y = u32x4_t{0u, 0u, 0u, 0u};
-            else odd |= clean<F16>(y);
+            y = u32x4_t{rest ? 0u : y[0], rest ? 0u : y[1], rest ? 0u : y[2], rest ? 0u : y[3]};
+            odd |= clean<F16>(y);
           }
           *reinterpret_cast<u32x4_t*>(vt + row * D + 8 * ((q_unit * (QC / 8) + j) ^ swizzle<D>(row))) = y;
         }
       }
+      ahead();
     } else if (masked) {   // as in rows_body; a wave's LDS operations keep their order
 #pragma unroll
       for (int u = 0; u < NV; ++u) {
         u32x4_t* p = reinterpret_cast<u32x4_t*>(vt + 8 * (64 * u + lane));
         u32x4_t y = *p;
-        if (x.id[u * PASS / 16] < 0 || t0 + u * PASS + lane / UR >= w.kv) y = u32x4_t{0u, 0u, 0u, 0u};
+        if (id[u * PASS / 16] < 0 || t0 + u * PASS + lane / UR >= w.kv) y = u32x4_t{0u, 0u, 0u, 0u};
         else odd |= clean<F16>(y);
         *p = y;
       }
@@ -1068,7 +1108,7 @@ __device__ __forceinline__ void token_body(const PagedArgs& a, const PagedClass&
         if (masked) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (x.id[t] < 0 || key0 + i < r[n].lo || key0 + i >= r[n].hi) s[n][t][i] = ninf;
+            if (id[t] < 0 || key0 + i < r[n].lo || key0 + i >= r[n].hi) s[n][t][i] = ninf;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) cm = fmaxf(cm, s[n][t][i]);
@@ -1117,8 +1157,8 @@ __device__ __forceinline__ void token_body(const PagedArgs& a, const PagedClass&
     if (masked && __ballot(odd)) {
 #pragma unroll 1
       for (int j = 0; j < kStep; ++j) {
-        const int key = t0 + j, id = page_id(a, w, key);
-        if (id < 0) continue;
+        const int key = t0 + j, page = page_id(a, w, key);
+        if (page < 0) continue;
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
           if (!(r[n].on && key >= r[n].lo && key < r[n].hi)) continue;
@@ -1126,7 +1166,7 @@ __device__ __forceinline__ void token_body(const PagedArgs& a, const PagedClass&
           for (int d = 0; d < DB; ++d) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint16_t y = value_at<D, F16, FMT>(a, w.head, id, key & page_mask, 4 * g4 + 16 * d + i);
+              const uint16_t y = value_at<D, F16, FMT>(a, w.head, page, key & page_mask, 4 * g4 + 16 * d + i);
               if (not_finite<F16>(y)) o[n][d][i] += half_to_f32<F16>(y);
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -1147,16 +1187,28 @@ __device__ __forceinline__ void token_body(const PagedArgs& a, const PagedClass&
     load(t0, entries_of(t0), x0, vt0);
     e = entries_of(t0 + 4 * kStep);
   }
+  if constexpr (FMT != kHalfPages) {
+    // A step's codes leave their registers for the next step's as soon as they are converted.
+    while (t0 < end) {
+      compute(t0, x0, vt0, [&]() __attribute__((always_inline)) {
+        if (t0 + 4 * kStep < end) {
+          load(t0 + 4 * kStep, e, x0, vt0);
+          e = entries_of(t0 + 8 * kStep);
+        }
+      });
+      t0 += 4 * kStep;
+    }
+  }
   auto turn = [&](Step& x, uint16_t* vt, Step& xn, uint16_t* vn) __attribute__((always_inline)) {
-    if constexpr (FMT == kHalfPages) wave_landed();
+    wave_landed();
     if (t0 + 4 * kStep < end) {
       load(t0 + 4 * kStep, e, xn, vn);
       e = entries_of(t0 + 8 * kStep);
     }
-    compute(t0, x, vt);
+    compute(t0, x, vt, [] {});
     t0 += 4 * kStep;
   };
-  while (t0 < end) {
+  while (FMT == kHalfPages && t0 < end) {
     turn(x0, vt0, x1, vt1);
     if (t0 >= end) break;
     turn(x1, vt1, x0, vt0);
@@ -1290,15 +1342,16 @@ struct Shape {
 
 // Tiles of m rows for requests of more than `above` and at most `most` rows.
 Shape shape_of(bool token, int64_t m, int64_t above, int64_t most, int64_t rows, int64_t requests, int64_t max_keys,
-               int64_t kv_heads, int64_t group) {
+               int64_t kv_heads, int64_t group, int round) {
   Shape s{};
   s.cls.tokens = static_cast<int>(m / group);
   s.cls.above = static_cast<int>(above);
   s.cls.most = static_cast<int>(most);
   // up to 512 keys the launch that joins parts costs more than a split gives (one request of 500 keys: 12.8 us, 17.1 split)
   s.cls.min_keys = token && max_keys <= 512 ? 512 : 256;
-  const int64_t target = token && requests > 1 ? 3 * kRound : kRound;   // the most that chunk_of asks for
-  s.cls.per_round = 1.0001f / static_cast<float>(kRound);
+  const int64_t target = token && requests > 1 ? 3 * round : round;   // the most that chunk_of asks for
+  s.cls.round = round;
+  s.cls.per_round = 1.0001f / static_cast<float>(round);
   s.cls.finer = token && requests > 1;
   if (rows == 0 || s.cls.tokens == 0) return s;
   const int64_t some = std::min(requests, rows);
@@ -1321,18 +1374,19 @@ struct Plan {
   Shape rows, token;
   int sets;
 };
-Plan plan_of(int64_t rows, int64_t max_rows, int64_t requests, int64_t max_keys, int64_t kv_heads, int64_t group) {
+Plan plan_of(int64_t rows, int64_t max_rows, int64_t requests, int64_t max_keys, int64_t kv_heads, int64_t group,
+             int64_t row_bytes) {
   constexpr int64_t kAny = 0x7FFFFFFF;
   Plan p{};
   max_rows = std::max<int64_t>(max_rows, 1);
   p.sets = max_rows * group <= kTokenM ? 1 : 2;
   const int64_t m = p.sets * kTokenM;
   if (max_rows * group <= m) {   // a longer request, if there is one after all, takes several tiles
-    p.token = shape_of(true, m, 0, kAny, rows, requests, max_keys, kv_heads, group);
+    p.token = shape_of(true, m, 0, kAny, rows, requests, max_keys, kv_heads, group, p.sets == 1 && row_bytes <= kShortRow ? kShortRound : kRound);
     return p;
   }
-  p.token = shape_of(true, m, 0, m / group, rows, requests, max_keys, kv_heads, group);
-  p.rows = shape_of(false, kRowsM, m / group, kAny, rows, requests, max_keys, kv_heads, group);
+  p.token = shape_of(true, m, 0, m / group, rows, requests, max_keys, kv_heads, group, kRound);
+  p.rows = shape_of(false, kRowsM, m / group, kAny, rows, requests, max_keys, kv_heads, group, kRound);
   return p;
 }
 
@@ -1353,14 +1407,14 @@ int64_t workspace_bytes(const Plan& p, int64_t head_dim) {
 // Both kernels stage K and V in two halves of LDS, of which the compiler sees that reads of one need not wait for
 // the loads into the other.
 template <int D, bool F16, bool FORM, int FMT, int NQ>
-__global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedArgs a, PagedClass c) {
+__global__ __launch_bounds__(256, FMT != kHalfPages && NQ == 1 ? 3 : 2) void paged_token_kernel(PagedArgs a, PagedClass c) {
   __shared__ __attribute__((aligned(16))) uint16_t stage0[2 * kTile * D], stage1[2 * kTile * D];
   Where w;
   if (locate<false>(a, c, blockIdx.x, w)) token_body<D, F16, FORM, NQ, FMT>(a, c, w, stage0, stage1);
 }
 // Requests of both classes in one launch, the long ones first.
 template <int D, bool F16, bool FORM, int FMT>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_rows_kernel(PagedArgs a, PagedClass rows, PagedClass token,
+__global__ __launch_bounds__(256, D == 64 && !(FORM && FMT != kHalfPages) ? 3 : 2) void paged_rows_kernel(PagedArgs a, PagedClass rows, PagedClass token,
                                                                           int n_rows) {
   __shared__ __attribute__((aligned(16))) uint16_t stage0[2 * kTile * D], stage1[2 * kTile * D];
   Where w;
@@ -1465,7 +1519,8 @@ int paged_call(const PagedCall& c, const char* what) {
   bool f16;
   PagedArgs a;
   if (const int rc = make_args(c, what, FMT, &f16, &a)) return rc;
-  Plan p = plan_of(c.rows, c.max_rows, c.requests, c.width * c.page, c.kv_heads, a.group);
+  Plan p = plan_of(c.rows, c.max_rows, c.requests, c.width * c.page, c.kv_heads, a.group,
+                   FMT == kHalfPages ? 2 * c.head_dim : FMT == kFp8Pages ? c.head_dim : c.head_dim / 2);
   // a grid has less than 2^32 threads
   if (p.rows.items + p.token.items >= (1 << 24)) return fail(QKV_ERR_UNSUPPORTED, "%s: too many rows", what);
   const int64_t need = workspace_bytes(p, c.head_dim);
