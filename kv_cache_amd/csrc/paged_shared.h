@@ -3,7 +3,7 @@
 //
 // A row sees its parent's tokens and then its own request's up to itself.  A tile holds either rows of one request over
 // its own keys, or heirs of one parent, of whatever requests, over the parent's; tiles are those of the two bodies of
-// paged_tiles.h, and one launch does both kinds.  Every tile's keys are split into chunks, as many keys for all, so that
+// paged_tiles.h, and one launch does both kinds.  The tiles' keys are split into chunks of about the same length, so that
 // the launch's workgroups are as even as they can be; a (row, head)'s parts, its own and its parent's, are joined by a
 // second launch in their order.  Only tiles in one chunk of rows without a parent write the output themselves.
 #pragma once
@@ -13,7 +13,8 @@
 namespace qkv {
 namespace {
 
-constexpr int kRounds = 2;   // workgroups that chunks are cut for, in rounds of those that run at once
+constexpr int kRounds = 2;         // most workgroups that chunks are cut for, in rounds of those that run at once
+constexpr int kLaneRequests = 2;   // requests of a lane in the search of a workgroup's work without barriers
 
 struct SharedArgs {
   PagedClass rows, token;   // acc and ml of rows serve both
@@ -53,50 +54,92 @@ __device__ __forceinline__ int locate_shared(const PagedArgs& a, const SharedArg
     return static_cast<float>(s.nt[0]) * static_cast<float>(s.keys[0]) +
            static_cast<float>(s.nt[1]) * static_cast<float>(s.keys[1]);
   };
-  auto set_chunk = [&](float work) {
-    const float keys = work * a.kv_heads * c.rows.per_round;
+  auto round_up = [&](float keys) {
     const int least = max(c.rows.min_keys, static_cast<int>(fminf(keys, 1073741824.0f)) + 1);
-    w.chunk = __builtin_amdgcn_readfirstlane((least + kTile - 1) & -kTile);
+    return __builtin_amdgcn_readfirstlane((least + kTile - 1) & -kTile);
   };
-  int kind, at, nt, units;
-  if (a.requests <= 64) {
-    const Shares s = shares_of(lane);
-    set_chunk(wave_total(work_of(s)));
-    int begin[2], unit[2], items[2], ns[2], item0 = 0, unit0 = 0;
-    uint64_t hit[2];
+  // How much of the workgroups that run at once a request's tiles take under w.chunk: a chunk counts as one, keys that fill
+  // none as their share and what a workgroup costs by itself.
+  auto slots_of = [&](const Shares& s) {
+    const float per = __builtin_amdgcn_rcpf(static_cast<float>(w.chunk));
+    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      ns[i] = splits_of(s.keys[i]);
-      items[i] = s.nt[i] * a.kv_heads * ns[i];
-      const int mine = items[i] * units_of(s.n_rows[i]), up = wave_scan(items[i]), up_units = wave_scan(mine);
-      begin[i] = item0 + up - items[i];
-      unit[i] = unit0 + up_units - mine;
-      item0 += __builtin_amdgcn_readlane(up, 63);
-      unit0 += __builtin_amdgcn_readlane(up_units, 63);
-      hit[i] = __ballot(item >= begin[i] && item - begin[i] < items[i]);
+      const float share = static_cast<float>(s.keys[i]) * per;
+      sum += static_cast<float>(s.nt[i]) * (share > 1.0f ? ceilf(share) : fminf(1.0f, share + 0.1f));
     }
-    kind = hit[0] ? 0 : 1;
-    const uint64_t any = hit[0] ? hit[0] : hit[1];
-    if (!any) return 0;
-    w.b = __builtin_ctzll(any);
-    auto take = [&](int x, int y) { return __builtin_amdgcn_readlane(kind ? y : x, w.b); };
-    at = item - take(begin[0], begin[1]);
-    w.part = take(unit[0], unit[1]);
-    nt = take(s.nt[0], s.nt[1]);
-    w.kv = take(s.keys[0], s.keys[1]);
-    w.n_split = take(ns[0], ns[1]);
-    w.row0 = take(s.row0[0], s.row0[1]);
-    w.n_rows = take(s.n_rows[0], s.n_rows[1]);
+    return sum * a.kv_heads;
+  };
+  // One round of chunks where one comes out, up to a fifth longer than the work's share (64 requests behind 32768 keys: 90
+  // us, 102 in two rounds), else two.
+  auto set_chunk = [&](float per, auto&& slots) {
+    for (int i = 0; i < 4; ++i) {
+      w.chunk = round_up(per * (1.0f + 0.0667f * i));
+      if (slots() <= static_cast<float>(kRound)) return;
+    }
+    w.chunk = round_up(per * 0.5f);
+  };
+  int kind, at, nt;
+  const int parts = (a.requests + 63) >> 6;   // of 64 requests
+  if (parts <= kLaneRequests) {
+    // every wave for itself, kLaneRequests a lane
+    Shares s[kLaneRequests];
+    float work = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kLaneRequests; ++k) {
+      s[k] = Shares{};
+      if (k < parts) s[k] = shares_of(64 * k + lane);
+      work += work_of(s[k]);
+    }
+    set_chunk(wave_total(work) * a.kv_heads * c.rows.per_round, [&] {
+      float sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kLaneRequests; ++k)
+        if (k < parts) sum += slots_of(s[k]);
+      return wave_total(sum);
+    });
+    int item0 = 0, unit0 = 0;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < kLaneRequests; ++k) {
+        if (found || k >= parts) continue;   // the same for every lane
+        const int ns = splits_of(s[k].keys[i]), items = s[k].nt[i] * a.kv_heads * ns;
+        const int mine = items * units_of(s[k].n_rows[i]), up = wave_scan(items), up_units = wave_scan(mine);
+        const int begin = item0 + up - items, unit = unit0 + up_units - mine;
+        const uint64_t hit = __ballot(item >= begin && item - begin < items);
+        if (hit) {
+          const int from = __builtin_ctzll(hit);
+          found = true;
+          kind = i;
+          w.b = 64 * k + from;
+          at = item - __builtin_amdgcn_readlane(begin, from);
+          w.part = __builtin_amdgcn_readlane(unit, from);
+          nt = __builtin_amdgcn_readlane(s[k].nt[i], from);
+          w.kv = __builtin_amdgcn_readlane(s[k].keys[i], from);
+          w.n_split = __builtin_amdgcn_readlane(ns, from);
+          w.row0 = __builtin_amdgcn_readlane(s[k].row0[i], from);
+          w.n_rows = __builtin_amdgcn_readlane(s[k].n_rows[i], from);
+        }
+        item0 += __builtin_amdgcn_readlane(up, 63);
+        unit0 += __builtin_amdgcn_readlane(up_units, 63);
+      }
+    if (!found) return 0;
   } else {
     __shared__ float s_tot[4];
     __shared__ int s_part[8], s_hit[9];
-    float total = 0.0f;
-    for (int b0 = 0; b0 < a.requests; b0 += 256) total += work_of(shares_of(b0 + tid));
-    total = wave_total(total);
-    if (lane == 0) s_tot[wave] = total;
+    auto total = [&](auto&& f) {   // over all requests; the same in every thread
+      float sum = 0.0f;
+      for (int b0 = 0; b0 < a.requests; b0 += 256) sum += f(shares_of(b0 + tid));
+      sum = wave_total(sum);
+      __syncthreads();
+      if (lane == 0) s_tot[wave] = sum;
+      __syncthreads();
+      return (s_tot[0] + s_tot[1]) + (s_tot[2] + s_tot[3]);
+    };
     if (tid == 0) s_hit[0] = -1;
-    __syncthreads();
-    set_chunk((s_tot[0] + s_tot[1]) + (s_tot[2] + s_tot[3]));
+    set_chunk(total(work_of) * a.kv_heads * c.rows.per_round, [&] { return total(slots_of); });
     int carry = 0, unit_carry = 0;
     for (int i = 0; i < 2; ++i) {
       for (int b0 = 0; b0 < a.requests; b0 += 256) {
@@ -104,6 +147,7 @@ __device__ __forceinline__ int locate_shared(const PagedArgs& a, const SharedArg
         const int ns = splits_of(i ? s.keys[1] : s.keys[0]), tiles = i ? s.nt[1] : s.nt[0], n = i ? s.n_rows[1] : s.n_rows[0];
         const int items = tiles * a.kv_heads * ns, mine = items * units_of(n);
         const int up = wave_scan(items), up_units = wave_scan(mine);
+        __syncthreads();
         if (lane == 63) {
           s_part[2 * wave] = up;
           s_part[2 * wave + 1] = up_units;
@@ -147,7 +191,9 @@ __device__ __forceinline__ int locate_shared(const PagedArgs& a, const SharedArg
   }
   w.heirs = kind == 0;
   w.alone = !w.heirs && a.before[w.b] <= 0;
-  units = units_of(w.n_rows);
+  const int units = units_of(w.n_rows);
+  // as many keys for each of the tile's chunks
+  if (w.n_split > 1) w.chunk = __builtin_amdgcn_readfirstlane(((w.kv + w.n_split - 1) / w.n_split + kTile - 1) & -kTile);
   const int rest = __builtin_amdgcn_readfirstlane(at / a.kv_heads);
   w.head = at - rest * a.kv_heads;
   w.split = __builtin_amdgcn_readfirstlane(rest / nt);
@@ -262,7 +308,7 @@ SharedShape shared_shape_of(int64_t rows, int64_t max_rows, int64_t requests, in
   s.c.token.tokens = static_cast<int>(s.sets * kTokenM / group);
   s.c.rows.tokens = static_cast<int>(kRowsM / group);
   s.c.rows.min_keys = 256;
-  s.c.rows.per_round = 1.0001f / static_cast<float>(kRounds * kRound);
+  s.c.rows.per_round = 1.0001f / static_cast<float>(kRound);
   const int64_t some = std::min(requests, rows), more = max_keys > 256 ? kRounds * kRound : 0;
   const int64_t large = rows > s.c.token.tokens ? 2 * kv_heads * (rows / s.c.rows.tokens + std::min(requests, rows / (s.c.token.tokens + 1))) + more : 0;
   const int64_t small = s.c.token.tokens ? 2 * kv_heads * some + more : 0;
