@@ -30,12 +30,11 @@ struct Shares {
 // Which work workgroup `item` has: 0 none, 1 rows' tile, 2 a token tile.
 __device__ __forceinline__ int locate_shared(const PagedArgs& a, const SharedArgs& c, int item, Where& w) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const float per_rows = 1.0f / static_cast<float>(c.rows.tokens), per_token = 1.0f / static_cast<float>(max(c.token.tokens, 1));
   auto shares_of = [&](int b) {
     Shares s{};
     if (b >= a.requests) return s;
-    const auto tokens_of = [&](int n) {
-      return static_cast<int>(min(static_cast<int64_t>(max(n, 0)), static_cast<int64_t>(a.width) << a.shift));
-    };
+    const auto tokens_of = [&](int n) { return min(max(n, 0), a.width << a.shift); };   // (at most 2^30)
     s.n_rows[1] = rows_of(a, b, s.row0[1]);
     s.keys[1] = tokens_of(a.kv_lens[b]);
     s.row0[0] = min(max(a.heirs_cu[b], 0), a.rows);
@@ -43,12 +42,16 @@ __device__ __forceinline__ int locate_shared(const PagedArgs& a, const SharedArg
     s.keys[0] = tokens_of(a.parent_lens[b]);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int per = s.n_rows[i] > c.token.tokens ? c.rows.tokens : c.token.tokens;
-      s.nt[i] = s.n_rows[i] ? (s.n_rows[i] + per - 1) / per : 0;
+      // ceil(rows / tokens of a tile): half a row from the next whole number, which 2^20 rows are not rounded over
+      const float per = s.n_rows[i] > c.token.tokens ? per_rows : per_token;
+      s.nt[i] = s.n_rows[i] ? static_cast<int>((static_cast<float>(s.n_rows[i]) - 0.5f) * per) + 1 : 0;
     }
     return s;
   };
-  auto splits_of = [&](int keys) { return keys > w.chunk ? (keys + w.chunk - 1) / w.chunk : 1; };
+  // one more or less is as good: what a chunk holds follows from their number
+  auto splits_of = [&](int keys) {
+    return keys > w.chunk ? static_cast<int>(static_cast<float>(keys - 1) * __builtin_amdgcn_rcpf(static_cast<float>(w.chunk))) + 1 : 1;
+  };
   auto units_of = [&](int n_rows) { return n_rows > c.token.tokens ? kRowsM / kPartUnit : c.token_units; };
   auto work_of = [&](const Shares& s) {
     return static_cast<float>(s.nt[0]) * static_cast<float>(s.keys[0]) +
