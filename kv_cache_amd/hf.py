@@ -58,6 +58,10 @@ other than causal with left padding and the layer's window raises.
     model.config._attn_implementation = "paged"
     cache = hf.PagedCache(capacity=40960, page=64)
     out = model.generate(**tokenizer(prompts, padding=True), past_key_values=cache)
+
+``PagedCache(..., quantize="fp8")`` (or "fp4") keeps the pages as codes.  After a
+prompt, ``cache.batch_repeat_interleave(n)`` makes n sequences of each (samples
+of one prompt): they share its pages, which attention reads once for all.
 """
 
 from __future__ import annotations
@@ -339,13 +343,15 @@ class _PagedState:
     hold tokens, and the plan of the step that the first layer to reach it
     made."""
 
-    def __init__(self, capacity: int, page: int):
-        self.capacity, self.page = int(capacity), int(page)
+    def __init__(self, capacity: int, page: int, quantize: str | None = None):
+        self.capacity, self.page, self.quantize = int(capacity), int(page), quantize
         self.table = self.plan = None
         self.real = None         # bool [batch, columns]: those with a token; None while no step had a mask
         self.masks = []          # (mask, window) of the step's layers, compared with what the pages show
         self.length = self.new = 0   # columns stepped, padding included; of the last step
         self.open = False        # an update's columns have not been attended over yet
+        self.copies = 1          # sequences that continue each of the first prompts (``repeat``)
+        self.parents = self.shared = None   # of every request of the table; the step's rows by parent
 
     def check_closed(self) -> None:
         """Raises if the attention function did not take an earlier update:
@@ -381,9 +387,45 @@ class _PagedState:
             new = torch.full((batch,), n, dtype=torch.int32, device=device)
         else:
             new = self.real[:, length - n:length].sum(-1, dtype=torch.int32)
-        self.plan = self.table.step(new, batch * n, padded=n)
+        if self.parents is None:
+            self.plan = self.table.step(new, batch * n, padded=n)
+        else:   # the parents, behind their children in the table, get no tokens, and rows that the model does not have
+            requests = self.parents.numel()
+            if batch * (self.copies + 1) != requests * self.copies:
+                raise RuntimeError(f"the PagedCache was repeated for {requests - requests // (self.copies + 1)} sequences, "
+                                   f"this step has {batch}")
+            plan = self.table.step(torch.cat((new, new.new_zeros(requests - batch))), requests * n, padded=n)
+            self.shared = paged.share_rows(self.parents, plan.cu_rows, plan.kv_lens, self.table.lens, batch * n)
+            self.plan = plan._replace(slots=plan.slots[:batch * n], positions=self.shared.positions)
         self.length, self.new = length, n
         return self.plan
+
+    def repeat(self, copies: int) -> None:
+        """Every sequence becomes ``copies`` that continue it: the prompts stay
+        where they are, as parents of requests that begin without a token."""
+        old = self.table
+        batch = old.lens.numel()
+        table = paged.PageTable(batch * (copies + 1), self.capacity, old.pages + self.more_pages(copies), self.page,
+                                old.table.device)
+        table.table[batch * copies:] = old.table
+        table.lens[batch * copies:] = old.lens
+        more = table.pages - old.pages
+        table.free[:more] = torch.arange(table.pages - 1, old.pages - 1, -1, dtype=torch.int32, device=table.free.device)
+        table.free[more:] = old.free
+        table.count.copy_(old.count + more)
+        prompts = torch.arange(batch * copies, table.lens.numel(), dtype=torch.int32, device=table.lens.device)
+        self.parents = torch.cat((prompts.repeat_interleave(copies), torch.full_like(prompts, -1)))
+        if self.real is not None:
+            self.real = self.real.repeat_interleave(copies, 0)
+        self.table, self.copies = table, copies
+
+    def more_pages(self, copies: int) -> int:
+        """Pages that ``copies`` continuations of each of the table's sequences
+        need besides the free ones."""
+        batch = self.table.lens.numel() // (self.copies + 1 if self.parents is not None else 1)
+        pages = batch * -(-self.capacity // self.page)
+        need = batch * copies * -(-(self.capacity - self.length) // self.page)
+        return max(0, need - (pages - batch * -(-self.length // self.page)))
 
     def _compare(self, length: int, n: int, batch: int, device, mask, window, first: bool) -> None:
         """Takes the padding of the step's columns from the mask (``first``)
@@ -429,11 +471,14 @@ class _PagedState:
     def reset(self) -> None:
         if self.table is not None and self.length:
             self.table.release(torch.zeros_like(self.table.lens))
-        self.length, self.real, self.masks, self.open = 0, None, [], False
+        if self.parents is not None:   # a table for the next batch
+            self.table = self.parents = self.shared = None
+        self.length, self.real, self.masks, self.open, self.copies = 0, None, [], False, 1
 
 
 class PagedCacheLayer:
-    """One layer's K/V pages (bf16 or fp16).  ``update`` only counts the new
+    """One layer's K/V pages (bf16 or fp16, or codes of them with their
+    scales).  ``update`` only counts the new
     columns and hands the layer on to the attention function with their K/V;
     that one knows the mask, and writes what is no padding into the pages.
     Another attention function would see the new columns alone: the next
@@ -447,8 +492,9 @@ class PagedCacheLayer:
         self.state = state
         self.keys = self.values = None        # no dense K/V exist
         self.k_pages = self.v_pages = None
+        self.scales = {}                      # of quantised pages
         self.is_initialized = False
-        self.length = 0
+        self.length, self.copies = 0, 1
 
     def __repr__(self):
         return f"PagedCacheLayer(length={self.length}, capacity={self.state.capacity}, page={self.state.page})"
@@ -459,8 +505,8 @@ class PagedCacheLayer:
 
     def holds(self, key_states: torch.Tensor) -> bool:
         """Whether the pages are those of such keys."""
-        return (self.k_pages.shape == self.page_shape(key_states) and self.dtype == key_states.dtype
-                and self.device == key_states.device)
+        return (self.shape == self.page_shape(key_states) and self.k_pages.size(0) == self.shape[0]
+                and self.dtype == key_states.dtype and self.device == key_states.device)
 
     def take_back(self, n: int) -> None:
         """Undoes an update whose step was refused before anything was written;
@@ -471,10 +517,15 @@ class PagedCacheLayer:
 
     # -- CacheLayerMixin protocol ------------------------------------------
     def lazy_initialization(self, key_states: torch.Tensor, value_states: torch.Tensor) -> None:
-        shape = self.page_shape(key_states)
+        self.shape = self.page_shape(key_states)
         self.dtype, self.device = key_states.dtype, key_states.device
-        self.k_pages = torch.empty(shape, dtype=key_states.dtype, device=key_states.device)
-        self.v_pages = torch.empty(shape, dtype=value_states.dtype, device=key_states.device)
+        if self.state.quantize is None:
+            self.k_pages = torch.empty(self.shape, dtype=key_states.dtype, device=key_states.device)
+            self.v_pages = torch.empty(self.shape, dtype=value_states.dtype, device=key_states.device)
+        else:
+            (self.k_pages, k), (self.v_pages, v) = (
+                paged.quantized_pages(*self.shape, self.state.quantize, key_states.device) for _ in range(2))
+            self.scales = dict(k_scales=k, v_scales=v)
         self.is_initialized = True
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args, **kwargs):
@@ -502,8 +553,28 @@ class PagedCacheLayer:
         return self.state.capacity
 
     def reset(self) -> None:
-        self.length = 0
+        self.length, self.copies = 0, 1
         self.state.reset()
+
+    def batch_repeat_interleave(self, repeats: int) -> None:
+        """Every sequence becomes ``repeats`` that share its pages: what they
+        add goes to pages of their own, and attention reads the shared ones
+        once for all of them.  Once after a prompt; not again before reset."""
+        state = self.state
+        if repeats < 1:
+            raise RuntimeError(f"repeats must be positive, got {repeats}")
+        if repeats == 1:
+            return
+        state.check_closed()
+        if self.length == 0 or state.length != self.length or self.copies != 1 or state.copies not in (1, repeats):
+            raise RuntimeError("PagedCacheLayer is repeated once, after a step of all layers")
+        more = state.more_pages(repeats)
+        if state.copies == 1:
+            state.repeat(repeats)
+        grown = lambda x: torch.cat((x.view(torch.uint8), x.new_empty((more, *x.shape[1:])).view(torch.uint8))).view(x.dtype)  # noqa: E731
+        self.k_pages, self.v_pages = grown(self.k_pages), grown(self.v_pages)
+        self.scales = {name: grown(x) for name, x in self.scales.items()}
+        self.copies = repeats
 
     def crop(self, max_length: int) -> None:
         raise RuntimeError("PagedCacheLayer cannot be cropped")
@@ -511,7 +582,7 @@ class PagedCacheLayer:
     def reorder_cache(self, beam_idx) -> None:
         raise RuntimeError("PagedCacheLayer cannot be reordered")
 
-    batch_repeat_interleave = batch_select_indices = reorder_cache
+    batch_select_indices = reorder_cache
 
     def offload(self):
         raise RuntimeError("PagedCacheLayer cannot be offloaded")
@@ -522,15 +593,20 @@ class PagedCacheLayer:
 class PagedCache:
     """A transformers ``Cache`` whose layers keep K/V in pages of ``page``
     tokens under one page table; ``capacity`` bounds the columns (tokens and
-    padding) of a sequence."""
+    padding) of a sequence.  ``quantize`` "fp8" or "fp4" keeps them as codes
+    with a scale for 32 channels (``paged.quantized_pages``).
+    ``batch_repeat_interleave(n)`` after a prompt makes n sequences of each
+    that share its pages."""
 
-    def __new__(cls, capacity: int, page: int = 64):
+    def __new__(cls, capacity: int, page: int = 64, quantize: str | None = None):
         from transformers.cache_utils import Cache, CacheLayerMixin
 
         if not (16 <= page <= 4096 and page & (page - 1) == 0):
             raise RuntimeError(f"page must be a power of two in [16, 4096], got {page}")
+        if quantize not in (None, "fp8", "fp4"):
+            raise RuntimeError(f"quantize must be None, fp8 or fp4, got {quantize!r}")
         return Cache(layer_class_to_replicate=functools.partial(_paged_layer_class(CacheLayerMixin),
-                                                               _PagedState(capacity, page)))
+                                                               _PagedState(capacity, page, quantize)))
 
 
 @functools.lru_cache(maxsize=1)
@@ -595,11 +671,12 @@ def paged_attention_forward(module, query: torch.Tensor, key: torch.Tensor, valu
         layer.take_back(key.size(2))
         raise
     rows = lambda x: x.transpose(1, 2).reshape(b * n, x.size(1), d)  # noqa: E731  (a view of what projections give)
-    paged.append(rows(key), rows(value), layer.k_pages, layer.v_pages, plan.slots)
+    paged.append(rows(key), rows(value), layer.k_pages, layer.v_pages, plan.slots, **layer.scales)
+    extra = layer.scales if state.shared is None else dict(layer.scales, shared=state.shared)
     first = None if sliding_window is None else plan.positions - (int(sliding_window) - 1)
     out = paged.attention(rows(query), layer.k_pages, layer.v_pages, state.table.table, plan.cu_rows, plan.kv_lens,
                           d ** -0.5 if scaling is None else float(scaling), max_rows=n,
-                          softcap=0.0 if softcap is None else float(softcap), first_keys=first)
+                          softcap=0.0 if softcap is None else float(softcap), first_keys=first, **extra)
     state.open = False
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
         out = _NoBackward.apply(out, query, key, value)

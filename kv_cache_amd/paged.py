@@ -198,9 +198,10 @@ class SharedRows:
     __slots__ = ("buffer", "rows", "requests", "positions")
 
     def __init__(self, requests: int, rows: int, device):
-        words = _lib.load().qkv_paged_share_words(rows, requests)
-        _require(words >= 0, f"share_rows takes 1 to 4096 requests and 1 to 2^20 rows, got {requests} and {rows}")
-        self.buffer = torch.empty(words, dtype=torch.int32, device=device)
+        if not (1 <= requests <= 4096 and 1 <= rows <= 1 << 20):
+            raise RuntimeError(f"share_rows takes 1 to 4096 requests and 1 to 2^20 rows, got {requests} and {rows}")
+        # qkv_paged_share_words
+        self.buffer = torch.empty(3 * rows + 4 * requests + 1, dtype=torch.int32, device=device)
         self.rows, self.requests, self.positions = rows, requests, self.buffer[:rows]
 
 
@@ -216,8 +217,9 @@ def share_rows(parents: torch.Tensor, cu_rows: torch.Tensor, kv_lens: torch.Tens
     own tokens.  The parent's own parent does not count.  Release a parent
     after its last child."""
     lib = _lib.load()
-    _require(parents.is_cuda, "parents must be CUDA")
     n, idx = parents.numel(), parents.get_device()
+    if idx < 0:
+        raise RuntimeError("parents must be CUDA")
     _i32("parents", parents, n, idx)
     _i32("cu_rows", cu_rows, n + 1, idx)
     _i32("kv_lens", kv_lens, n, idx)
@@ -258,31 +260,29 @@ def quantized_pages(pages: int, kv_heads: int, page: int, head_dim: int, kind: s
     return scales.new_empty((pages, kv_heads, page, head_dim // 2)), scales
 
 
-def _check_codes(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales, v_scales) -> tuple[int, int, tuple, tuple]:
-    """(code, head dim, strides of the pages, strides of the scales) of a
-    layer's quantised pages, checked."""
-    code = _CODES.get(k_pages.dtype)
+def _check_codes(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales, v_scales) -> tuple:
+    """(code, device index, shape of the values, strides of the pages, strides
+    of the scales) of a layer's quantised pages, checked."""
+    code, idx, shape, ps = _CODES.get(k_pages.dtype), k_pages.get_device(), k_pages.shape, k_pages.stride()
     if code is None:
         raise RuntimeError(f"quantised pages must be float8_e4m3fn or uint8, got {k_pages.dtype}")
-    if (not k_pages.is_cuda or k_pages.dim() != 4 or k_pages.shape != v_pages.shape
-            or v_pages.dtype is not k_pages.dtype or v_pages.get_device() != k_pages.get_device()):
+    if (idx < 0 or len(shape) != 4 or v_pages.shape != shape or v_pages.dtype is not k_pages.dtype
+            or v_pages.get_device() != idx):
         raise RuntimeError("k_pages and v_pages must be CUDA [pages, kv_heads, page, dim] of one shape, dtype and "
                            "device with contiguous channels")
-    ps = k_pages.stride()
-    if ps != v_pages.stride() or ps[3] != 1:
+    if v_pages.stride() != ps or ps[3] != 1:
         raise RuntimeError("k_pages and v_pages must have the same strides, with contiguous channels")
-    pages, heads, page, dim = k_pages.shape
+    pages, heads, page, dim = shape
     dim *= code   # two to a byte
-    shape = (pages, heads, page, dim // _BLOCK)
     if dim % _BLOCK or k_scales is None or v_scales is None:
         raise RuntimeError(f"quantised pages have k_scales and v_scales and a multiple of {_BLOCK} channels")
-    ss = k_scales.stride()
-    for t in (k_scales, v_scales):
-        if (t.dtype is not torch.uint8 or t.shape != shape or t.get_device() != k_pages.get_device()
-                or t.stride() != ss or ss[3] != 1 or ss[2] != shape[3]):
-            raise RuntimeError(f"k_scales and v_scales must be uint8 {list(shape)} on {k_pages.device} of the same "
-                               "strides, a head's tokens without gaps")
-    return code, dim, ps, ss
+    blocks, ss = dim // _BLOCK, k_scales.stride()
+    if (k_scales.dtype is not torch.uint8 or v_scales.dtype is not torch.uint8 or k_scales.get_device() != idx
+            or v_scales.get_device() != idx or k_scales.shape != (pages, heads, page, blocks)
+            or v_scales.shape != k_scales.shape or v_scales.stride() != ss or ss[3] != 1 or ss[2] != blocks):
+        raise RuntimeError(f"k_scales and v_scales must be uint8 {[pages, heads, page, blocks]} on {k_pages.device} of "
+                           "the same strides, a head's tokens without gaps")
+    return code, idx, (pages, heads, page, dim), ps, ss
 
 
 def append(key: torch.Tensor, value: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -328,9 +328,7 @@ def append(key: torch.Tensor, value: torch.Tensor, k_pages: torch.Tensor, v_page
 
 def _append_codes(key, value, k_pages, v_pages, slots, k_scales, v_scales) -> None:
     lib = _lib.load()
-    code, dim, ps, ss = _check_codes(k_pages, v_pages, k_scales, v_scales)
-    pages, heads, page, _ = k_pages.shape
-    idx = k_pages.get_device()
+    code, idx, (pages, heads, page, dim), ps, ss = _check_codes(k_pages, v_pages, k_scales, v_scales)
     rows = slots.numel()
     _check_slots(slots, rows, idx)
     dtype = _lib.half_code("key", key)
@@ -366,20 +364,24 @@ def read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, cu_r
     left as they were."""
     lib = _lib.load()
     if k_scales is not None or v_scales is not None or k_pages.dtype in _CODES:
-        code, dim, ps, ss = _check_codes(k_pages, v_pages, k_scales, v_scales)
-        dtype = torch.bfloat16 if dtype is None else dtype
-        _require(dtype in _HALF, f"dtype must be bfloat16 or float16, got {dtype}")
+        code, on, (pages, heads, page, dim), ps, ss = _check_codes(k_pages, v_pages, k_scales, v_scales)
+        if dtype is None:
+            dtype = torch.bfloat16
+        elif dtype not in _HALF:
+            raise RuntimeError(f"dtype must be bfloat16 or float16, got {dtype}")
     else:
         _, ps, vs = _check_pages(k_pages, v_pages)
         _require(vs == ps, "k_pages and v_pages must have the same strides")
         _require(dtype is None or dtype is k_pages.dtype, f"pages of {k_pages.dtype} are not read as {dtype}")
-        code, dim, ss, dtype = 0, k_pages.size(3), (0, 0), k_pages.dtype
-    pages, heads, page, _ = k_pages.shape
+        code, on, ss, dtype = 0, k_pages.get_device(), (0, 0), k_pages.dtype
+        pages, heads, page, dim = k_pages.shape
     idx, n, width, ld = _check_table(table)
-    _require(k_pages.get_device() == idx, f"table must be on {k_pages.device}")
+    if on != idx:
+        raise RuntimeError(f"table must be on {k_pages.device}")
     _i32("cu_rows", cu_rows, n + 1, idx)
     _i32("kv_lens", kv_lens, n, idx)
-    _require(rows >= 0, "rows must not be negative")
+    if rows < 0:
+        raise RuntimeError("rows must not be negative")
     if out is None:
         key = torch.empty((rows, heads, dim), dtype=dtype, device=k_pages.device)
         value = torch.empty_like(key)
@@ -448,7 +450,7 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     last request are left as they were."""
     lib = _lib.load()
     if k_scales is not None or v_scales is not None or k_pages.dtype in _CODES:
-        code, dim, ks, ss = _check_codes(k_pages, v_pages, k_scales, v_scales)
+        code, on, (pages, kv_heads, page, dim), ks, ss = _check_codes(k_pages, v_pages, k_scales, v_scales)
         dtype = _lib.half_code("query", query)
     else:
         dtype, ks, vs = _check_pages(k_pages, v_pages)
@@ -457,10 +459,10 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         if query.dtype is not k_pages.dtype:
             raise RuntimeError(f"query must be {k_pages.dtype} [rows, q_heads, dim] on {k_pages.device} with contiguous "
                                "channels")
-        code, dim, ss = 0, k_pages.size(3), (0, 0)
+        code, on, ss = 0, k_pages.get_device(), (0, 0)
+        pages, kv_heads, page, dim = k_pages.shape
     idx, n, width, ld = _check_table(table)
-    pages, kv_heads, page, _ = k_pages.shape
-    if k_pages.get_device() != idx:
+    if on != idx:
         raise RuntimeError(f"table must be on {k_pages.device}")
     if query.dim() != 3 or query.get_device() != idx or query.stride(2) != 1 or query.size(2) != dim:
         raise RuntimeError(f"query must be {query.dtype} [rows, q_heads, {dim}] on {k_pages.device} with contiguous "
