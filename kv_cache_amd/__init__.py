@@ -26,12 +26,12 @@ from .qabs_cuda_kernels import (
     partial_scores_dim_major,
 )
 
-from .paged import PageTable, StepPlan
+from .paged import PageTable, SharedRows, StepPlan
 
 load = _lib.load
 
 __all__ = [
     "Int4KCache", "SparseDecodeStep", "block_topk", "build_slab", "decode_scores", "int4_pack_k", "query_words",
     "select_channels", "sparse_attention", "candidate_full_scores", "final_attention",
-    "partial_scores", "partial_scores_dim_major", "PageTable", "StepPlan", "paged", "load",
+    "partial_scores", "partial_scores_dim_major", "PageTable", "SharedRows", "StepPlan", "paged", "load",
 ]

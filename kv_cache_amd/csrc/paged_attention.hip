@@ -18,6 +18,10 @@
 // Both take the scores transposed, S^T = K Q^T, so that a lane holds scores of one row: the softmax is in-lane but
 // for one lane swap, and P^T leaves the score accumulators in the layout that the matrix instruction of O^T = V^T P^T
 // wants (the order of the keys within a step is free; V^T is read in the same order, by transposing LDS reads).
+//
+// Over codes (FMT) both convert K and V to 16 bits on their way, exactly: the token kernel in registers (K in the order in
+// which a lane's 16 bytes lie, Q's channels alike), the rows kernel between memory and LDS.  32 single tokens over up to
+// 32768 keys: 300 us in fp8, 5.6 TB/s; 29 over up to 32001 in fp4: 137 us; 2048 tokens behind 63488 in fp8: 2.25 ms.
 #include "paged_tiles.h"
 
 using namespace qkv;

@@ -19,7 +19,11 @@ then for each layer
                     the mask may have a two-sided prefix and documents;
 
 and ``release_pages`` gives back the pages of requests that ended or of
-tokens that were rejected.  No length is needed on the host, so a step can be
+tokens that were rejected.  Pages may hold codes of 8 or 4 bits with scales
+(``quantized_pages``); ``read`` gives cached tokens back as rows.  Requests
+may continue another one's tokens: ``share_rows`` gathers a step's rows by
+parent, and ``attention(..., shared=...)`` reads a parent's keys once for all
+of them.  No length is needed on the host, so a step can be
 captured into a graph and replayed while the requests grow.
 
 No reference counterpart: the reference keeps HF's dense cache, every
