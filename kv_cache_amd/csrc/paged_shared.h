@@ -6,8 +6,8 @@
 // paged_tiles.h, and one launch does both kinds.  The tiles' keys are split into chunks of about the same length, so that
 // the launch's workgroups are as even as they can be; a (row, head)'s parts, its own and its parent's, are joined by a
 // second launch in their order.  Only tiles in one chunk of rows without a parent write the output themselves.
-// 64 requests behind 32768 tokens, up to 600 of their own, 32/8 heads: 67 us and 7.5 for the join (one call for each
-// request's keys would read 8.6 GB); twice the prefix takes 36 us more, the rate of a large library product.
+// 64 requests behind 32768 tokens, up to 600 of their own, 32/8 heads: 67 us and 7.5 for the join (843 us where every
+// request reads the prefix itself); twice the prefix takes 36 us more, the rate of a large library product.
 #pragma once
 
 #include "paged_tiles.h"

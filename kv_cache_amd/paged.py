@@ -286,7 +286,7 @@ def _check_codes(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales, v_scale
             or v_scales.shape != k_scales.shape or v_scales.stride() != ss or ss[3] != 1 or ss[2] != blocks):
         raise RuntimeError(f"k_scales and v_scales must be uint8 {[pages, heads, page, blocks]} on {k_pages.device} of "
                            "the same strides, a head's tokens without gaps")
-    return code, idx, (pages, heads, page, dim), ps, ss
+    return code, idx, (pages, heads, page, dim), ps, ss[:2]
 
 
 def append(key: torch.Tensor, value: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -341,7 +341,7 @@ def _append_codes(key, value, k_pages, v_pages, slots, k_scales, v_scales) -> No
             raise RuntimeError(f"{name} must be {key.dtype} [{rows}, {heads}, {dim}] on {k_pages.device} with "
                                "contiguous channels: key, value and slots have as many rows")
     # row and head strides of the rows, page, head and token strides of the pages, page and head strides of the scales
-    st = _lib.strides(*key.stride()[:2], *value.stride()[:2], *ps[:3], *ss[:2])
+    st = _lib.strides(*key.stride()[:2], *value.stride()[:2], *ps[:3], *ss)
     at = ctypes.addressof(st)
     guard = _lib.enter_device(idx)
     try:
@@ -377,7 +377,7 @@ def read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, cu_r
         _, ps, vs = _check_pages(k_pages, v_pages)
         _require(vs == ps, "k_pages and v_pages must have the same strides")
         _require(dtype is None or dtype is k_pages.dtype, f"pages of {k_pages.dtype} are not read as {dtype}")
-        code, on, ss, dtype = 0, k_pages.get_device(), (0, 0), k_pages.dtype
+        code, on, ss, dtype = 0, k_pages.get_device(), (0, 0), k_pages.dtype   # (no scales)
         pages, heads, page, dim = k_pages.shape
     idx, n, width, ld = _check_table(table)
     if on != idx:
@@ -394,7 +394,7 @@ def read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, cu_r
         for t in out:
             _require(t.shape == (rows, heads, dim) and t.dtype is dtype and t.get_device() == idx and t.stride(2) == 1,
                      f"out must be two {dtype} [{rows}, {heads}, {dim}] on {k_pages.device} with contiguous channels")
-    st = _lib.strides(*ps[:3], *ss[:2], *key.stride()[:2], *value.stride()[:2])
+    st = _lib.strides(*ps[:3], *ss, *key.stride()[:2], *value.stride()[:2])
     at = ctypes.addressof(st)
     guard = _lib.enter_device(idx)
     try:
@@ -463,7 +463,7 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         if query.dtype is not k_pages.dtype:
             raise RuntimeError(f"query must be {k_pages.dtype} [rows, q_heads, dim] on {k_pages.device} with contiguous "
                                "channels")
-        code, on, ss = 0, k_pages.get_device(), (0, 0)
+        code, on, ss = 0, k_pages.get_device(), ()
         pages, kv_heads, page, dim = k_pages.shape
     idx, n, width, ld = _check_table(table)
     if on != idx:
@@ -500,28 +500,33 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         _require(workspace.get_device() == idx and workspace.is_contiguous(),
                  f"workspace must be contiguous on cuda:{idx}")
         ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    slopes_ptr = None if slopes is None else slopes.data_ptr()
+    prefix_ptr = None if prefix_lens is None else prefix_lens.data_ptr()
+    first_ptr = None if first_keys is None else first_keys.data_ptr()
     # row and head strides of the query, page, head and token strides of the pages, row and head strides of out, page
     # and head strides of the scales
-    st = _lib.strides(*query.stride()[:2], *ks[:3], *out.stride()[:2], *ss[:2])
+    st = _lib.strides(*query.stride()[:2], *ks[:3], *out.stride()[:2], *ss)
     at = ctypes.addressof(st)
-    # what the three calls share, before and behind the pages' own
-    rest = (pages, page, table.data_ptr(), ld, width, n, cu_rows.data_ptr(), kv_lens.data_ptr(), rows, most, q_heads,
-            kv_heads, dim, scaling, softcap, None if slopes is None else slopes.data_ptr(),
-            None if prefix_lens is None else prefix_lens.data_ptr(),
-            None if first_keys is None else first_keys.data_ptr(), ws_ptr, ws_bytes, out.data_ptr(), at + 40, dtype)
     guard = _lib.enter_device(idx)
     try:
         if shared is not None:
-            rc = lib.qkv_paged_attention_shared(query.data_ptr(), at, k_pages.data_ptr(), v_pages.data_ptr(), at + 16,
-                                                _lib.ptr(k_scales), _lib.ptr(v_scales), at + 56, code,
-                                                shared.buffer.data_ptr(), *rest, _lib.stream_on(idx))
+            rc = lib.qkv_paged_attention_shared(
+                query.data_ptr(), at, k_pages.data_ptr(), v_pages.data_ptr(), at + 16, _lib.ptr(k_scales),
+                _lib.ptr(v_scales), at + 56, code, shared.buffer.data_ptr(), pages, page, table.data_ptr(), ld, width, n,
+                cu_rows.data_ptr(), kv_lens.data_ptr(), rows, most, q_heads, kv_heads, dim, scaling, softcap, slopes_ptr,
+                prefix_ptr, first_ptr, ws_ptr, ws_bytes, out.data_ptr(), at + 40, dtype, _lib.stream_on(idx))
         elif code:
-            rc = lib.qkv_paged_attention_codes(query.data_ptr(), at, k_pages.data_ptr(), v_pages.data_ptr(), at + 16,
-                                               k_scales.data_ptr(), v_scales.data_ptr(), at + 56, code, *rest,
-                                               _lib.stream_on(idx))
+            rc = lib.qkv_paged_attention_codes(
+                query.data_ptr(), at, k_pages.data_ptr(), v_pages.data_ptr(), at + 16, k_scales.data_ptr(),
+                v_scales.data_ptr(), at + 56, code, pages, page, table.data_ptr(), ld, width, n, cu_rows.data_ptr(),
+                kv_lens.data_ptr(), rows, most, q_heads, kv_heads, dim, scaling, softcap, slopes_ptr, prefix_ptr,
+                first_ptr, ws_ptr, ws_bytes, out.data_ptr(), at + 40, dtype, _lib.stream_on(idx))
         else:
-            rc = lib.qkv_paged_attention(query.data_ptr(), at, k_pages.data_ptr(), v_pages.data_ptr(), at + 16, *rest,
-                                         _lib.stream_on(idx))
+            rc = lib.qkv_paged_attention(
+                query.data_ptr(), at, k_pages.data_ptr(), v_pages.data_ptr(), at + 16, pages, page, table.data_ptr(), ld,
+                width, n, cu_rows.data_ptr(), kv_lens.data_ptr(), rows, most, q_heads, kv_heads, dim, scaling, softcap,
+                slopes_ptr, prefix_ptr, first_ptr, ws_ptr, ws_bytes, out.data_ptr(), at + 40, dtype,
+                _lib.stream_on(idx))
     finally:
         _lib.leave_device(guard)
     _lib.check(rc)

@@ -36,7 +36,8 @@ def _plan(parents, rows, kv, lens, total):
     return positions, heirs
 
 
-@pytest.mark.parametrize("requests,most,total", [(1, 3, 4), (2, 1, 2), (33, 1, 40), (64, 5, 400), (65, 3, 300), (1000, 2, 2500),
+@pytest.mark.parametrize("requests,most,total", [(1, 3, 4), (2, 1, 2), (33, 1, 40), (64, 5, 400), (65, 3, 300), (255, 1, 200),
+                                                 (257, 2, 300), (400, 2, 900), (512, 1, 600), (512, 20, 9000), (513, 1, 600), (1000, 2, 2500),
                                                  (1025, 1, 1200), (4096, 1, 4096), (4095, 3, 13000), (7, 3000, 22000)])
 def test_share_rows(requests, most, total):
     rng = random.Random(requests)
