@@ -6,7 +6,7 @@
 // paged_tiles.h, and one launch does both kinds.  The tiles' keys are split into chunks of about the same length, so that
 // the launch's workgroups are as even as they can be; a (row, head)'s parts, its own and its parent's, are joined by a
 // second launch in their order.  Only tiles in one chunk of rows without a parent write the output themselves.
-// 64 requests behind 32768 tokens, up to 600 of their own, 32/8 heads: 67 us and 7.5 for the join (843 us where every
+// 64 requests behind 32768 tokens, up to 600 of their own, 32/8 heads: 67 us and 7 for the join (843 us where every
 // request reads the prefix itself); twice the prefix takes 36 us more, the rate of a large library product.
 #pragma once
 
@@ -331,8 +331,10 @@ int launch_shared(const PagedArgs& a, const SharedShape& s, hipStream_t st, cons
   if (s.sets == 1) paged_shared_kernel<D, F16, FORM, FMT, 1><<<n, 256, 0, st>>>(a, s.c);
   else paged_shared_kernel<D, F16, FORM, FMT, 2><<<n, 256, 0, st>>>(a, s.c);
   const int64_t pairs = static_cast<int64_t>(a.rows) * a.kv_heads * a.group;
-  // few (row, head)s, and so many parts of each: one a workgroup
-  if (pairs <= 16384) paged_shared_join_kernel<D, F16, 1><<<static_cast<unsigned>(pairs), 256, 0, st>>>(a, s.c);
+  // The fewer (row, head)s, the more parts each has: few have a workgroup each, more four a workgroup (51 requests' 7
+  // drafts: 99 us in all, 106 with one), many, of prompts, eight.
+  if (pairs <= 1024) paged_shared_join_kernel<D, F16, 1><<<static_cast<unsigned>(pairs), 256, 0, st>>>(a, s.c);
+  else if (pairs <= 16384) paged_shared_join_kernel<D, F16, 4><<<static_cast<unsigned>(cdiv(pairs, 4)), 256, 0, st>>>(a, s.c);
   else paged_shared_join_kernel<D, F16, 8><<<static_cast<unsigned>(cdiv(pairs, 8)), 256, 0, st>>>(a, s.c);
   return check_launch(what);
 }
