@@ -50,7 +50,7 @@ __device__ __forceinline__ int locate_shared(const PagedArgs& a, const SharedArg
     }
     return s;
   };
-  // one more or less is as good: what a chunk holds follows from their number
+  // one more or less is as good: what a chunk holds follows from their number (below)
   auto splits_of = [&](int keys) {
     return keys > w.chunk ? static_cast<int>(static_cast<float>(keys - 1) * __builtin_amdgcn_rcpf(static_cast<float>(w.chunk))) + 1 : 1;
   };
@@ -197,7 +197,8 @@ __device__ __forceinline__ int locate_shared(const PagedArgs& a, const SharedArg
   w.heirs = kind == 0;
   w.alone = !w.heirs && a.before[w.b] <= 0;
   const int units = units_of(w.n_rows);
-  // as many keys for each of the tile's chunks
+  // as many keys for each of the tile's chunks, all of them in one
+  w.chunk = w.kv;
   if (w.n_split > 1) w.chunk = __builtin_amdgcn_readfirstlane(((w.kv + w.n_split - 1) / w.n_split + kTile - 1) & -kTile);
   const int rest = __builtin_amdgcn_readfirstlane(at / a.kv_heads);
   w.head = at - rest * a.kv_heads;

@@ -413,3 +413,16 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for w, many in zip(want, got):
         assert all(torch.equal(w, y) for y in many)
+
+
+@pytest.mark.parametrize("unit", [2624, 3008])
+def test_a_chunk_and_one_key(unit):
+    """A request of one key more than a chunk whose reciprocal, rounded, times the chunk is below one: 512 workgroups of
+    `unit` keys, as 31 requests of two chunks and one of a chunk and that key, 8 KV heads."""
+    kv = [2 * unit] * 31 + [unit + 1]
+    c = _case(kv, [1] * 32, 8, 8, 64, 64, "bf16", seed=60)
+    for b in range(32):     # the last key's value shows in the output
+        c["v_pages"][int(c["table"][b, (kv[b] - 1) // 64]), :, (kv[b] - 1) % 64] = 512.0
+    plan = paged.share_rows(_i32([-1] * 32), c["cu_rows"], c["kv_lens"], c["kv_lens"], 32)
+    want, tol = _reference(c)
+    _within(paged.attention(**c, shared=plan, max_rows=1), want, tol)
