@@ -368,6 +368,10 @@ class _PagedState:
         if length - n != (self.length if first else self.length - self.new):
             raise RuntimeError(f"the layers of a PagedCache step together: a layer steps from {length - n} columns to "
                                f"{length}, the cache holds {self.length}")
+        if self.parents is not None and batch * (self.copies + 1) != self.parents.numel() * self.copies:
+            requests = self.parents.numel()
+            raise RuntimeError(f"the PagedCache was repeated for {requests - requests // (self.copies + 1)} sequences, "
+                               f"this step has {batch}")
         if first:
             self.masks = []
             if self.length == 0:
@@ -391,9 +395,6 @@ class _PagedState:
             self.plan = self.table.step(new, batch * n, padded=n)
         else:   # the parents, behind their children in the table, get no tokens, and rows that the model does not have
             requests = self.parents.numel()
-            if batch * (self.copies + 1) != requests * self.copies:
-                raise RuntimeError(f"the PagedCache was repeated for {requests - requests // (self.copies + 1)} sequences, "
-                                   f"this step has {batch}")
             plan = self.table.step(torch.cat((new, new.new_zeros(requests - batch))), requests * n, padded=n)
             self.shared = paged.share_rows(self.parents, plan.cu_rows, plan.kv_lens, self.table.lens, batch * n)
             self.plan = plan._replace(slots=plan.slots[:batch * n], positions=self.shared.positions)

@@ -117,8 +117,10 @@ def test_refusals(plain):
         cache.batch_repeat_interleave(2)
     with pytest.raises(RuntimeError, match="repeated for 4 sequences, this step has 2"):
         _columns(model, "paged", cache, ids, None, [1], 8)
+    with pytest.raises(RuntimeError, match="repeated for 4 sequences, this step has 2"):
+        _columns(model, "paged", cache, ids, _left_padded([9, 8], 9), [1], 8)      # with a mask too
     rows = ids.repeat_interleave(2, 0)
-    got = _columns(model, "paged", cache, rows, None, [1, 3], 8)      # the refused step left it as it was
+    got = _columns(model, "paged", cache, rows, None, [1, 3], 8)      # the refused steps left it as it was
     want = _columns(model, "sdpa", _dense(model), rows, None, [12])[:, 8:]
     assert (got - want).abs().max() <= 1e-4 * want.abs().max()
     layer = hf.PagedCacheLayer(hf._PagedState(32, 16))
