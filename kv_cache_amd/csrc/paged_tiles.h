@@ -868,12 +868,14 @@ __device__ __forceinline__ void rows_body(const PagedArgs& a, const PagedClass& 
     // workgroup for 8-byte stores to 32 rows at a time
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     uint16_t* mine = stage0 + wave * 32 * D;
+    int own = l32;
+    asm("" : "+v"(own));   // own * D is not l32 * D of the loop, which would be kept, and spilled, for it
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const float x[4] = {o[d][4 * q] * inv, o[d][4 * q + 1] * inv, o[d][4 * q + 2] * inv, o[d][4 * q + 3] * inv};
-        *reinterpret_cast<u32x2_t*>(mine + l32 * D + 8 * (unit_at<D, FMT>(4 * d + q) ^ (l32 & (UR - 1))) + 4 * half) = pack4_half<F16>(x);
+        *reinterpret_cast<u32x2_t*>(mine + own * D + 8 * (unit_at<D, FMT>(4 * d + q) ^ (own & (UR - 1))) + 4 * half) = pack4_half<F16>(x);
       }
 #pragma unroll
     for (int i = 0; i < 32 * UR / 64; ++i) {
