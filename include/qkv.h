@@ -1058,7 +1058,10 @@ int qkv_paged_share(const int32_t* parents, const int32_t* cu_rows, const int32_
                     int64_t requests, int64_t rows, int32_t* shared, void* stream);
 
 /* Bytes of workspace for qkv_paged_attention_shared; -1 for sizes it does not
- * take. */
+ * take: what qkv_paged_attention does not, more than 4096 requests or 2^20
+ * rows, 2^26 rows times query heads or more.  It holds partial outputs in 32
+ * bits of every (row, query head), twice: 32 KB a row with 32 heads of 128
+ * channels. */
 int64_t qkv_paged_attention_shared_workspace_bytes(int64_t rows, int64_t max_rows, int64_t requests, int64_t width,
                                                    int64_t page, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
 

@@ -326,6 +326,13 @@ int64_t shared_bytes(const SharedShape& s, int64_t rows, int64_t kv_heads, int64
   return s.units * kPartUnit * 4 * (head_dim + 2) + 16 * rows * kv_heads;
 }
 
+// What a call may have: a grid has less than 2^32 threads, and the parts' rows are counted in 31 bits.
+constexpr int64_t kMaxPairs = 1 << 26;   // (row, query head)s
+bool good_shared(const SharedShape& s, int64_t rows, int64_t requests, int64_t q_heads) {
+  return requests <= kMaxPlanned && rows <= kMaxPlannedRows && s.items < (1 << 24) && s.units < (1 << 27) &&
+         rows * q_heads < kMaxPairs;
+}
+
 template <int D, bool F16, bool FORM, int FMT>
 int launch_shared(const PagedArgs& a, const SharedShape& s, hipStream_t st, const char* what) {
   const unsigned n = static_cast<unsigned>(s.items);
@@ -347,10 +354,11 @@ int shared_call(const PagedCall& c, const int32_t* plan, const char* what) {
   if (const int rc = make_args(c, what, FMT, &f16, &a)) return rc;
   if (!plan) return fail(QKV_ERR_INVALID, "%s: null pointer", what);
   SharedShape s = shared_shape_of(c.rows, c.max_rows, c.requests, c.width * c.page, c.kv_heads, a.group);
-  // a grid has less than 2^32 threads, and the parts' rows are counted in 31 bits
-  if (c.requests > kMaxPlanned || c.rows > kMaxPlannedRows || s.items >= (1 << 24) || s.units >= (1 << 27) ||
-      c.rows * c.q_heads >= (1 << 26))
-    return fail(QKV_ERR_UNSUPPORTED, "%s: too many rows or requests", what);
+  if (!good_shared(s, c.rows, c.requests, c.q_heads))
+    return fail(QKV_ERR_UNSUPPORTED, "%s: too many rows or requests (at most %d requests and %lld rows, and fewer than %lld "
+                "rows times query heads), got %lld requests, %lld rows, %lld heads", what, kMaxPlanned,
+                static_cast<long long>(kMaxPlannedRows), static_cast<long long>(kMaxPairs), static_cast<long long>(c.requests),
+                static_cast<long long>(c.rows), static_cast<long long>(c.q_heads));
   const int64_t need = shared_bytes(s, c.rows, c.kv_heads, c.head_dim);
   if (c.rows > 0 && (!c.workspace || c.workspace_bytes < need || !aligned(c.workspace, 16)))
     return fail(QKV_ERR_INVALID, "%s: workspace must be 16-byte aligned and hold %lld bytes", what,

@@ -8,7 +8,7 @@ QKV_EXPORT int64_t qkv_paged_attention_shared_workspace_bytes(int64_t rows, int6
                                                               int64_t kv_heads, int64_t head_dim) {
   if (!good_sizes(rows, requests, width, page, q_heads, kv_heads, head_dim)) return -1;
   const SharedShape s = shared_shape_of(rows, max_rows, requests, width * page, kv_heads, q_heads / kv_heads);
-  return shared_bytes(s, rows, kv_heads, head_dim);
+  return good_shared(s, rows, requests, q_heads) ? shared_bytes(s, rows, kv_heads, head_dim) : -1;
 }
 
 QKV_EXPORT int qkv_paged_attention_shared(const void* query, const int64_t* q_strides, const void* k_pages,
