@@ -531,6 +531,9 @@ class PagedCacheLayer:
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args, **kwargs):
         self.state.check_closed()
+        if self.copies != self.state.copies:   # its pages would not hold what the table gives out
+            raise RuntimeError("layers of this PagedCache were not repeated with the others: call batch_repeat_interleave on "
+                               "the cache, and reset() it after a call that failed")
         n = key_states.size(-2)
         if self.length + n > self.state.capacity:
             raise RuntimeError(f"Paged cache capacity {self.state.capacity} exceeded ({self.length + n} tokens)")
