@@ -420,6 +420,14 @@ class _PagedState:
             self.real = self.real.repeat_interleave(copies, 0)
         self.table, self.copies = table, copies
 
+    def check_repeat(self, copies: int, more: int) -> None:
+        """Raises where the table of ``repeat`` would be larger than a step
+        takes."""
+        requests, pages = self.table.lens.numel() * (copies + 1), self.table.pages + more
+        if requests > 4096 or pages > 1 << 20:
+            raise RuntimeError(f"a PagedCache takes 4096 sequences, prompts among them, and 2^20 pages: {copies} of each of "
+                               f"{self.table.lens.numel()} prompts make {requests} and {pages}")
+
     def more_pages(self, copies: int) -> int:
         """Pages that ``copies`` continuations of each of the table's sequences
         need besides the free ones."""
@@ -573,6 +581,8 @@ class PagedCacheLayer:
         if self.length == 0 or state.length != self.length or self.copies != 1 or state.copies not in (1, repeats):
             raise RuntimeError("PagedCacheLayer is repeated once, after a step of all layers")
         more = state.more_pages(repeats)
+        if state.copies == 1:   # (the table has grown otherwise)
+            state.check_repeat(repeats, more)
         if state.copies == 1:
             state.repeat(repeats)
         grown = lambda x: torch.cat((x.view(torch.uint8), x.new_empty((more, *x.shape[1:])).view(torch.uint8))).view(x.dtype)  # noqa: E731

@@ -27,3 +27,28 @@ def test_layers_repeated_apart_are_refused(plain):  # noqa: F811
     got = torch.cat((got.repeat_interleave(3, 0), _columns(model, "paged", cache, rows, None, [1, 3], 8)), 1)
     want = _columns(model, "sdpa", _dense(model), rows, None, [8, 4])
     assert (got - want).abs().max() <= 1e-4 * want.abs().max()
+
+
+@pytest.mark.parametrize("prompts,capacity,repeats", [(1, 32, 4096), (2, 32, 2048), (1, 1 << 14, 1100)])
+def test_more_than_a_step_takes_is_refused(plain, prompts, capacity, repeats):  # noqa: F811
+    """4096 sequences, prompts among them, or 2^20 pages: refused before the cache changes."""
+    model, ids = _model(), _tokens(prompts, 10, 7)
+    cache = hf.PagedCache(capacity=capacity, page=16)
+    got = _columns(model, "paged", cache, ids, None, [8])
+    pool, state = cache.layers[0].k_pages.shape[0], cache.layers[0].state
+    with pytest.raises(RuntimeError, match="4096 sequences, prompts among them, and 2\\^20 pages"):
+        cache.batch_repeat_interleave(repeats)
+    assert state.copies == 1 and state.parents is None
+    assert all(layer.copies == 1 and layer.k_pages.shape[0] == pool == state.table.pages for layer in cache.layers)
+    got = torch.cat((got, _columns(model, "paged", cache, ids, None, [2], 8)), 1)      # it goes on as it was
+    want = _columns(model, "sdpa", _dense(model), ids, None, [10])
+    assert (got - want).abs().max() <= 1e-4 * want.abs().max()
+    assert state.more_pages(repeats) > 0
+
+
+def test_as_many_as_a_step_takes(plain):  # noqa: F811
+    model, ids = _model(), _tokens(1, 9, 8)
+    cache = hf.PagedCache(capacity=16, page=16)
+    _columns(model, "paged", cache, ids, None, [8])
+    cache.batch_repeat_interleave(4095)
+    assert cache.layers[0].state.table.lens.numel() == 4096
