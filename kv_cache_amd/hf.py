@@ -66,6 +66,7 @@ of one prompt): they share its pages, which attention reads once for all.
 
 from __future__ import annotations
 
+import copy
 import functools
 import math
 import weakref
@@ -352,6 +353,7 @@ class _PagedState:
         self.open = False        # an update's columns have not been attended over yet
         self.copies = 1          # sequences that continue each of the first prompts (``repeat``)
         self.parents = self.shared = None   # of every request of the table; the step's rows by parent
+        self.children = None     # the table without the parents, where there are some
 
     def check_closed(self) -> None:
         """Raises if the attention function did not take an earlier update:
@@ -393,11 +395,13 @@ class _PagedState:
             new = self.real[:, length - n:length].sum(-1, dtype=torch.int32)
         if self.parents is None:
             self.plan = self.table.step(new, batch * n, padded=n)
-        else:   # the parents, behind their children in the table, get no tokens, and rows that the model does not have
-            requests = self.parents.numel()
-            plan = self.table.step(torch.cat((new, new.new_zeros(requests - batch))), requests * n, padded=n)
+        else:   # the parents, behind their children in the table, have no rows
+            plan = self.children.step(new, batch * n, padded=n)
+            parents = self.parents.numel() - batch
+            plan = plan._replace(cu_rows=torch.cat((plan.cu_rows, plan.cu_rows[-1:].expand(parents))),
+                                 kv_lens=torch.cat((plan.kv_lens, self.table.lens[batch:])))
             self.shared = paged.share_rows(self.parents, plan.cu_rows, plan.kv_lens, self.table.lens, batch * n)
-            self.plan = plan._replace(slots=plan.slots[:batch * n], positions=self.shared.positions)
+            self.plan = plan._replace(positions=self.shared.positions)
         self.length, self.new = length, n
         return self.plan
 
@@ -419,6 +423,8 @@ class _PagedState:
         if self.real is not None:
             self.real = self.real.repeat_interleave(copies, 0)
         self.table, self.copies = table, copies
+        self.children = copy.copy(table)   # their rows of the same table
+        self.children.table, self.children.lens = table.table[:batch * copies], table.lens[:batch * copies]
 
     def check_repeat(self, copies: int, more: int) -> None:
         """Raises where the table of ``repeat`` would be larger than a step
@@ -481,7 +487,7 @@ class _PagedState:
         if self.table is not None and self.length:
             self.table.release(torch.zeros_like(self.table.lens))
         if self.parents is not None:   # a table for the next batch
-            self.table = self.parents = self.shared = None
+            self.table = self.parents = self.shared = self.children = None
         self.length, self.real, self.masks, self.open, self.copies = 0, None, [], False, 1
 
 

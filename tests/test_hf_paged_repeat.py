@@ -5,7 +5,7 @@ adapter's other CPU tests."""
 import pytest
 import torch
 
-from kv_cache_amd import hf
+from kv_cache_amd import hf, paged
 from test_hf_paged import _model, _tokens
 from test_hf_paged_shared import _columns, _dense, plain  # noqa: F401
 
@@ -52,3 +52,23 @@ def test_as_many_as_a_step_takes(plain):  # noqa: F811
     _columns(model, "paged", cache, ids, None, [8])
     cache.batch_repeat_interleave(4095)
     assert cache.layers[0].state.table.lens.numel() == 4096
+
+
+@pytest.mark.parametrize("prompts,copies", [(1, 3), (3, 2)])
+def test_prompts_have_no_rows_in_a_step(plain, monkeypatch, prompts, copies):  # noqa: F811
+    """A step asks for the rows of the model's batch alone, so that 2^20 of them fit."""
+    model, ids = _model(), _tokens(prompts, 20, 9)
+    cache = hf.PagedCache(capacity=48, page=16)
+    _columns(model, "paged", cache, ids, None, [8])
+    cache.batch_repeat_interleave(copies)
+    asked, made = [], []
+    step, share = paged.PageTable.step, paged.share_rows
+    monkeypatch.setattr(paged.PageTable, "step", lambda t, new, rows, **kw: asked.append((new.numel(), rows)) or step(t, new, rows, **kw))
+    monkeypatch.setattr(paged, "share_rows", lambda parents, cu, kv, lens, rows: made.append((cu.tolist(), kv.tolist(), lens.tolist(), rows))
+                        or share(parents, cu, kv, lens, rows))
+    batch = prompts * copies
+    _columns(model, "paged", cache, ids.repeat_interleave(copies, 0), None, [5, 1], 8)
+    assert asked == [(batch, 5 * batch), (batch, batch)]
+    for (cu, kv, lens, rows), n, own in zip(made, (5, 1), (5, 6)):
+        assert cu == [n * b for b in range(batch + 1)] + [n * batch] * prompts and rows == n * batch
+        assert kv == lens == [own] * batch + [8] * prompts
