@@ -152,12 +152,11 @@ __global__ __launch_bounds__(256) void read_kernel(RowsOf r, Rows16 x, CodePages
     s_slot[tid] = slot;
   }
   __syncthreads();
-  const int heads = r.units_row / r.units_head;
   for (int u = tid; u < n * r.units_row; u += 256) {
     const int i = u / r.units_row, in_row = u - i * r.units_row;
     const int head = in_row / r.units_head, c = 8 * (in_row - head * r.units_head);
     const int64_t slot = s_slot[i], row = row0 + i;
-    if (slot == -2 || head >= heads) continue;
+    if (slot == -2) continue;
     u32x4_t k{0u, 0u, 0u, 0u}, v = k;
     if (slot >= 0) {
       const int64_t id = slot >> r.shift, at = slot & ((1 << r.shift) - 1);
