@@ -1060,7 +1060,7 @@ int qkv_paged_share(const int32_t* parents, const int32_t* cu_rows, const int32_
 /* Bytes of workspace for qkv_paged_attention_shared; -1 for sizes it does not
  * take: what qkv_paged_attention does not, more than 4096 requests or 2^20
  * rows, 2^26 rows times query heads or more.  It holds partial outputs in 32
- * bits of every (row, query head), twice: 32 KB a row with 32 heads of 128
+ * bits of every (row, query head), twice: 33 KB a row with 32 heads of 128
  * channels. */
 int64_t qkv_paged_attention_shared_workspace_bytes(int64_t rows, int64_t max_rows, int64_t requests, int64_t width,
                                                    int64_t page, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
@@ -1071,7 +1071,8 @@ int64_t qkv_paged_attention_shared_workspace_bytes(int64_t rows, int64_t max_row
  * kv_lens[b] - (cu_rows[b+1] - cu_rows[b]) + i of the parent's tokens and its
  * own behind them, and sees the keys first_keys[row] <= j < max(p + 1,
  * prefix_lens[b]) of them; rows before its own first token, and rows that see
- * none, get zeros.  A parent's keys are read once for all rows behind it. */
+ * none, get zeros.  A parent's keys are read for all rows behind it together,
+ * once for every 128 (row, query head)s of a KV head. */
 int qkv_paged_attention_shared(const void* query, const int64_t* q_strides, const void* k_pages, const void* v_pages,
                                const int64_t* page_strides, const void* k_scales, const void* v_scales,
                                const int64_t* scale_strides, int code, const int32_t* shared, int64_t pages,

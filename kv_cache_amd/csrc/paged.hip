@@ -325,7 +325,7 @@ __global__ __launch_bounds__(kPlanThreads) void share_kernel(ShareArgs a) {
 }
 
 // The same for at most kCounted requests: an heir's place is the sum of the tokens of all requests before its own in that
-// order, added up one by one; no sort, and two barriers (64 requests: 3 us, 5 to 9 sorted).
+// order, added up one by one; no sort, and two barriers (5 requests: 2.3 us, 65: 3.7; 512 take 18, as 513 do sorted).
 constexpr int kCounted = 512;
 template <bool WITH_ROWS>
 __global__ __launch_bounds__(kPlanThreads) void share_few_kernel(ShareArgs a) {

@@ -10,7 +10,7 @@
 // keys are split over several workgroups where there are few tiles.  How far is decided on the GPU from the lengths
 // (locate, below): no length is needed on the host.  Two kernels: `rows` for tiles of 128 (token, head) rows, whose
 // 4 waves hold 32 rows each and share tiles of 64 keys in LDS, bound by the matrix cores (2048 tokens behind 63488, 32/8
-// heads: 2.09 ms, 1036 TFLOP/s, 83% of what a large library product reaches); `token` for requests of at most 16 or 32
+// heads: 2.09 ms, 1036 TFLOP/s, 77 to 83% of a large library product's rate); `token` for requests of at most 16 or 32
 // (token, head) rows, whose 4 waves walk different keys of the same rows, bound by memory (32 requests of up to 32768
 // keys: 530 us, 6.14 TB/s).  Requests of 17 to 32 rows in the rows kernel leave three of its waves idle (7 drafts of 5
 // tokens, 4 heads: 57 us, 47 in the token kernel).
@@ -21,7 +21,7 @@
 //
 // Over codes (FMT) both convert K and V to 16 bits on their way, exactly: the token kernel in registers (K in the order in
 // which a lane's 16 bytes lie, Q's channels alike), the rows kernel between memory and LDS.  32 single tokens over up to
-// 32768 keys: 300 us in fp8, 5.6 TB/s; 29 over up to 32001 in fp4: 137 us; 2048 tokens behind 63488 in fp8: 2.25 ms.
+// 32768 keys: 300 us in fp8, 5.6 TB/s; 29 over up to 32001 in fp4: 137 us; 2048 tokens behind 63488 in fp8: 2.22 to 2.36 ms by card.
 #include "paged_tiles.h"
 
 using namespace qkv;

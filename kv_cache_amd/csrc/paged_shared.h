@@ -1,5 +1,5 @@
-// Attention of requests that continue another request's tokens, their parent's: each parent's keys are read once for all
-// rows behind it.
+// Attention of requests that continue another request's tokens, their parent's: each parent's keys are read for all rows
+// behind it together, once for every tile of 128 (row, query head)s.
 //
 // A row sees its parent's tokens and then its own request's up to itself.  A tile holds either rows of one request over
 // its own keys, or heirs of one parent, of whatever requests, over the parent's; tiles are those of the two bodies of
@@ -75,8 +75,8 @@ __device__ __forceinline__ int locate_shared(const PagedArgs& a, const SharedArg
     }
     return sum * a.kv_heads;
   };
-  // One round of chunks where one comes out, up to a fifth longer than the work's share (64 requests behind 32768 keys: 90
-  // us, 102 in two rounds), else two.
+  // One round of chunks where one comes out, up to a fifth longer than the work's share (64 requests behind 32768 keys: 82
+  // us in all, 92 in two rounds), else two.
   auto set_chunk = [&](float per, auto&& slots) {
     for (int i = 0; i < 4; ++i) {
       w.chunk = round_up(per * (1.0f + 0.0667f * i));

@@ -61,7 +61,8 @@ other than causal with left padding and the layer's window raises.
 
 ``PagedCache(..., quantize="fp8")`` (or "fp4") keeps the pages as codes.  After a
 prompt, ``cache.batch_repeat_interleave(n)`` makes n sequences of each (samples
-of one prompt): they share its pages, which attention reads once for all.
+of one prompt): they share its pages, which attention reads for all of them
+together.
 """
 
 from __future__ import annotations
@@ -577,7 +578,9 @@ class PagedCacheLayer:
     def batch_repeat_interleave(self, repeats: int) -> None:
         """Every sequence becomes ``repeats`` that share its pages: what they
         add goes to pages of their own, and attention reads the shared ones
-        once for all of them.  Once after a prompt; not again before reset."""
+        for all of them together.  Once after a prompt; not again before
+        reset.  The layer's pages grow by a copy: for a moment they exist
+        twice."""
         state = self.state
         if repeats < 1:
             raise RuntimeError(f"repeats must be positive, got {repeats}")

@@ -22,8 +22,8 @@ and ``release_pages`` gives back the pages of requests that ended or of
 tokens that were rejected.  Pages may hold codes of 8 or 4 bits with scales
 (``quantized_pages``); ``read`` gives cached tokens back as rows.  Requests
 may continue another one's tokens: ``share_rows`` gathers a step's rows by
-parent, and ``attention(..., shared=...)`` reads a parent's keys once for all
-of them.  No length is needed on the host, so a step can be
+parent, and ``attention(..., shared=...)`` reads a parent's keys for all of
+them together.  No length is needed on the host, so a step can be
 captured into a graph and replayed while the requests grow.
 
 No reference counterpart: the reference keeps HF's dense cache, every
@@ -361,7 +361,7 @@ def read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, cu_r
     """K and V of cached tokens, [rows, Hkv, D] each: row i of request b is
     the token at kv_lens[b] - (cu_rows[b + 1] - cu_rows[b]) + i, so that
     cu_rows = the sums of kv_lens reads whole requests; zeros where a request
-    has no token.  Quantised pages give ``dtype`` (bf16 if not said), which
+    has no token.  Channels are a multiple of 32.  Quantised pages give ``dtype`` (bf16 if not said), which
     holds what they stand for without a rounding (fp16 below 2^-14 with fewer
     bits, and infinities past 65504); others their own.  Rows of ``out`` (two
     tensors, any row and head strides of 16 bytes) behind the last request are
@@ -448,7 +448,10 @@ def attention(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     p = n + kv_lens[b] - (cu_rows[b + 1] - cu_rows[b]) + i of the parent's
     tokens and its own behind them, first_keys and prefix_lens count from the
     parent's first, and rows before a request's own first token get zeros.  A
-    parent's keys are read once for all rows behind it.
+    parent's keys are read for all rows behind it together, once for every 128
+    (row, query head)s of a KV head.  The workspace then holds partial outputs
+    of every (row, query head), about 33 KB a row with 32 heads of 128
+    channels; rows times query heads stay below 2^26.
 
     Returns [rows, Hq, D] in the query's dtype; rows of ``out`` behind the
     last request are left as they were."""
