@@ -143,3 +143,9 @@ def test_a_captured_step_of_many_requests():
     k = c["kv_lens"].tolist()
     whole, _ = _whole(c, [-1] + [0] * (n - 1), k)
     _within(out, *_reference(whole))
+
+
+@pytest.mark.parametrize("hq,hkv,dim,kind", [(64, 1, 64, "none"), (128, 1, 128, "fp8"), (16, 16, 64, "fp4"), (33, 1, 128, "none")])
+def test_heads_of_a_kv_head(hq, hkv, dim, kind):
+    # more heads a KV head than a token tile has rows; none shared
+    _check([-1, 0, 0, 5, 0, -1], [700, 9, 40, 33, 1, 90], [0, 1, 7, 2, 1, 3], hq, hkv, dim, 16, "bf16", kind, seed=75)
